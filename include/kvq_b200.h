@@ -342,6 +342,138 @@ const char* kvq_last_error(void);
 /* KVQ_ABI_VERSION of the loaded library. */
 int kvq_abi_version(void);
 
+/*
+ * The paged 4-bit cache: the same packed rows, held in pages that the requests
+ * of a batch take and give back, for steps that mix requests of any length
+ * with one or many new tokens each. No reference counterpart (the reference's
+ * cache is one padded buffer per sequence).
+ *
+ * A pool half (K or V) is a kvq_packed: words uint32 [pages, n_kv_heads,
+ * page_size, head_dim/8], scales and biases dtype [pages, n_kv_heads,
+ * page_size, head_dim/group_size], contiguous and 16-byte aligned; page_size
+ * is 16, 32, 64 or 128. Slot s is position s % page_size of page s /
+ * page_size. Request b's position p is in page block_tables[b * width + p /
+ * page_size]. A batch has 1 to 4096 requests (rows).
+ */
+typedef struct kvq_packed {
+    const uint32_t* words;
+    const void* scales;
+    const void* biases;
+} kvq_packed;
+
+/*
+ * Tables, slots and offsets of a step from the requests' lengths.
+ *
+ * kvq_paged_tables: request b holds lens[b] positions and brings step[b] new
+ * tokens (negative counts as 0). The pages it lacks are taken from the top of
+ * the stack free_pages[0 .. *n_free), requests in row order, and written into
+ * its row of block_tables; cu_new [rows + 1] are the running sums of step, and
+ * token i of the step gets slots[i] and positions[i]; entries past the last
+ * token are -1 and 0, up to max_tokens. lens_out and n_free_out are the
+ * lengths and the stack's height after the step. A step that does not fit
+ * takes nothing: *status has bit 1 when the stack holds too few pages, 2 when
+ * a request outgrows its row of the tables, 4 when there are more than
+ * max_tokens tokens, and then cu_new is 0, every slot -1, lens_out = lens and
+ * n_free_out = *n_free.
+ *
+ * kvq_paged_truncate: request b keeps min(lens[b], step[b]) positions; the
+ * pages behind them go on the stack (rows in order, each row's in table
+ * order; what would pass `pool` is dropped), lens_out and n_free_out likewise.
+ * cu_new, slots, positions and status are not used. The rows' table entries
+ * are left as they are.
+ *
+ * Inputs are read while outputs are written: an output that overlaps lens,
+ * step or n_free is refused.
+ */
+typedef struct kvq_tables {
+    const int32_t* lens;      /* [rows]                                        */
+    const int32_t* step;      /* [rows] new tokens, or positions to keep       */
+    int32_t* block_tables;    /* [rows, width]                                 */
+    int32_t* free_pages;      /* [pool] page ids                               */
+    const int32_t* n_free;    /* [1]                                           */
+    int32_t* cu_new;          /* [rows + 1]                                    */
+    int64_t* slots;           /* [max_tokens]                                  */
+    int32_t* positions;       /* [max_tokens]                                  */
+    int32_t* lens_out;        /* [rows]                                        */
+    int32_t* n_free_out;      /* [1]                                           */
+    int32_t* status;          /* [1]                                           */
+    uint32_t rows;
+    uint32_t width;           /* entries per row of block_tables               */
+    uint32_t pool;            /* entries of free_pages                         */
+    uint32_t page_size;
+    uint32_t max_tokens;
+} kvq_tables;
+int kvq_paged_tables(const kvq_tables* a, void* stream);
+int kvq_paged_truncate(const kvq_tables* a, void* stream);
+
+/*
+ * Rows by slot. kvq_paged_append quantizes keys and values [tokens,
+ * n_kv_heads, head_dim] (dtype; strides in elements, head_dim contiguous) into
+ * their slots, bit for bit as kvq_quantize does. kvq_paged_gather writes the
+ * slots' values scale * code + bias into keys and values (contiguous,
+ * out_dtype: the cache's dtype or KVQ_F32). A slot below 0 or past the pool is
+ * not written, and reads as zeros. Two tokens of one append must not name the
+ * same slot (the row would hold a mixture of both).
+ */
+typedef struct kvq_paged_rows {
+    kvq_packed k, v;
+    const void* keys;
+    const void* values;
+    const int64_t* slots;     /* [tokens]                                      */
+    uint64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    uint32_t tokens;
+    uint32_t n_kv_heads;
+    uint32_t head_dim;        /* 64 or 128                                     */
+    uint32_t group_size;      /* 32, 64 or 128; divides head_dim               */
+    uint32_t pages;
+    uint32_t page_size;
+    uint32_t dtype;
+    uint32_t out_dtype;
+} kvq_paged_rows;
+int kvq_paged_append(const kvq_paged_rows* a, void* stream);
+int kvq_paged_gather(const kvq_paged_rows* a, void* stream);
+
+/*
+ * The step's attention. Request b brings the tokens cu_new[b] .. cu_new[b+1)
+ * of q, new_k and new_v; its i-th token sees the ctx_lens[b] positions cached
+ * before the step (dequantized from the pages) and the step's own keys and
+ * values 0..i of the request at full precision -- for one new token, the step
+ * of kvq_decode. out [tokens, n_heads, head_dim] dtype, contiguous. Rows of
+ * `out` behind the last request's tokens are left as they were.
+ *
+ * max_ctx bounds ctx_lens and max_new the new tokens of a request (longer ones
+ * are cut to it); the launch is sized by them, so a captured step serves every
+ * batch within them. Pages are read up to ctx_lens only. A page id outside
+ * the pool is never dereferenced: the rows that would read it come out NaN.
+ * kvq_paged_workspace_bytes is 0 for invalid arguments and for none needed.
+ */
+typedef struct kvq_paged_args {
+    const void* q;
+    const void* new_k;
+    const void* new_v;
+    kvq_packed k, v;
+    const int32_t* block_tables;  /* [rows, width]                             */
+    const int32_t* ctx_lens;      /* [rows]                                    */
+    const int32_t* cu_new;        /* [rows + 1]                                */
+    uint64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride,
+        v_token_stride, v_head_stride;   /* elements; head_dim is contiguous   */
+    uint32_t rows;
+    uint32_t tokens;              /* rows of q, new_k, new_v and out           */
+    uint32_t n_heads;
+    uint32_t n_kv_heads;
+    uint32_t head_dim;
+    uint32_t group_size;
+    uint32_t pages;
+    uint32_t page_size;
+    uint32_t width;
+    uint32_t max_ctx;
+    uint32_t max_new;
+    uint32_t dtype;
+} kvq_paged_args;
+size_t kvq_paged_workspace_bytes(const kvq_paged_args* a);
+int kvq_paged_attend(const kvq_paged_args* a, void* out, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,7 +29,9 @@ EXPORTS = ("kvq_workspace_bytes", "kvq_decode", "kvq_decode_partial", "kvq_split
            "kvq_peer_region_bytes", "kvq_peer_record_offset", "kvq_peer_alloc", "kvq_peer_open",
            "kvq_peer_close", "kvq_peer_free", "kvq_peer_merge", "kvq_peer_status",
            "kvq_peer_last_error", "kvq_tsplit_region_bytes", "kvq_tsplit_supported", "kvq_tsplit_split_count",
-           "kvq_tsplit_decode", "kvq_stage_copy")
+           "kvq_tsplit_decode", "kvq_stage_copy",
+           "kvq_paged_tables", "kvq_paged_truncate", "kvq_paged_append", "kvq_paged_gather",
+           "kvq_paged_workspace_bytes", "kvq_paged_attend")
 
 
 class NativeUnavailable(RuntimeError):
@@ -57,6 +59,37 @@ class KvqArgs(ctypes.Structure):
         ("has_new_entry", ctypes.c_uint32), ("cache_batch_stride", ctypes.c_uint64),
         ("t_begin", ctypes.c_uint32), ("t_end", ctypes.c_uint32),
     ]
+
+
+class KvqTables(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in (
+        "lens", "step", "block_tables", "free_pages", "n_free", "cu_new", "slots", "positions",
+        "lens_out", "n_free_out", "status")]
+        + [(n, ctypes.c_uint32) for n in ("rows", "width", "pool", "page_size", "max_tokens")])
+
+
+_POOLS = [(f"{half}_{part}", ctypes.c_void_p) for half in ("k", "v")
+          for part in ("words", "scales", "biases")]
+
+
+class KvqPagedRows(ctypes.Structure):
+    _fields_ = (_POOLS + [(n, ctypes.c_void_p) for n in ("keys", "values", "slots")]
+                + [(n, ctypes.c_uint64) for n in (
+                    "k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride")]
+                + [(n, ctypes.c_uint32) for n in (
+                    "tokens", "n_kv_heads", "head_dim", "group_size", "pages", "page_size",
+                    "dtype", "out_dtype")])
+
+
+class KvqPagedArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "new_k", "new_v")] + _POOLS
+                + [(n, ctypes.c_void_p) for n in ("block_tables", "ctx_lens", "cu_new")]
+                + [(n, ctypes.c_uint64) for n in (
+                    "q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+                    "v_token_stride", "v_head_stride")]
+                + [(n, ctypes.c_uint32) for n in (
+                    "rows", "tokens", "n_heads", "n_kv_heads", "head_dim", "group_size", "pages",
+                    "page_size", "width", "max_ctx", "max_new", "dtype")])
 
 
 _lock = threading.Lock()
@@ -98,6 +131,12 @@ def _declare(lib) -> None:
         "kvq_tsplit_split_count": (U32, [AP]),
         "kvq_tsplit_decode": (I, [AP, P, SZ, U32, U32, P, U64, P]),
         "kvq_stage_copy": (I, [P, P, SZ, P]),
+        "kvq_paged_tables": (I, [P, P]),
+        "kvq_paged_truncate": (I, [P, P]),
+        "kvq_paged_append": (I, [P, P]),
+        "kvq_paged_gather": (I, [P, P]),
+        "kvq_paged_workspace_bytes": (SZ, [P]),
+        "kvq_paged_attend": (I, [P, P, P, SZ, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

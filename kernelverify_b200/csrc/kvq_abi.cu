@@ -12,6 +12,7 @@
 
 #include "kvq_b200.h"
 #include "kvq_launch.h"
+#include "kvq_paged.h"
 #include "kvq_partial.cuh"
 
 namespace {
@@ -333,6 +334,17 @@ int noalloc_scratch(void** out) {
 }  // namespace
 
 namespace kvq {
+
+int api_fail(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    return fail(code, "%s", buf);
+}
+
+int api_device_ok() { return device_ok(); }
 
 // The merges are launched as programmatic dependents of the kernel before
 // them on the stream (the split stage): their CTAs are launched while it
