@@ -1,0 +1,16 @@
+// Launchers of the paged attention's kernels, one translation unit per element
+// type; kvq_paged_attn.cu chooses among them.
+#pragma once
+
+#include "kvq_paged.h"
+
+namespace kvq {
+namespace paged {
+
+// Requests with at most most_new new tokens, 8 nt query columns per pass over
+// the cache, on `grid` CTAs.
+cudaError_t launch_few_f16(const Attend& a, int nt, uint32_t most_new, uint32_t grid, void* ws, cudaStream_t s);
+cudaError_t launch_few_f32(const Attend& a, uint32_t most_new, uint32_t grid, void* ws, cudaStream_t s);
+
+}  // namespace paged
+}  // namespace kvq

@@ -1,0 +1,165 @@
+// How the paged attention kernels divide a ragged step among their CTAs.
+//
+// The step is a list of units (request, cache head, tile of query columns),
+// each a run of key tiles. Only the device knows the lengths, so every CTA
+// makes the running sum of the requests' tiles in shared memory and takes an
+// equal, contiguous share of the whole list: no CTA has more than one share
+// whatever the lengths, and none waits for another. A unit that lies in one
+// share is finished there. Of the others, a CTA leaves at most two partial
+// results -- of the unit that began before its share (slot 0), and of the one
+// that goes on after it (slot 1) -- and the merge kernel joins a unit's parts,
+// which are those of consecutive CTAs, in their order (results do not depend on
+// timing).
+#pragma once
+
+#include <atomic>
+
+#include "kvq_common.cuh"
+#include "kvq_paged.h"
+
+namespace kvq {
+namespace paged {
+
+// What the CTA in whose share a split unit begins leaves for the merge: the
+// unit spans this CTA and the parts - 1 that follow. parts = 0: none.
+struct Split {
+    uint32_t parts, token0, hk, col0, cols;
+};
+
+// Partials live in the workspace as [grid] Split, then per (CTA, slot) m[cols],
+// l[cols], O[cols][DH]; all of it is written before it is read.
+__host__ __device__ inline size_t split_bytes(uint32_t grid) { return ((size_t)grid * sizeof(Split) + 255) / 256 * 256; }
+__host__ __device__ inline size_t slot_floats(uint32_t cols, uint32_t dh) { return (size_t)cols * (dh + 2); }
+
+// The request's tokens in this step, cut to the bounds the caller gave.
+struct Request {
+    uint32_t ctx, token0, n;
+};
+__device__ __forceinline__ Request request_of(const Attend& a, uint32_t b) {
+    Request r;
+    r.ctx = min((uint32_t)max(a.ctx_lens[b], 0), a.max_ctx);
+    r.token0 = min((uint32_t)max(a.cu_new[b], 0), a.tokens);
+    const uint32_t end = min((uint32_t)max(a.cu_new[b + 1], 0), a.tokens);
+    r.n = end > r.token0 ? min(end - r.token0, a.max_new) : 0;
+    return r;
+}
+
+// before[b] = tiles of the requests in front of b, before[rows] the total:
+// tiles_of(b) summed over the rows by all THREADS threads of the block.
+template <int THREADS, typename F>
+__device__ void sum_tiles(uint32_t* before, uint32_t rows, F&& tiles_of) {
+    __shared__ uint32_t scratch[THREADS / 32];
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t per = (rows + THREADS - 1) / THREADS;
+    const uint32_t r0 = min(rows, tid * per), r1 = min(rows, r0 + per);
+    uint32_t own = 0;
+    for (uint32_t r = r0; r < r1; ++r) {
+        const uint32_t t = tiles_of(r);
+        if (per > 1) before[r] = t;
+        own += t;
+    }
+    uint32_t incl = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= (uint32_t)o) incl += u;
+    }
+    if (lane == 31) scratch[warp] = incl;
+    __syncthreads();
+    uint32_t at = incl - own;
+    for (uint32_t w = 0; w < warp; ++w) at += scratch[w];
+    if (per == 1) {
+        if (r0 < r1) before[r0] = at;
+    } else {
+        for (uint32_t r = r0; r < r1; ++r) {
+            const uint32_t t = before[r];
+            before[r] = at;
+            at += t;
+        }
+    }
+    if (tid == THREADS - 1) before[rows] = at;
+    __syncthreads();
+}
+
+// The last request in front of which at most x tiles lie.
+__device__ __forceinline__ uint32_t row_of_tile(const uint32_t* before, uint32_t rows, uint32_t x) {
+    uint32_t lo = 0, hi = rows;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (before[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// One block per (CTA of the split kernel, column): the unit's parts joined,
+// out = sum_p O_p 2^(m_p - m) / sum_p l_p 2^(m_p - m), m = max_p m_p in log2.
+template <typename T, int DH, int COLS>
+__global__ void __launch_bounds__(DH) join_kernel(Attend a, const unsigned char* __restrict__ ws) {
+    __shared__ float weight[DH];
+    __shared__ float red[DH / 32];
+    pdl_wait();
+    const uint32_t cta = blockIdx.x, col = blockIdx.y, d = threadIdx.x;
+    const Split u = reinterpret_cast<const Split*>(ws)[cta];
+    if (u.parts == 0 || col >= u.cols) return;
+    const float* slots = reinterpret_cast<const float*>(ws + split_bytes(gridDim.x));
+    constexpr size_t SLOT = (size_t)COLS * (DH + 2);
+    // part 0 is this CTA's slot 1, part p > 0 CTA cta + p's slot 0
+    const auto part = [&](uint32_t p) { return slots + (2 * (size_t)(cta + p) + (p == 0 ? 1 : 0)) * SLOT; };
+    float m = -INFINITY;
+    for (uint32_t p = d; p < u.parts; p += DH) m = fmaxf(m, part(p)[col]);
+    m = warp_max(m);
+    if ((d & 31) == 0) red[d >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < DH / 32; ++w) m = fmaxf(m, red[w]);
+    float o = 0.0f, l = 0.0f;
+    for (uint32_t p0 = 0; p0 < u.parts; p0 += DH) {
+        const uint32_t n = min((uint32_t)DH, u.parts - p0);
+        __syncthreads();
+        if (d < n) weight[d] = exp2f(part(p0 + d)[col] - m);
+        __syncthreads();
+#pragma unroll 8
+        for (uint32_t p = 0; p < n; ++p) {
+            const float* s = part(p0 + p);
+            o += weight[p] * s[2 * COLS + (size_t)col * DH + d];
+            l += weight[p] * s[COLS + col];
+        }
+    }
+    const uint32_t c = u.col0 + col, tok = u.token0 + c / a.r, head = u.hk * a.r + c % a.r;
+    static_cast<T*>(a.out)[((size_t)tok * a.n_heads + head) * DH + d] = from_f32<T>(o / l);
+}
+
+// A kernel's dynamic shared memory limit, set once per device (`done` is the
+// kernel's own), so that later launches, captured ones included, make no
+// attribute calls.
+template <typename K>
+cudaError_t allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (bit && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_acq_rel);
+    return e;
+}
+
+template <typename T, int DH, int COLS>
+cudaError_t launch_join(const Attend& a, uint32_t grid, const unsigned char* ws, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid, COLS);
+    cfg.blockDim = dim3(DH);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, join_kernel<T, DH, COLS>, a, ws);
+}
+
+}  // namespace paged
+}  // namespace kvq
