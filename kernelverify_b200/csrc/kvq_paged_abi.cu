@@ -6,6 +6,7 @@
 
 namespace kvq {
 namespace paged {
+bool attend_fits(const Attend& a);
 size_t attend_workspace(const Attend& a);
 cudaError_t launch_attend(const Attend& a, void* workspace, cudaStream_t stream);
 }  // namespace paged
@@ -207,6 +208,7 @@ int attend_of(const kvq_paged_args* a, Attend* p) {
     p->max_new = a->max_new < a->tokens ? a->max_new : a->tokens;
     p->dtype = (int)a->dtype;
     p->scale = 1.0f / sqrtf((float)a->head_dim);
+    if (!attend_fits(*p)) return api_fail(KVQ_ERR_INVALID, "max_ctx and max_new allow too many tiles for one step: lower them or split the batch");
     return KVQ_OK;
 }
 

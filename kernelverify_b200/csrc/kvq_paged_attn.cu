@@ -12,38 +12,78 @@ namespace paged {
 namespace {
 
 struct Choice {
-    int nt;              // few: column tiles of 8
-    uint32_t cols, grid;
+    uint32_t few_most;       // new tokens of a request up to which the few kernel takes it (0: none)
+    int nt;                  // its column tiles of 8
+    uint32_t few_grid, many_grid;
+    bool vec;
+    bool fits;               // the tiles can be counted in 31 bits
 };
+
+uint32_t grid_for(uint64_t tiles, uint64_t least, uint64_t most) {
+    const uint64_t n = (tiles + least - 1) / least;
+    return (uint32_t)(n < 1 ? 1 : (n > most ? most : n));
+}
 
 Choice choose(const Attend& a) {
     Choice c{};
-    const uint64_t cols = (uint64_t)a.max_new * a.r;
+    c.fits = true;
+    const uint64_t cols = (uint64_t)a.max_new * a.r, sms = (uint64_t)sm_count();
+    const uint64_t rows = a.rows < a.tokens ? a.rows : a.tokens;
+    c.few_most = 0xFFFFFFFFu;
     c.nt = a.dtype == KVQ_F16 && cols > 8 ? 2 : 1;
-    c.cols = 8u * c.nt;
-    const uint64_t per_sm = a.dtype == KVQ_F16 && c.nt == 1 ? 2 : 1;
-    // tiles the step can have at most: no CTA for less than a round of eight
-    const uint64_t tokens = a.tokens, ct = (cols + c.cols - 1) / c.cols;
-    const uint64_t units = (uint64_t)(a.rows < tokens ? a.rows : tokens) * a.n_kv_heads * ct;
-    const uint64_t tiles = units * ((uint64_t)a.max_ctx / 16 + 1);
-    uint64_t grid = per_sm * (uint64_t)sm_count();
-    if (grid > (tiles + 7) / 8) grid = (tiles + 7) / 8;
-    c.grid = (uint32_t)(grid < 1 ? 1 : grid);
+    if (a.dtype == KVQ_F16 && a.r <= 128 && cols > 16) {
+        // one request: the many kernel alone, whatever it brings
+        c.nt = 1;
+        c.few_most = a.rows == 1 ? 0 : (a.r >= 8 ? 1 : 8 / a.r);
+        // units have at most 256 query rows
+        const uint64_t tu = 2 * (128 / a.r), units = (uint64_t)a.n_kv_heads * (a.tokens / tu + rows);
+        const uint64_t tiles = units * (((uint64_t)a.max_ctx + a.max_new) / MANY_KEYS + 2);
+        c.fits = tiles < TOO_MANY;
+        c.many_grid = grid_for(tiles, 4, sms);
+        const size_t es = 2;
+        c.vec = true;
+        for (const void* p : {a.q, a.new_k, a.new_v}) c.vec = c.vec && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+        for (uint64_t st : {a.q_token, a.q_head, a.k_token, a.k_head, a.v_token, a.v_head}) c.vec = c.vec && st * es % 16 == 0;
+    }
+    if (c.few_most) {
+        // no CTA for less than a round of its eight warps
+        const uint64_t few = c.few_most < a.max_new ? c.few_most : a.max_new, w = 8u * c.nt;
+        const uint64_t tiles = rows * a.n_kv_heads * ((few * a.r + w - 1) / w) * ((uint64_t)a.max_ctx / 16 + 1);
+        c.fits = c.fits && tiles < TOO_MANY;
+        c.few_grid = grid_for(tiles, 8, (a.dtype == KVQ_F16 && c.nt == 1 ? 2 : 1) * sms);
+    }
     return c;
+}
+
+size_t few_bytes(const Attend& a, const Choice& c) {
+    if (!c.few_most) return 0;
+    return (split_bytes(c.few_grid) + 2 * (size_t)c.few_grid * slot_floats(8u * c.nt, a.head_dim) * sizeof(float) + 255) / 256 * 256;
+}
+size_t many_bytes(const Attend& a, const Choice& c) {
+    if (!c.many_grid) return 0;
+    return split_bytes(c.many_grid) + 2 * (size_t)c.many_grid * slot_floats(MANY_COLS, a.head_dim) * sizeof(float);
 }
 
 }  // namespace
 
+bool attend_fits(const Attend& a) { return a.tokens == 0 || a.max_new == 0 || choose(a).fits; }
+
 size_t attend_workspace(const Attend& a) {
     if (a.tokens == 0 || a.max_new == 0) return 0;
     const Choice c = choose(a);
-    return split_bytes(c.grid) + 2 * (size_t)c.grid * slot_floats(c.cols, a.head_dim) * sizeof(float);
+    return few_bytes(a, c) + many_bytes(a, c);
 }
 
 cudaError_t launch_attend(const Attend& a, void* ws, cudaStream_t s) {
     const Choice c = choose(a);
-    if (a.dtype == KVQ_F16) return launch_few_f16(a, c.nt, 0xFFFFFFFFu, c.grid, ws, s);
-    return launch_few_f32(a, 0xFFFFFFFFu, c.grid, ws, s);
+    if (c.many_grid) {
+        const cudaError_t e = launch_many_f16(a, c.few_most + 1, c.vec, c.many_grid,
+                                              static_cast<unsigned char*>(ws) + few_bytes(a, c), s);
+        if (e != cudaSuccess) return e;
+    }
+    if (!c.few_most) return cudaSuccess;
+    if (a.dtype == KVQ_F16) return launch_few_f16(a, c.nt, c.few_most, c.few_grid, ws, s);
+    return launch_few_f32(a, c.few_most, c.few_grid, ws, s);
 }
 
 }  // namespace paged

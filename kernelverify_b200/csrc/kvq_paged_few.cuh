@@ -165,11 +165,10 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
     const uint32_t H = a.n_kv_heads;
     const auto tiles_in = [](uint32_t ctx) { return max(1u, (ctx + TP - 1) / TP); };
     const auto col_tiles = [&](const Request& r) { return r.n > most_new ? 0u : (r.n * a.r + COLS - 1) / COLS; };
-    sum_tiles<THREADS>(before, a.rows, [&](uint32_t b) {
+    const uint32_t total = sum_tiles<THREADS>(before, a.rows, [&](uint32_t b) {
         const Request r = request_of(a, b);
-        return col_tiles(r) * H * tiles_in(r.ctx);
+        return (uint64_t)col_tiles(r) * H * tiles_in(r.ctx);
     });
-    const uint32_t total = before[a.rows];
     // a whole round of the warps is the least a CTA takes
     const uint32_t share = ((total + gridDim.x - 1) / gridDim.x + CW - 1) / CW * CW;
     const uint64_t start64 = (uint64_t)blockIdx.x * share;

@@ -1,0 +1,623 @@
+// Paged attention for requests with many new tokens (prompt chunks), fp16, on
+// the 5th-generation tensor cores.
+//
+// A unit is up to 256 query rows of one (request, cache head): two M tiles of
+// 128 rows, a row being one (token, query head), the R heads of a token side
+// by side, so the R heads share every key they read. Keys come in tiles of
+// 128: the cached positions first, dequantized to fp16, then the step's own
+// entries under the causal mask. Both products are tcgen05.mma kind::f16 of
+// 128 x 128 x DH:
+//
+//   S_i = Q_i K^T   (both operands in shared memory, fp32 S in tensor memory)
+//   O_i += P_i V    (P_i fp16 in tensor memory over S_i's columns)
+//
+// Sixteen warps in four warpgroups, registers re-split with setmaxnreg:
+//   0, 1  softmax of M tile 0 and 1, a thread per row: S from tensor memory,
+//         an online softmax whose reference moves (and rescales O) only when
+//         the row's maximum passed it by 2^8, P back to tensor memory; at the
+//         end O / l to the output, or the unit's part to the workspace
+//   2     loads: a thread per key; 4-bit rows become fp16 by one HFMA2 per two
+//         codes, stored with the 128-byte swizzle the MMAs read
+//   3     one thread issues the MMAs
+// While one M tile is in its softmax the tensor cores work for the other. K
+// and V tiles have the same layout, rows of keys: K is read as a K-major
+// operand, V as an MN-major one. Within each run of eight dims, operands hold
+// them in the order 0 4 1 5 2 6 3 7 that unpacking a word gives; scores do not
+// depend on it and the output is put back in order.
+//
+// Rounded to fp16: the dequantized K and V (as a cache held in fp16 would be)
+// and the weights P; everything else is fp32. P is at most 2^14 and its sum is
+// taken before the rounding.
+#pragma once
+
+#include <atomic>
+
+#include "kvq_paged_work.cuh"
+#include "kvq_umma.cuh"
+
+namespace kvq {
+namespace paged {
+namespace many {
+
+using mma4::and_or;
+using mma4::ex2;
+using mma4::mbar_arrive;
+using mma4::mbar_init;
+using mma4::mbar_try_wait;
+using umma::fence_async_smem;
+using umma::idesc;
+using umma::tc_fence_after;
+using umma::tc_fence_before;
+using umma::tmem_alloc;
+using umma::tmem_dealloc;
+using umma::tmem_relinquish;
+using umma::tmem_wait_ld;
+using umma::tmem_wait_st;
+using umma::umma;
+using umma::umma_commit;
+
+constexpr int THREADS = 512;
+constexpr int KT = 128;                    // keys per tile
+constexpr int ROWS = 128;                  // query rows per M tile
+constexpr int COLS = 2 * ROWS;             // query rows per unit
+constexpr int STAGES = 2;                  // K and V tiles in shared memory, each
+constexpr float RAISE = 8.0f, START = 6.0f;
+// registers per thread at launch and after the re-split; the sum over the four
+// warpgroups must stay the launch's (a larger one would wait forever)
+constexpr int REG_LAUNCH = 128, REG_SOFTMAX = 176, REG_LOAD = 112, REG_MMA = 48;
+static_assert(2 * REG_SOFTMAX + REG_LOAD + REG_MMA <= 4 * REG_LAUNCH, "register re-split over the launch budget");
+constexpr uint64_t WAIT_NS = 1000000000ull;
+
+template <int DH>
+struct Cfg {
+    static constexpr int PANELS = DH / 64;             // 64 dims: 128-byte rows
+    static constexpr int PANEL = KT * 128;
+    static constexpr int TILE = PANELS * PANEL;        // a 128-row operand
+    static constexpr int Q = 0;
+    static constexpr int K = 2 * TILE;
+    static constexpr int V = K + STAGES * TILE;
+    static constexpr int BAR = V + STAGES * TILE;
+    // q_full[2], s_full[2], p_full[2], o_full[2], then k_full, k_empty, v_full,
+    // v_empty [STAGES] each, and the MMA thread's last one
+    static constexpr int NBAR = 8 + 4 * STAGES + 2;
+    static constexpr int MISC = BAR + NBAR * 8;        // TMEM address, error flag
+    static constexpr int BEFORE = MISC + 16;           // uint32 [rows + 1]
+    static constexpr uint32_t S0 = 0, O0 = 256;        // TMEM columns: S_i at 128 i, O_i at 256 + 128 i
+    static_assert(PANEL % 1024 == 0, "swizzle atoms are 1024-byte aligned");
+};
+
+// ---- PTX wrappers ------------------------------------------------------------
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+        "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),
+          "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]),
+          "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]),
+          "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]),
+        "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
+        "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(id), "r"(accumulate)
+        : "memory");
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Descriptor of an operand with the 128-byte swizzle: rows of 128 bytes, eight
+// to a 1024-byte atom. K-major (Q, K): the rows are M or N, atoms along them
+// 1024 bytes apart. MN-major (V): the rows are K, atoms along them 1024 bytes
+// apart (stride offset), the next 64 of N a panel apart (leading offset).
+__device__ __forceinline__ uint64_t desc128(uint32_t saddr, uint32_t leading) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((leading >> 4) & 0x3FFFu) << 16) |
+           ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// byte offset of 16-byte chunk c (eight dims) of row r in a panel
+__device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+
+// Every wait ends: after a second of device time, or once another wait gave up.
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* err) {
+    if (mbar_try_wait(bar, parity)) return;
+    const uint64_t t0 = now_ns();
+    do {
+        if (mbar_try_wait(bar, parity) || *err) return;
+    } while (now_ns() - t0 < WAIT_NS);
+    *err = 1;
+}
+
+// eight fp16 in natural order -> the operands' order 0 4 1 5 2 6 3 7
+__device__ __forceinline__ uint4 reorder(uint4 x) {
+    return make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410),
+                      __byte_perm(x.y, x.w, 0x7632));
+}
+// a word's eight codes -> fp16 scale * code + bias, rounded once: 1024 + c (or
+// 1024 + 16 c) is exact, and so is c after one subtraction (or multiply-add)
+__device__ __forceinline__ uint4 values_of(uint32_t w, __half2 s, __half2 z) {
+    const __half2 big = __half2half2(__ushort_as_half(0x6400)), one16 = __half2half2(__ushort_as_half(0x2C00)),
+                  m64 = __half2half2(__ushort_as_half(0xD400));
+    uint32_t x[4] = {and_or<0x000F000Fu, 0x64006400u>(w), and_or<0x00F000F0u, 0x64006400u>(w),
+                     and_or<0x000F000Fu, 0x64006400u>(w >> 8), and_or<0x00F000F0u, 0x64006400u>(w >> 8)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        __half2 h = *reinterpret_cast<__half2*>(&x[i]);
+        h = i & 1 ? __hfma2(h, one16, m64) : __hsub2(h, big);
+        h = __hfma2(h, s, z);
+        x[i] = *reinterpret_cast<uint32_t*>(&h);
+    }
+    return make_uint4(x[0], x[1], x[2], x[3]);
+}
+
+// sum_{i=0}^{n-1} floor((a i + b) / 128)
+__device__ __forceinline__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+    uint64_t s = 0;
+    while (n > 0) {
+        s += n * (n - 1) / 2 * (a / m) + n * (b / m);
+        a %= m;
+        b %= m;
+        const uint64_t y = a * n + b;
+        if (y < m) break;
+        n = y / m;
+        b = y % m;
+        const uint64_t t = a;
+        a = m;
+        m = t;
+    }
+    return s;
+}
+
+// A request's units and their key tiles. Unit i brings tokens [i tu, (i + 1)
+// tu) and needs the cached tiles and the own tiles up to its last token.
+struct Shape {
+    Request rq;
+    uint32_t tu, units, past;          // tokens per unit, units per cache head, cached tiles
+    // key tiles of the units in front of unit i
+    __device__ __forceinline__ uint32_t in_front(uint32_t i) const {
+        if (i < units) return i * past + (uint32_t)floor_sum(i, KT, tu, tu + KT - 1);
+        return i * past + (uint32_t)floor_sum(i - 1, KT, tu, tu + KT - 1) + (rq.n + KT - 1) / KT;
+    }
+};
+__device__ __forceinline__ Shape shape_of(const Attend& a, uint32_t b, uint32_t least_new) {
+    Shape s;
+    s.rq = request_of(a, b);
+    s.tu = 2 * (ROWS / a.r);
+    s.past = (s.rq.ctx + KT - 1) / KT;
+    s.units = s.rq.n >= least_new ? (s.rq.n + s.tu - 1) / s.tu : 0;
+    return s;
+}
+
+// The part [lo, hi) (in tiles of the whole step) of a unit in a CTA's share.
+struct Part {
+    Shape s;
+    uint32_t b, hk, unit, u0, u1, lo, hi;
+    uint32_t tok0, n_tok;              // the unit's tokens
+    bool second;                       // its second M tile has any
+};
+__device__ __forceinline__ Part part_at(const Attend& a, const uint32_t* before, uint32_t least_new, uint32_t at, uint32_t end) {
+    Part p;
+    p.b = row_of_tile(before, a.rows, at);
+    p.s = shape_of(a, p.b, least_new);
+    const uint32_t per_head = p.s.in_front(p.s.units);
+    const uint32_t rem = at - before[p.b];
+    p.hk = rem / per_head;
+    const uint32_t x = rem - p.hk * per_head;
+    uint32_t lo = 0, hi = p.s.units;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (p.s.in_front(mid) <= x) lo = mid;
+        else hi = mid;
+    }
+    p.unit = lo;
+    p.u0 = before[p.b] + p.hk * per_head + p.s.in_front(lo);
+    p.u1 = before[p.b] + p.hk * per_head + p.s.in_front(lo + 1);
+    p.lo = at;
+    p.hi = min(end, p.u1);
+    p.tok0 = lo * p.s.tu;
+    p.n_tok = min(p.s.tu, p.s.rq.n - p.tok0);
+    p.second = p.n_tok > p.s.tu / 2;
+    return p;
+}
+
+template <int DH, int GROUP>
+__global__ void __launch_bounds__(THREADS, 1)
+many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ ws) {
+    using C = Cfg<DH>;
+    constexpr int G = DH / GROUP, W = DH / 8;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (mma4::s_addr(smem_raw) & 1023u)) & 1023u);
+    uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::BAR);
+    uint64_t *q_full = bar, *s_full = bar + 2, *p_full = bar + 4, *o_full = bar + 6;
+    uint64_t *k_full = bar + 8, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES;
+    uint64_t* drained = v_empty + STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::MISC);
+    volatile int* err = reinterpret_cast<volatile int*>(smem + C::MISC + 4);
+    uint32_t* before = reinterpret_cast<uint32_t*>(smem + C::BEFORE);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wg = warp >> 2;
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&q_full[i], 4);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_full[i], 1);
+        }
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(&k_full[i], 4);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 4);
+            mbar_init(&v_empty[i], 1);
+        }
+        mbar_init(drained, 1);
+        *err = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        reinterpret_cast<Split*>(ws)[blockIdx.x].parts = 0;
+    }
+    const uint32_t total = sum_tiles<THREADS>(before, a.rows, [&](uint32_t b) {
+        const Shape s = shape_of(a, b, least_new);
+        return s.units ? (uint64_t)s.in_front(s.units) * a.n_kv_heads : 0ull;
+    });
+    const uint32_t share = (total + gridDim.x - 1) / gridDim.x;
+    const uint64_t start64 = (uint64_t)blockIdx.x * share;
+    if (start64 >= total) return;
+    const uint32_t start = (uint32_t)start64, end = min(total, start + share);
+
+    if (warp == 12) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (wg < 2) {
+        // ---------------------------- softmax ------------------------------------
+        regs_inc<REG_SOFTMAX>();
+        const int mt = wg, row = tid & 127;
+        const uint32_t tokm = ROWS / a.r;
+        const uint32_t rt = row / a.r, rh = row - rt * a.r;          // the row's token of the M tile, head
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // TMEM lane 32 (warp % 4), bits 16 up
+        const uint32_t s_at = tmem + lanes + C::S0 + 128 * mt, o_at = tmem + lanes + C::O0 + 128 * mt;
+        const float scale2 = a.scale * 1.4426950408889634f;
+        uint32_t tiles_done = 0, parts_done = 0;
+        for (uint32_t at = start; at < end;) {
+            const Part p = part_at(a, before, least_new, at, end);
+            at = p.hi;
+            if (mt == 1 && !p.second) continue;
+            const uint32_t tok = p.tok0 + mt * tokm + rt;           // of the request
+            const bool live = rt < tokm && tok < p.s.rq.n;
+            // this M tile's queries (the last MMA that read the buffer is done: its
+            // scores have been read)
+            {
+                unsigned char* dst = smem + C::Q + mt * C::TILE;
+                const __half* q = static_cast<const __half*>(a.q) + (p.s.rq.token0 + tok) * a.q_token + (p.hk * a.r + rh) * a.q_head;
+#pragma unroll
+                for (int c = 0; c < W; ++c) {
+                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                    if (live) {
+                        if (vec) {
+                            x = reinterpret_cast<const uint4*>(q)[c];
+                        } else {
+                            __half h[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) h[i] = q[8 * c + i];
+                            x = *reinterpret_cast<const uint4*>(h);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(dst + (c >> 3) * C::PANEL + swizzled(row, c & 7)) = reorder(x);
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[mt]);
+            }
+            float ref = -INFINITY, l = 0.0f;
+            for (uint32_t j = p.lo; j < p.hi; ++j, ++tiles_done) {
+                wait(&s_full[mt], tiles_done & 1, err);
+                __syncwarp();
+                tc_fence_after();
+                uint32_t s[KT];
+#pragma unroll
+                for (int c = 0; c < KT; c += 32) ld32(s_at + c, s + c);
+                tmem_wait_ld();
+                // visible keys of the tile: the cached ones up to the length, of the
+                // step's own those up to the row's token
+                const uint32_t tile = j - p.u0;
+                const int lim = tile < p.s.past ? (int)min((uint32_t)KT, p.s.rq.ctx - tile * KT)
+                                                : (int)tok - (int)((tile - p.s.past) * KT) + 1;
+                if (__any_sync(0xffffffffu, lim < KT)) {
+#pragma unroll
+                    for (int c = 0; c < KT; ++c)
+                        if (c >= lim) s[c] = 0xff800000u;
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < KT; c += 2) top = fmaxf(top, fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])));
+                top *= scale2;
+                const bool over = top - ref > RAISE;
+                if (__any_sync(0xffffffffu, over)) {
+                    const float to = over ? top - START : ref;
+                    // a row that has seen nothing yet has nothing to rescale
+                    const float f = ref == -INFINITY ? 0.0f : ex2(ref - to);
+                    ref = to;
+                    l *= f;
+                    if (j > p.lo) {
+#pragma unroll
+                        for (int c = 0; c < DH; c += 16) {
+                            uint32_t o[16];
+                            umma::tmem_ld16(o_at + c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            umma::tmem_st16(o_at + c, o);
+                        }
+                    }
+                }
+                const float sub = ref == -INFINITY ? 0.0f : ref;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < KT; c += 2) {
+                    const float x = ex2(fmaf(__uint_as_float(s[c]), scale2, -sub));
+                    const float y = ex2(fmaf(__uint_as_float(s[c + 1]), scale2, -sub));
+                    sum[(c >> 1) & 3] += x + y;
+                    const __half2 h = __floats2half2_rn(x, y);
+                    s[c >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+                    if (c % 64 == 62) st32(s_at + c / 2 - 31, s + c / 2 - 31);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[mt]);
+            }
+            // ---- the part's result ------------------------------------------------
+            wait(&o_full[mt], parts_done & 1, err);
+            ++parts_done;
+            __syncwarp();
+            tc_fence_after();
+            const bool whole = p.u0 >= start && p.u1 <= end;
+            const uint32_t col = mt * tokm * a.r + row;                 // row of the unit
+            float* slot = reinterpret_cast<float*>(ws + split_bytes(gridDim.x)) +
+                          (2 * (size_t)blockIdx.x + (p.u0 >= start ? 1 : 0)) * slot_floats(COLS, DH);
+            __half* out = static_cast<__half*>(a.out) +
+                          ((size_t)(p.s.rq.token0 + tok) * a.n_heads + p.hk * a.r + rh) * DH;
+            const float inv = *err ? NAN : (whole ? 1.0f / l : 1.0f);
+#pragma unroll
+            for (int c = 0; c < DH; c += 32) {
+                uint32_t o[32];
+                __syncwarp();
+                ld32(o_at + c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    if (!live) break;
+                    // columns hold dims 0 4 1 5 2 6 3 7
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[(e >> 1) + 4 * (e & 1)] = __uint_as_float(o[i + e]) * inv;
+                    if (whole) {
+                        alignas(16) __half2 h[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+                        *reinterpret_cast<uint4*>(out + c + i) = *reinterpret_cast<const uint4*>(h);
+                    } else {
+                        float4* d = reinterpret_cast<float4*>(slot + 2 * COLS + (size_t)col * DH + c + i);
+                        d[0] = make_float4(x[0], x[1], x[2], x[3]);
+                        d[1] = make_float4(x[4], x[5], x[6], x[7]);
+                    }
+                }
+            }
+            if (!whole && live) {
+                slot[col] = ref;
+                slot[COLS + col] = l;
+            }
+            if (tid == 0 && p.u0 >= start && p.u1 > end)
+                reinterpret_cast<Split*>(ws)[blockIdx.x] = {(p.u1 - 1) / share - blockIdx.x + 1, p.s.rq.token0, p.hk,
+                                                            p.tok0 * a.r, p.n_tok * a.r};
+            tc_fence_before();
+        }
+    } else if (wg == 2) {
+        // ------------------------------ loads -------------------------------------
+        regs_dec<REG_LOAD>();
+        const uint32_t row = tid & 127;
+        uint32_t done = 0;
+        for (uint32_t at = start; at < end;) {
+            const Part p = part_at(a, before, least_new, at, end);
+            at = p.hi;
+            for (uint32_t j = p.lo; j < p.hi; ++j, ++done) {
+                const uint32_t st = done % STAGES, use = done / STAGES, tile = j - p.u0;
+                unsigned char* kd = smem + C::K + st * C::TILE;
+                unsigned char* vd = smem + C::V + st * C::TILE;
+                if (tile < p.s.past) {
+                    const uint32_t pos = tile * KT + row;
+                    const bool live = pos < p.s.rq.ctx;
+                    bool bad = false;
+                    uint4 kw[W / 4], vw[W / 4];
+                    __half sc[4][G];
+                    if (live) {
+                        uint32_t page = (uint32_t)a.block_tables[(size_t)p.b * a.width + (pos >> a.page_shift)];
+                        bad = page >= a.pages;
+                        if (bad) page = 0;
+                        const uint64_t r = (((uint64_t)page * a.n_kv_heads + p.hk) << a.page_shift) + (pos & ((1u << a.page_shift) - 1));
+#pragma unroll
+                        for (int i = 0; i < W / 4; ++i) {
+                            kw[i] = reinterpret_cast<const uint4*>(a.k.words + r * W)[i];
+                            vw[i] = reinterpret_cast<const uint4*>(a.v.words + r * W)[i];
+                        }
+#pragma unroll
+                        for (int i = 0; i < G; ++i) {
+                            sc[0][i] = static_cast<const __half*>(a.k.scales)[r * G + i];
+                            sc[1][i] = static_cast<const __half*>(a.k.biases)[r * G + i];
+                            sc[2][i] = static_cast<const __half*>(a.v.scales)[r * G + i];
+                            sc[3][i] = static_cast<const __half*>(a.v.biases)[r * G + i];
+                        }
+                    } else {
+                        // keys past the length: zeros, which the mask (K) and the zero
+                        // weights (V) leave without effect
+#pragma unroll
+                        for (int i = 0; i < W / 4; ++i) kw[i] = vw[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                        for (int i = 0; i < G; ++i)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) sc[x][i] = __ushort_as_half(0);
+                    }
+                    if (bad) {
+#pragma unroll
+                        for (int i = 0; i < G; ++i) sc[1][i] = __ushort_as_half(0x7FFF);
+                    }
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (use) wait(half ? &v_empty[st] : &k_empty[st], (use - 1) & 1, err);
+                        unsigned char* d = half ? vd : kd;
+                        const uint4* w = half ? vw : kw;
+#pragma unroll
+                        for (int c = 0; c < W; ++c) {
+                            const uint32_t word = c % 4 == 0 ? w[c / 4].x : c % 4 == 1 ? w[c / 4].y : c % 4 == 2 ? w[c / 4].z : w[c / 4].w;
+                            *reinterpret_cast<uint4*>(d + (c >> 3) * C::PANEL + swizzled(row, c & 7)) =
+                                values_of(word, __half2half2(sc[2 * half][c * 8 / GROUP]), __half2half2(sc[2 * half + 1][c * 8 / GROUP]));
+                        }
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(half ? &v_full[st] : &k_full[st]);
+                    }
+                } else {
+                    const uint32_t own = (tile - p.s.past) * KT + row;
+                    const bool live = own < p.s.rq.n;
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        const __half* src = half ? static_cast<const __half*>(a.new_v) + (p.s.rq.token0 + own) * a.v_token + p.hk * a.v_head
+                                                 : static_cast<const __half*>(a.new_k) + (p.s.rq.token0 + own) * a.k_token + p.hk * a.k_head;
+                        uint4 x[W];
+#pragma unroll
+                        for (int c = 0; c < W; ++c) {
+                            x[c] = make_uint4(0u, 0u, 0u, 0u);
+                            if (live) {
+                                if (vec) {
+                                    x[c] = reinterpret_cast<const uint4*>(src)[c];
+                                } else {
+                                    __half h[8];
+#pragma unroll
+                                    for (int i = 0; i < 8; ++i) h[i] = src[8 * c + i];
+                                    x[c] = *reinterpret_cast<const uint4*>(h);
+                                }
+                            }
+                        }
+                        if (use) wait(half ? &v_empty[st] : &k_empty[st], (use - 1) & 1, err);
+                        unsigned char* d = half ? vd : kd;
+#pragma unroll
+                        for (int c = 0; c < W; ++c)
+                            *reinterpret_cast<uint4*>(d + (c >> 3) * C::PANEL + swizzled(row, c & 7)) = reorder(x[c]);
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(half ? &v_full[st] : &k_full[st]);
+                    }
+                }
+            }
+        }
+    } else {
+        // --------------------------- the MMAs -----------------------------------------
+        regs_dec<REG_MMA>();
+        if (warp == 12 && lane == 0) {
+            constexpr uint32_t ID_S = idesc(false, false, false, KT, ROWS);
+            constexpr uint32_t ID_O = idesc(false, false, true, DH, ROWS);
+            const uint32_t base = mma4::s_addr(smem);
+            uint32_t done = 0, parts[2] = {0, 0}, tiles[2] = {0, 0};
+            const auto scores = [&](int i, uint32_t st) {
+#pragma unroll
+                for (int k = 0; k < DH / 16; ++k) {
+                    const uint32_t off = (k >> 2) * C::PANEL + (k & 3) * 32;
+                    umma(tmem + C::S0 + 128 * i, desc128(base + C::Q + i * C::TILE + off, 16),
+                         desc128(base + C::K + st * C::TILE + off, 16), ID_S, k > 0);
+                }
+            };
+            const auto combine = [&](int i, uint32_t st, bool first) {
+#pragma unroll
+                for (int k = 0; k < KT / 16; ++k)
+                    umma_ts(tmem + C::O0 + 128 * i, tmem + C::S0 + 128 * i + 8 * k,
+                            desc128(base + C::V + st * C::TILE + k * 2048, C::PANEL), ID_O, !first || k > 0);
+            };
+            for (uint32_t at = start; at < end;) {
+                const Part p = part_at(a, before, least_new, at, end);
+                at = p.hi;
+                const int n = p.second ? 2 : 1;
+                for (int i = 0; i < n; ++i) wait(&q_full[i], parts[i] & 1, err);
+                for (uint32_t j = p.lo; j <= p.hi; ++j) {
+                    const uint32_t st = done % STAGES, pst = (done - 1) % STAGES;
+                    if (j < p.hi) wait(&k_full[st], (done / STAGES) & 1, err);
+                    if (j > p.lo) wait(&v_full[pst], ((done - 1) / STAGES) & 1, err);
+                    for (int i = 0; i < n; ++i) {
+                        if (j > p.lo) {
+                            wait(&p_full[i], (tiles[i] - 1) & 1, err);
+                            tc_fence_after();
+                            combine(i, pst, j - 1 == p.lo);
+                            if (j == p.hi) umma_commit(&o_full[i]);
+                            if (i == n - 1) umma_commit(&v_empty[pst]);
+                        }
+                        if (j < p.hi) {
+                            tc_fence_after();
+                            scores(i, st);
+                            umma_commit(&s_full[i]);
+                            if (i == n - 1) umma_commit(&k_empty[st]);
+                            ++tiles[i];
+                        }
+                    }
+                    if (j < p.hi) ++done;
+                }
+                for (int i = 0; i < n; ++i) ++parts[i];
+            }
+            // nothing of this CTA's is in flight when its tensor memory goes
+            umma_commit(drained);
+            for (const uint64_t t0 = now_ns(); !mbar_try_wait(drained, 0) && now_ns() - t0 < WAIT_NS;) {}
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 12) tmem_dealloc(tmem, 512);
+    pdl_launch_dependents();
+}
+
+template <int DH, int GROUP>
+cudaError_t launch_many(const Attend& a, uint32_t least_new, bool vec, uint32_t grid, void* ws, cudaStream_t stream) {
+    using C = Cfg<DH>;
+    auto kernel = many_kernel<DH, GROUP>;
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(kernel, 1024 + C::BEFORE + (MAX_ROWS + 1) * 4, done);
+    if (e != cudaSuccess) return e;
+    // the register re-split assumes the launch's count (host-side constant of the build)
+    static const int regs = [&] {
+        cudaFuncAttributes f{};
+        return cudaFuncGetAttributes(&f, kernel) == cudaSuccess ? f.numRegs : 0;
+    }();
+    if (regs != REG_LAUNCH) return cudaErrorInvalidConfiguration;
+    const size_t smem = 1024 + C::BEFORE + ((size_t)a.rows + 1) * 4;
+    kernel<<<grid, THREADS, smem, stream>>>(a, least_new, vec, static_cast<unsigned char*>(ws));
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    return launch_join<__half, DH, COLS>(a, grid, static_cast<const unsigned char*>(ws), stream);
+}
+
+}  // namespace many
+}  // namespace paged
+}  // namespace kvq

@@ -45,40 +45,48 @@ __device__ __forceinline__ Request request_of(const Attend& a, uint32_t b) {
 }
 
 // before[b] = tiles of the requests in front of b, before[rows] the total:
-// tiles_of(b) summed over the rows by all THREADS threads of the block.
+// tiles_of(b) summed over the rows by all THREADS threads of the block. Sums
+// stop at TOO_MANY (the host refuses steps that can have as many, so only
+// offsets that are no running sum get there): returned as a total of 0, and
+// the step is left undone.
+constexpr uint64_t TOO_MANY = 0x7FFFFFFFull;
 template <int THREADS, typename F>
-__device__ void sum_tiles(uint32_t* before, uint32_t rows, F&& tiles_of) {
-    __shared__ uint32_t scratch[THREADS / 32];
+__device__ uint32_t sum_tiles(uint32_t* before, uint32_t rows, F&& tiles_of) {
+    __shared__ uint64_t scratch[THREADS / 32];
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t per = (rows + THREADS - 1) / THREADS;
     const uint32_t r0 = min(rows, tid * per), r1 = min(rows, r0 + per);
-    uint32_t own = 0;
+    uint64_t own = 0;
     for (uint32_t r = r0; r < r1; ++r) {
-        const uint32_t t = tiles_of(r);
-        if (per > 1) before[r] = t;
+        const uint64_t t = min((uint64_t)tiles_of(r), TOO_MANY);
+        if (per > 1) before[r] = (uint32_t)t;
         own += t;
     }
-    uint32_t incl = own;
+    uint64_t incl = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
+        const uint64_t u = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= (uint32_t)o) incl += u;
     }
     if (lane == 31) scratch[warp] = incl;
     __syncthreads();
-    uint32_t at = incl - own;
-    for (uint32_t w = 0; w < warp; ++w) at += scratch[w];
+    uint64_t at = incl - own, total = 0;
+    for (uint32_t w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) at += scratch[w];
+        total += scratch[w];
+    }
     if (per == 1) {
-        if (r0 < r1) before[r0] = at;
+        if (r0 < r1) before[r0] = (uint32_t)at;
     } else {
         for (uint32_t r = r0; r < r1; ++r) {
             const uint32_t t = before[r];
-            before[r] = at;
+            before[r] = (uint32_t)at;
             at += t;
         }
     }
-    if (tid == THREADS - 1) before[rows] = at;
+    if (tid == THREADS - 1) before[rows] = (uint32_t)total;
     __syncthreads();
+    return total < TOO_MANY ? (uint32_t)total : 0;
 }
 
 // The last request in front of which at most x tiles lie.
@@ -92,42 +100,46 @@ __device__ __forceinline__ uint32_t row_of_tile(const uint32_t* before, uint32_t
     return lo;
 }
 
-// One block per (CTA of the split kernel, column): the unit's parts joined,
+// A warp per (CTA of the split kernel, column): the unit's parts joined,
 // out = sum_p O_p 2^(m_p - m) / sum_p l_p 2^(m_p - m), m = max_p m_p in log2.
+constexpr int JOIN_WARPS = 8;
 template <typename T, int DH, int COLS>
-__global__ void __launch_bounds__(DH) join_kernel(Attend a, const unsigned char* __restrict__ ws) {
-    __shared__ float weight[DH];
-    __shared__ float red[DH / 32];
-    pdl_wait();
-    const uint32_t cta = blockIdx.x, col = blockIdx.y, d = threadIdx.x;
-    const Split u = reinterpret_cast<const Split*>(ws)[cta];
-    if (u.parts == 0 || col >= u.cols) return;
-    const float* slots = reinterpret_cast<const float*>(ws + split_bytes(gridDim.x));
+__global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(Attend a, const unsigned char* __restrict__ ws) {
+    constexpr int V = DH / 32;             // dims per lane
     constexpr size_t SLOT = (size_t)COLS * (DH + 2);
+    pdl_wait();
+    const uint32_t cta = blockIdx.x, lane = threadIdx.x & 31, col = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5);
+    const Split u = reinterpret_cast<const Split*>(ws)[cta];
+    if (col >= COLS || u.parts == 0 || col >= u.cols) return;
+    const float* slots = reinterpret_cast<const float*>(ws + split_bytes(gridDim.x));
     // part 0 is this CTA's slot 1, part p > 0 CTA cta + p's slot 0
     const auto part = [&](uint32_t p) { return slots + (2 * (size_t)(cta + p) + (p == 0 ? 1 : 0)) * SLOT; };
     float m = -INFINITY;
-    for (uint32_t p = d; p < u.parts; p += DH) m = fmaxf(m, part(p)[col]);
+    for (uint32_t p = lane; p < u.parts; p += 32) m = fmaxf(m, part(p)[col]);
     m = warp_max(m);
-    if ((d & 31) == 0) red[d >> 5] = m;
-    __syncthreads();
+    float o[V], l = 0.0f;
 #pragma unroll
-    for (int w = 0; w < DH / 32; ++w) m = fmaxf(m, red[w]);
-    float o = 0.0f, l = 0.0f;
-    for (uint32_t p0 = 0; p0 < u.parts; p0 += DH) {
-        const uint32_t n = min((uint32_t)DH, u.parts - p0);
-        __syncthreads();
-        if (d < n) weight[d] = exp2f(part(p0 + d)[col] - m);
-        __syncthreads();
+    for (int i = 0; i < V; ++i) o[i] = 0.0f;
+    for (uint32_t p0 = 0; p0 < u.parts; p0 += 32) {
+        float w = 0.0f;
+        if (p0 + lane < u.parts) {
+            w = exp2f(part(p0 + lane)[col] - m);
+            l += w * part(p0 + lane)[COLS + col];
+        }
+        const uint32_t n = min(32u, u.parts - p0);
 #pragma unroll 8
         for (uint32_t p = 0; p < n; ++p) {
-            const float* s = part(p0 + p);
-            o += weight[p] * s[2 * COLS + (size_t)col * DH + d];
-            l += weight[p] * s[COLS + col];
+            const float f = __shfl_sync(0xffffffffu, w, p);
+            const float* s = part(p0 + p) + 2 * COLS + (size_t)col * DH + lane * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] += f * s[i];
         }
     }
+    l = warp_sum(l);
     const uint32_t c = u.col0 + col, tok = u.token0 + c / a.r, head = u.hk * a.r + c % a.r;
-    static_cast<T*>(a.out)[((size_t)tok * a.n_heads + head) * DH + d] = from_f32<T>(o / l);
+    T* out = static_cast<T*>(a.out) + ((size_t)tok * a.n_heads + head) * DH + lane * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = from_f32<T>(o[i] / l);
 }
 
 // A kernel's dynamic shared memory limit, set once per device (`done` is the
@@ -150,8 +162,8 @@ cudaError_t allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
 template <typename T, int DH, int COLS>
 cudaError_t launch_join(const Attend& a, uint32_t grid, const unsigned char* ws, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid, COLS);
-    cfg.blockDim = dim3(DH);
+    cfg.gridDim = dim3(grid, (COLS + JOIN_WARPS - 1) / JOIN_WARPS);
+    cfg.blockDim = dim3(32 * JOIN_WARPS);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
