@@ -102,8 +102,18 @@ __device__ __forceinline__ void parts_of(float x, float y, uint32_t (&h)[N]) {
         y -= f.y;
     }
 }
-// codes j and j + 4 of a word (or of two words' halves) as subnormal fp16x2
-__device__ __forceinline__ uint32_t nib(uint32_t w, int j) { return (w >> (4 * j)) & 0x000F000Fu; }
+// codes j and j + 4 of a word (or of two words' halves) as subnormal fp16x2:
+// c, or c - 8 (exact) for fp32 steps, whose sums over codes of one sign would
+// be far larger than what the bias then leaves of them
+template <bool HALF>
+__device__ __forceinline__ uint32_t nib(uint32_t w, int j) {
+    uint32_t x = (w >> (4 * j)) & 0x000F000Fu;
+    if constexpr (!HALF) {
+        const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(8)));
+        x = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return x;
+}
 __device__ __forceinline__ float pow2(int e) { return ldexpf(1.0f, e); }
 
 // c (+)= a * b; fp32 steps add in fp32 registers (see the head of this file)
@@ -421,7 +431,7 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                     const uint32_t wa = kw[pa * C::W + word_of(u)], wb = kw[pb * C::W + word_of(u)];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const uint32_t f[4] = {nib(wa, 2 * i), nib(wb, 2 * i), nib(wa, 2 * i + 1), nib(wb, 2 * i + 1)};
+                        const uint32_t f[4] = {nib<HALF>(wa, 2 * i), nib<HALF>(wb, 2 * i), nib<HALF>(wa, 2 * i + 1), nib<HALF>(wb, 2 * i + 1)};
 #pragma unroll
                         for (int p = 0; p < QP; ++p)
 #pragma unroll
@@ -443,7 +453,11 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
 #pragma unroll
                 for (int i = 0; i < G; ++i) {
                     const float sa = to_f32(ks[pa * G + i]), sb = to_f32(ks[pb * G + i]);
-                    const float za = to_f32(kz[pa * G + i]), zb = to_f32(kz[pb * G + i]);
+                    float za = to_f32(kz[pa * G + i]), zb = to_f32(kz[pb * G + i]);
+                    if (!HALF) {
+                        za = fmaf(8.0f, sa, za);
+                        zb = fmaf(8.0f, sb, zb);
+                    }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -455,6 +469,10 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                     vsb[i] = to_f32(vs[pb * G + i]);
                     vza[i] = to_f32(vz[pa * G + i]);
                     vzb[i] = to_f32(vz[pb * G + i]);
+                    if (!HALF) {                    // the codes' 8
+                        vza[i] = fmaf(8.0f, vsa[i], vza[i]);
+                        vzb[i] = fmaf(8.0f, vsb[i], vzb[i]);
+                    }
                 }
                 if (valid < TP) {
                     // rows past the length may hold anything
@@ -547,7 +565,7 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                         const uint32_t lo23 = prmt(w[2], w[3], 0x5410), hi23 = prmt(w[2], w[3], 0x7632);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const uint32_t f[4] = {nib(lo01, j), nib(hi01, j), nib(lo23, j), nib(hi23, j)};
+                            const uint32_t f[4] = {nib<HALF>(lo01, j), nib<HALF>(hi01, j), nib<HALF>(lo23, j), nib<HALF>(hi23, j)};
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -564,7 +582,7 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                             const uint32_t w01 = prmt(w[0], w[1], sel), w23 = prmt(w[2], w[3], sel);
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
-                                const uint32_t f[4] = {nib(w01, 2 * j), nib(w01, 2 * j + 1), nib(w23, 2 * j), nib(w23, 2 * j + 1)};
+                                const uint32_t f[4] = {nib<HALF>(w01, 2 * j), nib<HALF>(w01, 2 * j + 1), nib<HALF>(w23, 2 * j), nib<HALF>(w23, 2 * j + 1)};
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

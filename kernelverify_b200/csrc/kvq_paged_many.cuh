@@ -14,7 +14,7 @@
 // Sixteen warps in four warpgroups, registers re-split with setmaxnreg:
 //   0, 1  softmax of M tile 0 and 1, a thread per row: S from tensor memory,
 //         an online softmax whose reference moves (and rescales O) only when
-//         the row's maximum passed it by 2^8, P back to tensor memory; at the
+//         the row's maximum passed it by 2^14, P back to tensor memory; at the
 //         end O / l to the output, or the unit's part to the workspace
 //   2     loads: a thread per key; 4-bit rows become fp16 by one HFMA2 per two
 //         codes, stored with the 128-byte swizzle the MMAs read
@@ -61,12 +61,12 @@ constexpr int KT = 128;                    // keys per tile
 constexpr int ROWS = 128;                  // query rows per M tile
 constexpr int COLS = 2 * ROWS;             // query rows per unit
 constexpr int STAGES = 2;                  // K and V tiles in shared memory, each
-constexpr float RAISE = 8.0f, START = 6.0f;
+constexpr float RAISE = 14.0f, START = 4.0f;   // log2 room above the reference
 // registers per thread at launch and after the re-split; the sum over the four
 // warpgroups must stay the launch's (a larger one would wait forever)
 constexpr int REG_LAUNCH = 128, REG_SOFTMAX = 176, REG_LOAD = 112, REG_MMA = 48;
 static_assert(2 * REG_SOFTMAX + REG_LOAD + REG_MMA <= 4 * REG_LAUNCH, "register re-split over the launch budget");
-constexpr uint64_t WAIT_NS = 1000000000ull;
+constexpr long long WAIT_CYCLES = 2000000000ll;      // about a second
 
 template <int DH>
 struct Cfg {
@@ -117,6 +117,12 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint
         "r"(a), "l"(b), "r"(id), "r"(accumulate)
         : "memory");
 }
+// true in one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
 template <int N>
 __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -133,18 +139,13 @@ __device__ __forceinline__ uint64_t desc128(uint32_t saddr, uint32_t leading) {
 // byte offset of 16-byte chunk c (eight dims) of row r in a panel
 __device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
-// Every wait ends: after a second of device time, or once another wait gave up.
-__device__ __forceinline__ uint64_t now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
+// Every wait ends: after WAIT_CYCLES, or once another wait gave up.
 __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* err) {
     if (mbar_try_wait(bar, parity)) return;
-    const uint64_t t0 = now_ns();
+    const long long t0 = clock64();
     do {
         if (mbar_try_wait(bar, parity) || *err) return;
-    } while (now_ns() - t0 < WAIT_NS);
+    } while (clock64() - t0 < WAIT_CYCLES);
     *err = 1;
 }
 
@@ -538,25 +539,15 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
     } else {
         // --------------------------- the MMAs -----------------------------------------
         regs_dec<REG_MMA>();
-        if (warp == 12 && lane == 0) {
+        if (warp == 12) {
+            // The whole warp walks the tiles and one elected lane issues, so that
+            // the operands' descriptors stay in uniform registers: under a
+            // condition on the lane number each MMA took 190 cycles to issue
+            // against the 64 it runs.
             constexpr uint32_t ID_S = idesc(false, false, false, KT, ROWS);
             constexpr uint32_t ID_O = idesc(false, false, true, DH, ROWS);
             const uint32_t base = mma4::s_addr(smem);
             uint32_t done = 0, parts[2] = {0, 0}, tiles[2] = {0, 0};
-            const auto scores = [&](int i, uint32_t st) {
-#pragma unroll
-                for (int k = 0; k < DH / 16; ++k) {
-                    const uint32_t off = (k >> 2) * C::PANEL + (k & 3) * 32;
-                    umma(tmem + C::S0 + 128 * i, desc128(base + C::Q + i * C::TILE + off, 16),
-                         desc128(base + C::K + st * C::TILE + off, 16), ID_S, k > 0);
-                }
-            };
-            const auto combine = [&](int i, uint32_t st, bool first) {
-#pragma unroll
-                for (int k = 0; k < KT / 16; ++k)
-                    umma_ts(tmem + C::O0 + 128 * i, tmem + C::S0 + 128 * i + 8 * k,
-                            desc128(base + C::V + st * C::TILE + k * 2048, C::PANEL), ID_O, !first || k > 0);
-            };
             for (uint32_t at = start; at < end;) {
                 const Part p = part_at(a, before, least_new, at, end);
                 at = p.hi;
@@ -566,29 +557,43 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                     const uint32_t st = done % STAGES, pst = (done - 1) % STAGES;
                     if (j < p.hi) wait(&k_full[st], (done / STAGES) & 1, err);
                     if (j > p.lo) wait(&v_full[pst], ((done - 1) / STAGES) & 1, err);
-                    for (int i = 0; i < n; ++i) {
-                        if (j > p.lo) {
-                            wait(&p_full[i], (tiles[i] - 1) & 1, err);
-                            tc_fence_after();
-                            combine(i, pst, j - 1 == p.lo);
-                            if (j == p.hi) umma_commit(&o_full[i]);
-                            if (i == n - 1) umma_commit(&v_empty[pst]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (i == n) break;
+                        if (j > p.lo) wait(&p_full[i], (tiles[i] - 1) & 1, err);
+                        __syncwarp();
+                        tc_fence_after();
+                        if (elect_one()) {
+                            if (j > p.lo) {
+                                const uint64_t v = desc128(base + C::V + pst * C::TILE, C::PANEL);
+#pragma unroll
+                                for (int k = 0; k < KT / 16; ++k)
+                                    umma_ts(tmem + C::O0 + 128 * i, tmem + C::S0 + 128 * i + 8 * k, v + k * (2048 >> 4), ID_O,
+                                            j - 1 > p.lo || k > 0);
+                                if (j == p.hi) umma_commit(&o_full[i]);
+                                if (i == n - 1) umma_commit(&v_empty[pst]);
+                            }
+                            if (j < p.hi) {
+                                const uint64_t q = desc128(base + C::Q + i * C::TILE, 16), kd = desc128(base + C::K + st * C::TILE, 16);
+#pragma unroll
+                                for (int k = 0; k < DH / 16; ++k) {
+                                    const uint32_t off = ((k >> 2) * C::PANEL + (k & 3) * 32) >> 4;
+                                    umma(tmem + C::S0 + 128 * i, q + off, kd + off, ID_S, k > 0);
+                                }
+                                umma_commit(&s_full[i]);
+                                if (i == n - 1) umma_commit(&k_empty[st]);
+                            }
                         }
-                        if (j < p.hi) {
-                            tc_fence_after();
-                            scores(i, st);
-                            umma_commit(&s_full[i]);
-                            if (i == n - 1) umma_commit(&k_empty[st]);
-                            ++tiles[i];
-                        }
+                        __syncwarp();
+                        if (j < p.hi) ++tiles[i];
                     }
                     if (j < p.hi) ++done;
                 }
                 for (int i = 0; i < n; ++i) ++parts[i];
             }
             // nothing of this CTA's is in flight when its tensor memory goes
-            umma_commit(drained);
-            for (const uint64_t t0 = now_ns(); !mbar_try_wait(drained, 0) && now_ns() - t0 < WAIT_NS;) {}
+            if (elect_one()) umma_commit(drained);
+            for (const long long t0 = clock64(); !mbar_try_wait(drained, 0) && clock64() - t0 < WAIT_CYCLES;) {}
         }
     }
     tc_fence_before();
