@@ -50,6 +50,8 @@ int check_cache(uint32_t head_dim, uint32_t group, uint32_t dtype, uint32_t page
     if (int rc = check_page(page)) return rc;
     if (pages == 0 || pages > 0x7FFFFFFFu) return api_fail(KVQ_ERR_INVALID, "a pool of %u pages: 1 to 2^31 - 1", pages);
     if (heads == 0 || heads > 32767) return api_fail(KVQ_ERR_INVALID, "%u cache heads: 1 to 32767", heads);
+    if ((uint64_t)pages * heads * page > 0xFFFFFFFFull)
+        return api_fail(KVQ_ERR_INVALID, "a pool of %u pages x %u heads x %u rows: at most 2^32 - 1 rows", pages, heads, page);
     return KVQ_OK;
 }
 

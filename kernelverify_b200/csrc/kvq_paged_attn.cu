@@ -48,7 +48,7 @@ Choice choose(const Attend& a) {
     if (c.few_most) {
         // no CTA for less than a round of its eight warps
         const uint64_t few = c.few_most < a.max_new ? c.few_most : a.max_new, w = 8u * c.nt;
-        const uint64_t tiles = rows * a.n_kv_heads * ((few * a.r + w - 1) / w) * ((uint64_t)a.max_ctx / 16 + 1);
+        const uint64_t tiles = rows * a.n_kv_heads * ((few * a.r + w - 1) / w) * ((uint64_t)a.max_ctx / 32 + 1);
         c.fits = c.fits && tiles < TOO_MANY;
         c.few_grid = grid_for(tiles, 8, (a.dtype == KVQ_F16 && c.nt == 1 ? 2 : 1) * sms);
     }

@@ -3,20 +3,26 @@
 // one (token, query head) of a request, so the step is bound by the cache's
 // bytes.
 //
-// A warp takes 16 cached positions at a time: it streams them with
-// cp.async.bulk into its own ring (a page holds whole tiles; no warp waits for
-// another), and keeps its own online softmax; the CTA's eight warps are joined
-// when a unit ends. With codes c, scales s, z = bias:
+// A warp takes 32 cached positions at a time, as two blocks of 16: it streams
+// them with cp.async.bulk into its own ring (a page holds whole blocks; no warp
+// waits for another), and keeps its own online softmax; the CTA's eight warps
+// are joined when a unit ends. With codes c, scales s, z = bias:
 //
 //   scores   S^T[pos, col] = sum_g ks[pos,g] (sum_{d in g} c[pos,d] q[col,d])
 //                            + kz[pos,g] (sum_{d in g} q[col,d])
 //   combine  O^T[d, col]   = sum_pos c[pos,d] (p[pos,col] vs[pos,g(d)])
 //                            + sum_pos p[pos,col] vz[pos,g(d)]
 //
-// both as m16n8k16 fp16 MMAs with the codes as the A operand. Codes are never
-// converted: the bits of c are the fp16 subnormal c * 2^-24, which the tensor
-// cores multiply exactly, so two codes cost one shift and one AND, and the 2^24
-// goes into the scale. Which head dims (scores) and which positions (combine)
+// both as m16n8k16 fp16 MMAs with the codes as the A operand. For fp16 steps
+// codes are never converted: the bits of c are the fp16 subnormal c * 2^-24
+// (or, four bits higher, c * 2^-20), which the tensor cores multiply exactly,
+// so a word of eight codes costs one shift and four ANDs; the integer pipe is
+// what this kernel is short of next to memory. The factor 16 between the two
+// is in the query fragments, and in the combine, where odd codes are rows of
+// their own, in the result. ldmatrix.trans brings the V codes of two positions
+// into one register. The tensor cores align a subnormal's products by its
+// nominal exponent and so keep about 16 bits of their sums (measured 6e-6
+// relative); fp32 steps convert their codes to c - 8. Which head dims (scores) and which positions (combine)
 // a lane holds is free as long as both operands agree, and is chosen so that
 // the packed words are used where they are loaded. The weights p vs reach the
 // combine's B layout by one movmatrix per 8 x 8 block.
@@ -25,10 +31,10 @@
 // parts (2: 2^-22 relative, for fp16 steps; 3 for fp32 steps), held near the
 // top of fp16's range: p is relative to a reference that the running maximum
 // may pass by 2^14 before it moves (so accumulators are rarely rescaled), and
-// vs is divided by a power of two above the largest |vs| met so far. fp32
-// queries are three fp16 parts of q divided by a power of two per column, and
-// their MMAs start from zero and are added in fp32, since a long chain of
-// additions in the tensor cores truncates.
+// vs is divided by a power of two above the largest |vs| met so far. Queries
+// are scaled by a power of two per column (fp32 ones are three fp16 parts of
+// that, and their MMAs start from zero and are added in fp32, since a long
+// chain of additions in the tensor cores truncates).
 #pragma once
 
 #include <atomic>
@@ -50,7 +56,8 @@ using mma4::mma_f16;
 
 constexpr int CW = 8;                     // warps
 constexpr int THREADS = 32 * CW;
-constexpr int TP = 16;                    // positions per tile
+constexpr int BLK = 16, SUBS = 2;          // positions per block, blocks per tile
+constexpr int TP = BLK * SUBS;
 constexpr float RAISE = 14.0f, START = 5.0f;   // log2 room above the reference
 
 template <typename T, int DH_, int GROUP_, int NT_>
@@ -63,10 +70,11 @@ struct Cfg {
     static constexpr int MT = DH / 16;              // combine's 16-dim tiles
     static constexpr int QP = HALF ? 1 : 3, PP = HALF ? 2 : 3;
     static constexpr int COLS = 8 * NT;
-    static constexpr int WB = TP * W * 4, SB = TP * G * (int)sizeof(T);
+    static constexpr int WB = BLK * W * 4, SB = BLK * G * (int)sizeof(T);
     static constexpr int VW = WB, KS = 2 * WB, KZ = KS + SB, VS = KZ + SB, VZ = VS + SB;
-    static constexpr int STAGE = VZ + SB;
-    static constexpr int NST = 4;                   // tiles in flight per warp
+    static constexpr int BLOCK = VZ + SB;           // bytes of 16 positions
+    static constexpr int STAGE = SUBS * BLOCK;
+    static constexpr int NST = 2;                   // tiles per ring
     static constexpr int LD = DH + 4;               // floats per combined row (no bank conflicts)
     static constexpr int COMB = CW * STAGE * NST;   // fp32 [CW][COLS][LD], then m and l [CW][COLS]
     static constexpr int ML = COMB + CW * COLS * LD * 4;
@@ -76,11 +84,6 @@ struct Cfg {
     static_assert(STAGE % 16 == 0 && COMB % 16 == 0 && BAR % 8 == 0 && BEFORE % 16 == 0, "alignment");
 };
 
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-    uint32_t d;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
-    return d;
-}
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
@@ -102,19 +105,47 @@ __device__ __forceinline__ void parts_of(float x, float y, uint32_t (&h)[N]) {
         y -= f.y;
     }
 }
-// codes j and j + 4 of a word (or of two words' halves) as subnormal fp16x2:
-// c, or c - 8 (exact) for fp32 steps, whose sums over codes of one sign would
-// be far larger than what the bias then leaves of them
+// Codes j and j + 4 of a word (or code j of two positions) as fp16x2, times 16
+// for odd j: fp16 steps take c as a subnormal, in units of 2^-24; fp32 steps
+// take c - 8 (1024 + c and 1024 + 16 c are exact, and so is the difference),
+// since sums over codes of one sign would be far larger than what the bias then
+// leaves of them.
 template <bool HALF>
 __device__ __forceinline__ uint32_t nib(uint32_t w, int j) {
-    uint32_t x = (w >> (4 * j)) & 0x000F000Fu;
-    if constexpr (!HALF) {
-        const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(8)));
-        x = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return x;
+    const uint32_t v = j & 2 ? w >> 8 : w, mask = j & 1 ? 0x00F000F0u : 0x000F000Fu;
+    if constexpr (HALF) return v & mask;
+    const uint32_t x = (v & mask) | 0x64006400u;
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(j & 1 ? 0x6480 : 0x6408)));
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float pow2(int e) { return ldexpf(1.0f, e); }
+// 2^e for a normal exponent
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+// the G values of a position
+template <int G>
+__device__ __forceinline__ void scales_of(const __half* p, float (&x)[G]) {
+    if constexpr (G == 1) {
+        x[0] = __half2float(*p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < G; i += 2) {
+            const float2 f = __half22float2(reinterpret_cast<const __half2*>(p)[i / 2]);
+            x[i] = f.x;
+            x[i + 1] = f.y;
+        }
+    }
+}
+template <int G>
+__device__ __forceinline__ void scales_of(const float* p, float (&x)[G]) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) x[i] = p[i];
+}
+// four 8 x 8 b16 tiles, transposed: lanes 8 i .. 8 i + 7 give tile i's rows;
+// lane (g, t) receives rows 2t (low half) and 2t + 1 of column g in x[i]
+__device__ __forceinline__ void ldsm_trans(uint32_t saddr, uint32_t (&x)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                 : "r"(saddr));
+}
 
 // c (+)= a * b; fp32 steps add in fp32 registers (see the head of this file)
 template <bool HALF>
@@ -151,9 +182,10 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
     using C = Cfg<T, DH, GROUP, NT>;
     constexpr int G = C::G, COLS = C::COLS, QP = C::QP, PP = C::PP;
     constexpr bool HALF = C::HALF;
+    constexpr float UNIT = HALF ? 16777216.0f : 1.0f;      // a code in an MMA is c / UNIT, or 16 c / UNIT
     // exponents of the power of two above |vs|: from below what the quantizer
     // stores (its smallest step is 1e-7) to the type's largest
-    constexpr int VEXP0 = HALF ? -14 : -30, VEXP1 = HALF ? 16 : 100;
+    constexpr int VEXP0 = HALF ? -14 : -30, VEXP1 = HALF ? 16 : 90;
     extern __shared__ __align__(128) unsigned char smem[];
     uint32_t* before = reinterpret_cast<uint32_t*>(smem + C::BEFORE);
     float* comb = reinterpret_cast<float*>(smem + C::COMB);
@@ -186,53 +218,61 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
     const uint32_t start = (uint32_t)start64, end = min(total, start + share);
 
     // ---- the warp's stream of tiles -----------------------------------------
-    uint64_t row_at = 0;          // lane i: first cache row of the batch's i-th tile
-    uint32_t kind = 0;            // 0 no positions, 1 a page, 2 a page id outside the pool
-    uint32_t bad = 0;             // stages that hold such a page
+    // lane i looks up the batch's i-th tile: the cache row of each block, and per
+    // block whether it holds positions (bit) and its page id is in the pool (bad)
+    uint32_t row_at[SUBS] = {0, 0}, held = 0, bad_id = 0;
+    uint32_t bad = 0;                                  // stages with such a page
     const auto look = [&](uint32_t k0) {
         const uint64_t x64 = (uint64_t)start + warp + (uint64_t)CW * (k0 + lane);
-        kind = 0;
+        held = bad_id = 0;
         if (x64 >= end) return;
         const uint32_t x = (uint32_t)x64;
         const uint32_t b = row_of_tile(before, a.rows, x);
         const Request r = request_of(a, b);
-        const uint32_t tiles = tiles_in(r.ctx), rem = x - before[b], unit = rem / tiles;
-        const uint32_t pos = (rem - unit * tiles) * TP, hk = unit / col_tiles(r);
-        if (pos >= r.ctx) return;
-        uint32_t page = (uint32_t)a.block_tables[(size_t)b * a.width + (pos >> a.page_shift)];
-        kind = 1;
-        if (page >= a.pages) {
-            kind = 2;
-            page = 0;
+        const uint32_t tiles = tiles_in(r.ctx), rem = x - before[b], unit = rem / tiles, hk = unit / col_tiles(r);
+#pragma unroll
+        for (int i = 0; i < SUBS; ++i) {
+            const uint32_t pos = (rem - unit * tiles) * TP + i * BLK;
+            if (pos >= r.ctx) break;
+            uint32_t page = (uint32_t)a.block_tables[(size_t)b * a.width + (pos >> a.page_shift)];
+            held |= 1u << i;
+            if (page >= a.pages) {
+                bad_id = 1;
+                page = 0;
+            }
+            row_at[i] = ((page * H + hk) << a.page_shift) + (pos & ((1u << a.page_shift) - 1));
         }
-        row_at = (((uint64_t)page * H + hk) << a.page_shift) + (pos & ((1u << a.page_shift) - 1));
     };
+    // lanes 0..5 copy the first block's six runs, lanes 6..11 the second's
+    const int part = lane % 3, side = lane / 3 & 1, sub = lane / 6 & 1;
+    const Pool& pool = side ? a.v : a.k;
+    const unsigned char* src0 = part == 0 ? reinterpret_cast<const unsigned char*>(pool.words)
+                                          : static_cast<const unsigned char*>(part == 1 ? pool.scales : pool.biases);
+    const uint32_t row_bytes = part == 0 ? C::W * 4 : G * sizeof(T);
+    unsigned char* dst0 = ring + sub * C::BLOCK + (part == 0 ? side * C::WB : C::KS + (2 * side + part - 1) * C::SB);
+    const uint64_t policy = mma4::evict_first_policy();
     const uint32_t own = end - start > (uint32_t)warp ? (end - start - warp + CW - 1) / CW : 0;   // the warp's tiles
     const auto fill = [&](uint32_t k) {
         if (k >= own) return;
         if ((k & 31) == 0) look(k);
-        const uint64_t row = __shfl_sync(0xffffffffu, row_at, k & 31);
-        const uint32_t what = __shfl_sync(0xffffffffu, kind, k & 31);
+        const uint32_t r0 = __shfl_sync(0xffffffffu, row_at[0], k & 31), r1 = __shfl_sync(0xffffffffu, row_at[1], k & 31);
+        const uint32_t what = __shfl_sync(0xffffffffu, held | bad_id << SUBS, k & 31);
         const uint32_t s = k % C::NST;
-        bad = what == 2 ? bad | (1u << s) : bad & ~(1u << s);
-        if (what == 0) {
-            if (lane == 0) mbar_arrive(&bar[s]);
-            return;
+        bad = what >> SUBS ? bad | (1u << s) : bad & ~(1u << s);
+        const uint32_t n = __popc(what & ((1u << SUBS) - 1));
+        if (lane == 0) {
+            if (n) mbar_expect_tx(&bar[s], n * C::BLOCK);
+            else mbar_arrive(&bar[s]);
         }
-        if (lane == 0) mbar_expect_tx(&bar[s], C::STAGE);
         __syncwarp();
-        if (lane < 6) {
-            const int half = lane >= 3, part = lane - 3 * half;
-            const Pool& p = half ? a.v : a.k;
-            const unsigned char* src = part == 0 ? reinterpret_cast<const unsigned char*>(p.words) + row * (C::W * 4)
-                                       : static_cast<const unsigned char*>(part == 1 ? p.scales : p.biases) + row * (G * sizeof(T));
-            const int off = part == 0 ? half * C::WB : C::KS + (2 * half + part - 1) * C::SB;
-            bulk_g2s(ring + s * C::STAGE + off, src, part == 0 ? C::WB : C::SB, &bar[s], mma4::evict_first_policy());
-        }
+        if (lane < 6 * (int)n)
+            bulk_g2s(dst0 + s * C::STAGE, src0 + (uint64_t)(sub ? r1 : r0) * row_bytes, BLK * row_bytes, &bar[s], policy);
     };
     for (int k = 0; k < C::NST; ++k) fill(k);
 
     const float scale2 = a.scale * 1.4426950408889634f;     // scores in log2 units
+    // this lane's row address for ldsm_trans: tiles (positions 0..7, 8..15) x (16 bytes, the next 16)
+    const uint32_t v_at = mma4::s_addr(ring) + C::VW + (lane & 15) * (C::W * 4) + (lane >> 4) * 16;
     uint32_t k = 0;                                          // the warp's next tile
     for (uint32_t at = start; at < end;) {
         // ---- the unit this part of the share belongs to --------------------------
@@ -245,7 +285,7 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
 
         // query fragments: lane (g, t) holds column g's dims of its words
         uint32_t qf[QP][NT][C::SETS][4];
-        float qs[NT][2][G], cs[NT][2];
+        float qs[NT][2][G], cs[NT][2];            // of columns 2t, 2t + 1
         const auto word_of = [&](int u) { return GROUP >= 64 ? 8 * (u >> 1) + 2 * t + (u & 1) : 4 * u + t; };
         constexpr auto group_of = [](int u) { return GROUP >= 64 ? (u >> 1) * 64 / GROUP : u; };
 #pragma unroll
@@ -270,21 +310,19 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                     top = fmaxf(top, fabsf(x[u][i]));
                 }
             }
-            float down = 1.0f, up = 1.0f;
-            if constexpr (!HALF) {
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // the column's largest |q| at 2^12 (zero, huge and infinite ones as they are)
-                const int e = top > 1e-30f && top < 1e30f ? (int)(__float_as_uint(top) >> 23) - 127 - 12 : 0;
-                down = pow2(-e);
-                up = pow2(e);
-            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // the column's largest |q| between 2^10 and 2^11 (zero and infinite ones as
+            // they are), so that 16 q stays in range and small elements keep their bits
+            const int e = top > 1e-30f && top < 1e30f ? (int)(__float_as_uint(top) >> 23) - 127 - 10 : 0;
+            const float down = pow2(-e), up = pow2(e) * (scale2 * (UNIT / 16.0f));
 #pragma unroll
             for (int u = 0; u < C::SETS; ++u)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     uint32_t h[QP];
-                    parts_of<QP>(x[u][j] * down, x[u][j + 4] * down, h);
+                    const float f = j & 1 ? down : 16.0f * down;       // the codes' other factor
+                    parts_of<QP>(x[u][j] * f, x[u][j + 4] * f, h);
 #pragma unroll
                     for (int i = 0; i < QP; ++i) qf[i][nt][u][j] = h[i];
                 }
@@ -296,18 +334,20 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                 qs[nt][0][i] = __shfl_sync(0xffffffffu, v, 8 * t);
                 qs[nt][1][i] = __shfl_sync(0xffffffffu, v, 8 * t + 4);
             }
-            cs[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t) * scale2 * 16777216.0f;
-            cs[nt][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4) * scale2 * 16777216.0f;
+            cs[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t);
+            cs[nt][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
         }
 
-        float acc[C::MT][NT][4], ob[NT][2][G], l[NT][2], ref[NT][2];
+        // ref: what scores are relative to (0 until the column has one); room: how far
+        // above it a score may go (-inf until then)
+        float acc[C::MT][NT][4], ref[NT][2], room[NT][2], ob[NT][2][G], l[NT][2];
         int vexp = VEXP0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                l[nt][c] = 0.0f;
-                ref[nt][c] = -INFINITY;
+                l[nt][c] = ref[nt][c] = 0.0f;
+                room[nt][c] = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < G; ++i) ob[nt][c][i] = 0.0f;
             }
@@ -316,14 +356,13 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[m][nt][i] = 0.0f;
         }
-        // moves a column's reference where a score passed it by more than RAISE
-        const auto raise = [&](int nt, float top0, float top1) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const float top = c ? top1 : top0;
-                if (!(top - ref[nt][c] > RAISE)) continue;
-                const float to = top - START, f = ex2(ref[nt][c] - to);
-                ref[nt][c] = to;
+        // top: a column's highest score, relative to ref. Moves the reference where it
+        // is above the room, and returns by how much.
+        const auto raise = [&](int nt, int c, float top) {
+            if (!(top > room[nt][c])) return 0.0f;
+            const float by = top - START, f = ex2(-by);
+            ref[nt][c] += by;
+            if (room[nt][c] == RAISE) {         // else there is nothing yet to rescale
                 l[nt][c] *= f;
 #pragma unroll
                 for (int i = 0; i < G; ++i) ob[nt][c][i] *= f;
@@ -333,25 +372,25 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                     acc[m][nt][2 + c] *= f;
                 }
             }
+            room[nt][c] = RAISE;
+            return by;
         };
-        // head dim of the combine's row g (hi = 0) or g + 8 of tile m
-        const auto dim_of = [&](int m, int hi) {
-            if (GROUP >= 64) return 8 * (8 * (m >> 2) + g) + (m & 3) + 4 * hi;
-            return 8 * (8 * (m >> 2) + 4 * ((m >> 1) & 1) + (g & 3)) + 4 * (g >> 2) + 2 * (m & 1) + hi;
-        };
+        // head dim of the combine's row g (hi = 0) or g + 8 of tile m: code 2 (m % 2) + hi
+        // of the row's 16-bit unit; accumulators hold O UNIT / 2^vexp, times 16 for hi
+        const auto dim_of = [&](int m, int hi) { return 32 * (m >> 1) + 4 * g + 2 * (m & 1) + hi; };
 
         // ---- the step's own entries, in the share where the unit begins -----------
         // Entry j against every column: the quad's lanes hold column g's q.
         const auto own_entries = [&]() {
             if (u0 < start) return;
             const uint32_t last = min(rq.n, (col0 + COLS - 1) / a.r + 1);
-            const float unit_v = pow2(-vexp) * 5.9604644775390625e-8f;     // accumulators hold O / 2^(24 + vexp)
+            const float unit = pow2(-vexp) / UNIT;
             for (uint32_t j = warp; j < last; j += CW) {
                 const T* nk = static_cast<const T*>(a.new_k) + (rq.token0 + j) * a.k_token + hk * a.k_head;
                 const T* nv = static_cast<const T*>(a.new_v) + (rq.token0 + j) * a.v_token + hk * a.v_head;
-                float dot[NT];
+                float dot[NT], dot16[NT];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) dot[nt] = 0.0f;
+                for (int nt = 0; nt < NT; ++nt) dot[nt] = dot16[nt] = 0.0f;
 #pragma unroll
                 for (int u = 0; u < C::SETS; ++u) {
                     float x[8];
@@ -367,39 +406,42 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                                 q.x += h.x;
                                 q.y += h.y;
                             }
-                            dot[nt] += q.x * x[i];
-                            dot[nt] += q.y * x[i + 4];
+                            float& d = i & 1 ? dot[nt] : dot16[nt];
+                            d += q.x * x[i];
+                            d += q.y * x[i + 4];
                         }
                 }
                 float s[NT][2];
+                bool sees[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
+                    dot[nt] += dot16[nt] * 0.0625f;
                     dot[nt] += __shfl_xor_sync(0xffffffffu, dot[nt], 1);
                     dot[nt] += __shfl_xor_sync(0xffffffffu, dot[nt], 2);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        s[nt][c] = __shfl_sync(0xffffffffu, dot[nt], 8 * t + 4 * c) * cs[nt][c] * 5.9604644775390625e-8f;
+                        s[nt][c] = __shfl_sync(0xffffffffu, dot[nt], 8 * t + 4 * c) * (cs[nt][c] * (16.0f / UNIT)) - ref[nt][c];
                         const uint32_t col = col0 + nt * 8 + 2 * t + c;
                         // columns past the last one are zero queries: any weight will do
-                        if (col < n_cols && j > col / a.r) s[nt][c] = -INFINITY;
+                        sees[nt][c] = col >= n_cols || j <= col / a.r;
+                        if (!sees[nt][c]) s[nt][c] = -INFINITY;
                     }
-                    raise(nt, s[nt][0], s[nt][1]);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        s[nt][c] = s[nt][c] == -INFINITY ? 0.0f : ex2(s[nt][c] - ref[nt][c]);
+                        s[nt][c] = ex2(s[nt][c] - raise(nt, c, s[nt][c]));
                         if (g == 0) l[nt][c] += s[nt][c];
-                        s[nt][c] *= unit_v;
                     }
                 }
 #pragma unroll
                 for (int m = 0; m < C::MT; ++m)
 #pragma unroll
                     for (int hi = 0; hi < 2; ++hi) {
-                        const float v = to_f32(nv[dim_of(m, hi)]);
+                        const float v = to_f32(nv[dim_of(m, hi)]) * (hi ? 16.0f * unit : unit);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            acc[m][nt][2 * hi] += s[nt][0] * v;
-                            acc[m][nt][2 * hi + 1] += s[nt][1] * v;
+                            // a weight of zero would not keep an infinity out
+                            if (sees[nt][0]) acc[m][nt][2 * hi] += s[nt][0] * v;
+                            if (sees[nt][1]) acc[m][nt][2 * hi + 1] += s[nt][1] * v;
                         }
                     }
             }
@@ -407,189 +449,177 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
         own_entries();
 
         // ---- the cached tiles ------------------------------------------------------
-        // fragment row r (and k index r of the combine) is the tile's position
-        // r / 2 + 4 (r % 2) in each half of eight: the lanes of a quad then read
-        // consecutive rows
-        const int pa = (g >> 1) + 4 * (g & 1), pb = pa + 8;
+        float vlim = pow2(vexp), vinv = pow2(-vexp);
         for (; k < own && start + warp + k * CW < seg_end; ++k) {
             const uint32_t s = k % C::NST;
             if (!mbar_wait(&bar[s], (k / C::NST) & 1)) *err = 1;
-            const unsigned char* st = ring + s * C::STAGE;
+            const unsigned char* stage = ring + s * C::STAGE;
             const uint32_t pos0 = (start + warp + k * CW - u0) * TP;
             const uint32_t valid = rq.ctx > pos0 ? rq.ctx - pos0 : 0;
             if (valid > 0) {
-                float sacc[NT][G][4];
+                float p[SUBS][NT][4];                      // rows g (0, 1) and g + 8, columns 2t, 2t + 1
+                float vs[SUBS][2][G], vz[SUBS][2][G];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int i = 0; i < G; ++i)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) sacc[nt][i][c] = 0.0f;
-                const uint32_t* kw = reinterpret_cast<const uint32_t*>(st);
-#pragma unroll
-                for (int u = 0; u < C::SETS; ++u) {
-                    const uint32_t wa = kw[pa * C::W + word_of(u)], wb = kw[pb * C::W + word_of(u)];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t f[4] = {nib<HALF>(wa, 2 * i), nib<HALF>(wb, 2 * i), nib<HALF>(wa, 2 * i + 1), nib<HALF>(wb, 2 * i + 1)};
-#pragma unroll
-                        for (int p = 0; p < QP; ++p)
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-                                mma<HALF>(sacc[nt][group_of(u)], f, qf[p][nt][u][2 * i], qf[p][nt][u][2 * i + 1]);
-                    }
-                }
-                const T* ks = reinterpret_cast<const T*>(st + C::KS);
-                const T* kz = reinterpret_cast<const T*>(st + C::KZ);
-                const T* vs = reinterpret_cast<const T*>(st + C::VS);
-                const T* vz = reinterpret_cast<const T*>(st + C::VZ);
-                float p[NT][4];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) p[nt][c] = 0.0f;
-                float vsa[G], vsb[G], vza[G], vzb[G];
-                float vtop = 0.0f;
-#pragma unroll
-                for (int i = 0; i < G; ++i) {
-                    const float sa = to_f32(ks[pa * G + i]), sb = to_f32(ks[pb * G + i]);
-                    float za = to_f32(kz[pa * G + i]), zb = to_f32(kz[pb * G + i]);
-                    if (!HALF) {
-                        za = fmaf(8.0f, sa, za);
-                        zb = fmaf(8.0f, sb, zb);
-                    }
+                for (int b = 0; b < SUBS; ++b) {
+                    const unsigned char* st = stage + b * C::BLOCK;
+                    float sacc[NT][G][4];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            p[nt][c] += sacc[nt][i][c] * sa * cs[nt][c] + za * qs[nt][c][i];
-                            p[nt][2 + c] += sacc[nt][i][2 + c] * sb * cs[nt][c] + zb * qs[nt][c][i];
+                        for (int i = 0; i < G; ++i)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) sacc[nt][i][c] = 0.0f;
+                    const uint32_t* kw = reinterpret_cast<const uint32_t*>(st);
+#pragma unroll
+                    for (int u = 0; u < C::SETS; ++u) {
+                        const uint32_t wa = kw[g * C::W + word_of(u)], wb = kw[(g + 8) * C::W + word_of(u)];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t f[4] = {nib<HALF>(wa, 2 * i), nib<HALF>(wb, 2 * i), nib<HALF>(wa, 2 * i + 1),
+                                                   nib<HALF>(wb, 2 * i + 1)};
+#pragma unroll
+                            for (int x = 0; x < QP; ++x)
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt)
+                                    mma<HALF>(sacc[nt][group_of(u)], f, qf[x][nt][u][2 * i], qf[x][nt][u][2 * i + 1]);
                         }
-                    vsa[i] = to_f32(vs[pa * G + i]);
-                    vsb[i] = to_f32(vs[pb * G + i]);
-                    vza[i] = to_f32(vz[pa * G + i]);
-                    vzb[i] = to_f32(vz[pb * G + i]);
-                    if (!HALF) {                    // the codes' 8
-                        vza[i] = fmaf(8.0f, vsa[i], vza[i]);
-                        vzb[i] = fmaf(8.0f, vsb[i], vzb[i]);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int at_pos = (g + 8 * h) * G;
+                        float ks[G], kz[G];
+                        scales_of(reinterpret_cast<const T*>(st + C::KS) + at_pos, ks);
+                        scales_of(reinterpret_cast<const T*>(st + C::KZ) + at_pos, kz);
+                        scales_of(reinterpret_cast<const T*>(st + C::VS) + at_pos, vs[b][h]);
+                        scales_of(reinterpret_cast<const T*>(st + C::VZ) + at_pos, vz[b][h]);
+                        if (!HALF) {                          // the codes' 8
+#pragma unroll
+                            for (int i = 0; i < G; ++i) {
+                                kz[i] = fmaf(8.0f, ks[i], kz[i]);
+                                vz[b][h][i] = fmaf(8.0f, vs[b][h][i], vz[b][h][i]);
+                            }
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                float x = sacc[nt][0][2 * h + c] * ks[0], z = -ref[nt][c];
+#pragma unroll
+                                for (int i = 0; i < G; ++i) {
+                                    if (i) x = fmaf(sacc[nt][i][2 * h + c], ks[i], x);
+                                    z = fmaf(kz[i], qs[nt][c][i], z);
+                                }
+                                p[b][nt][2 * h + c] = fmaf(x, cs[nt][c], z);
+                            }
                     }
                 }
                 if (valid < TP) {
                     // rows past the length may hold anything
-                    const bool oa = (uint32_t)pa >= valid, obb = (uint32_t)pb >= valid;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int b = 0; b < SUBS; ++b)
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            if (oa) p[nt][c] = -INFINITY;
-                            if (obb) p[nt][2 + c] = -INFINITY;
+                        for (int h = 0; h < 2; ++h) {
+                            if ((uint32_t)(b * BLK + 8 * h + g) < valid) continue;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) p[b][nt][2 * h] = p[b][nt][2 * h + 1] = -INFINITY;
+#pragma unroll
+                            for (int i = 0; i < G; ++i) vs[b][h][i] = vz[b][h][i] = 0.0f;
                         }
-#pragma unroll
-                    for (int i = 0; i < G; ++i) {
-                        if (oa) vsa[i] = vza[i] = 0.0f;
-                        if (obb) vsb[i] = vzb[i] = 0.0f;
-                    }
                 }
                 if (bad & (1u << s)) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int b = 0; b < SUBS; ++b)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) p[nt][c] = NAN;
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) p[b][nt][c] = NAN;
                 }
+                float top[NT][2], vtop = 0.0f;
                 bool over = false;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) over |= fmaxf(p[nt][c], p[nt][2 + c]) - ref[nt][c] > RAISE;
+                    for (int c = 0; c < 2; ++c) {
+                        top[nt][c] = fmaxf(fmaxf(p[0][nt][c], p[0][nt][2 + c]), fmaxf(p[1][nt][c], p[1][nt][2 + c]));
+                        over |= top[nt][c] > room[nt][c];
+                    }
                 if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float top[2];
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            top[c] = fmaxf(p[nt][c], p[nt][2 + c]);
 #pragma unroll
-                            for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
+                            for (int o = 4; o < 32; o <<= 1) top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(0xffffffffu, top[nt][c], o));
+                            const float by = raise(nt, c, top[nt][c]);
+#pragma unroll
+                            for (int b = 0; b < SUBS; ++b) {
+                                p[b][nt][c] -= by;
+                                p[b][nt][2 + c] -= by;
+                            }
                         }
-                        raise(nt, top[0], top[1]);
-                    }
                 }
 #pragma unroll
-                for (int i = 0; i < G; ++i) vtop = fmaxf(vtop, fmaxf(fabsf(vsa[i]), fabsf(vsb[i])));
-                const int ve = min((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)) >> 23) - 126, VEXP1);
-                if (ve > vexp) {                   // |vs| < 2^ve
-                    const float f = pow2(vexp - ve);
-                    vexp = ve;
+                for (int b = 0; b < SUBS; ++b)
 #pragma unroll
-                    for (int m = 0; m < C::MT; ++m)
+                    for (int i = 0; i < G; ++i) vtop = fmaxf(vtop, fmaxf(fabsf(vs[b][0][i]), fabsf(vs[b][1][i])));
+                if (__any_sync(0xffffffffu, vtop >= vlim)) {
+                    const int ve = min((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)) >> 23) - 126, VEXP1);
+                    if (ve > vexp) {               // |vs| < 2^ve
+                        const float f = pow2(vexp - ve);
+                        vexp = ve;
+                        vlim = pow2(ve);
+                        vinv = pow2(-ve);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) acc[m][nt][c] *= f;
-                }
-                const float vinv = pow2(-vexp);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        p[nt][c] = ex2(p[nt][c] - ref[nt][c]);
-                        p[nt][2 + c] = ex2(p[nt][2 + c] - ref[nt][c]);
-                        l[nt][c] += p[nt][c] + p[nt][2 + c];
-                    }
-                uint32_t bf[G][NT][PP][2];
-#pragma unroll
-                for (int i = 0; i < G; ++i) {
-                    const float sa = vsa[i] * vinv, sb = vsb[i] * vinv;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) ob[nt][c][i] += p[nt][c] * vza[i] + p[nt][2 + c] * vzb[i];
-                        uint32_t ha[PP], hb[PP];
-                        parts_of<PP>(p[nt][0] * sa, p[nt][1] * sa, ha);
-                        parts_of<PP>(p[nt][2] * sb, p[nt][3] * sb, hb);
-#pragma unroll
-                        for (int x = 0; x < PP; ++x) {
-                            bf[i][nt][x][0] = movmatrix(ha[x]);
-                            bf[i][nt][x][1] = movmatrix(hb[x]);
-                        }
-                    }
-                }
-                const uint32_t* vw = reinterpret_cast<const uint32_t*>(st + C::VW);
-#pragma unroll
-                for (int m4 = 0; m4 < C::MT / 4; ++m4) {
-                    if constexpr (GROUP >= 64) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = vw[(t + 4 * i) * C::W + 8 * m4 + g];
-                        const uint32_t lo01 = prmt(w[0], w[1], 0x5410), hi01 = prmt(w[0], w[1], 0x7632);
-                        const uint32_t lo23 = prmt(w[2], w[3], 0x5410), hi23 = prmt(w[2], w[3], 0x7632);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t f[4] = {nib<HALF>(lo01, j), nib<HALF>(hi01, j), nib<HALF>(lo23, j), nib<HALF>(hi23, j)};
+                        for (int m = 0; m < C::MT; ++m)
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                                for (int x = 0; x < PP; ++x)
-                                    mma<HALF>(acc[4 * m4 + j][nt], f, bf[m4 * 64 / GROUP][nt][x][0], bf[m4 * 64 / GROUP][nt][x][1]);
+                                for (int c = 0; c < 4; ++c) acc[m][nt][c] *= f;
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < SUBS; ++b) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            p[b][nt][c] = ex2(p[b][nt][c]);
+                            l[nt][c & 1] += p[b][nt][c];
                         }
-                    } else {
-                        const uint32_t sel = g < 4 ? 0x5410 : 0x7632;
+                    uint32_t bf[G][NT][PP][2];
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            uint32_t w[4];
+                    for (int i = 0; i < G; ++i)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) w[i] = vw[(t + 4 * i) * C::W + 8 * m4 + 4 * q + (g & 3)];
-                            const uint32_t w01 = prmt(w[0], w[1], sel), w23 = prmt(w[2], w[3], sel);
+                        for (int h = 0; h < 2; ++h) {
+                            const float sc = vs[b][h][i] * vinv;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                uint32_t f[PP];
+                                parts_of<PP>(p[b][nt][2 * h] * sc, p[b][nt][2 * h + 1] * sc, f);
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) ob[nt][c][i] = fmaf(p[b][nt][2 * h + c], vz[b][h][i], ob[nt][c][i]);
+#pragma unroll
+                                for (int x = 0; x < PP; ++x) bf[i][nt][x][h] = movmatrix(f[x]);
+                            }
+                        }
+                    const uint32_t va = v_at + s * C::STAGE + b * C::BLOCK;
+#pragma unroll
+                    for (int c2 = 0; c2 < DH / 64; ++c2) {
+                        uint32_t w[4];              // 32 dims at positions 0..7 and 8..15, the next 32
+                        ldsm_trans(va + 32 * c2, w);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
-                                const uint32_t f[4] = {nib<HALF>(w01, 2 * j), nib<HALF>(w01, 2 * j + 1), nib<HALF>(w23, 2 * j), nib<HALF>(w23, 2 * j + 1)};
+                                const uint32_t f[4] = {nib<HALF>(w[2 * c], 2 * j), nib<HALF>(w[2 * c], 2 * j + 1),
+                                                       nib<HALF>(w[2 * c + 1], 2 * j), nib<HALF>(w[2 * c + 1], 2 * j + 1)};
+                                const int i = (2 * c2 + c) * 32 / GROUP;
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                                     for (int x = 0; x < PP; ++x)
-                                        mma<HALF>(acc[4 * m4 + 2 * q + j][nt], f, bf[2 * m4 + q][nt][x][0], bf[2 * m4 + q][nt][x][1]);
+                                        mma<HALF>(acc[4 * c2 + 2 * c + j][nt], f, bf[i][nt][x][0], bf[i][nt][x][1]);
                             }
-                        }
                     }
                 }
             }
@@ -598,6 +628,7 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
         }
 
         // ---- the warps' results of this part, joined ---------------------------------
+        const float back = pow2(vexp) * UNIT;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -613,17 +644,15 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                     for (int o = 4; o < 32; o <<= 1) bias[i] += __shfl_xor_sync(0xffffffffu, bias[i], o);
                 }
                 if (g == 0) {
-                    comb_m[warp * COLS + col] = ref[nt][c];
+                    comb_m[warp * COLS + col] = room[nt][c] == RAISE ? ref[nt][c] : -INFINITY;
                     comb_l[warp * COLS + col] = sum;
                 }
 #pragma unroll
                 for (int m = 0; m < C::MT; ++m)
 #pragma unroll
-                    for (int hi = 0; hi < 2; ++hi) {
-                        constexpr auto group_of_tile = [](int mm) { return GROUP >= 64 ? (mm >> 2) * 64 / GROUP : mm >> 1; };
+                    for (int hi = 0; hi < 2; ++hi)
                         comb[(warp * COLS + col) * C::LD + dim_of(m, hi)] =
-                            acc[m][nt][2 * hi + c] * 16777216.0f * pow2(vexp) + bias[group_of_tile(m)];
-                    }
+                            acc[m][nt][2 * hi + c] * (hi ? back / 16.0f : back) + bias[(m >> 1) * 32 / GROUP];
             }
         __syncthreads();
         const bool whole = u0 >= start && u1 <= end;

@@ -505,11 +505,8 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                 } else {
                     const uint32_t own = (tile - p.s.past) * KT + row;
                     const bool live = own < p.s.rq.n;
-#pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
-                        const __half* src = half ? static_cast<const __half*>(a.new_v) + (p.s.rq.token0 + own) * a.v_token + p.hk * a.v_head
-                                                 : static_cast<const __half*>(a.new_k) + (p.s.rq.token0 + own) * a.k_token + p.hk * a.k_head;
-                        uint4 x[W];
+                    const auto read_row = [&](const void* base, uint64_t token, uint64_t head, uint4 (&x)[W]) {
+                        const __half* src = static_cast<const __half*>(base) + (p.s.rq.token0 + own) * token + p.hk * head;
 #pragma unroll
                         for (int c = 0; c < W; ++c) {
                             x[c] = make_uint4(0u, 0u, 0u, 0u);
@@ -523,6 +520,32 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                                     x[c] = *reinterpret_cast<const uint4*>(h);
                                 }
                             }
+                        }
+                    };
+                    // A weight of zero does not keep an infinite or NaN value out of the
+                    // rows that are masked from it: such a value row is taken as zeros, and
+                    // its key as NaN, which reaches the rows that see it and no other.
+                    bool wild = false;
+                    {
+                        uint4 x[W];
+                        read_row(a.new_v, a.v_token, a.v_head, x);
+                        __half2 top = __half2half2(__ushort_as_half(0));
+#pragma unroll
+                        for (int c = 0; c < W; ++c) {
+                            const __half2* h = reinterpret_cast<const __half2*>(&x[c]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) top = __hmax2_nan(top, __habs2(h[i]));
+                        }
+                        wild = !(__low2float(top) <= 65504.0f && __high2float(top) <= 65504.0f);
+                    }
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        uint4 x[W];
+                        if (half) read_row(a.new_v, a.v_token, a.v_head, x);
+                        else read_row(a.new_k, a.k_token, a.k_head, x);
+                        if (wild) {
+#pragma unroll
+                            for (int c = 0; c < W; ++c) x[c].x = x[c].y = x[c].z = x[c].w = half ? 0u : 0x7FFF7FFFu;
                         }
                         if (use) wait(half ? &v_empty[st] : &k_empty[st], (use - 1) & 1, err);
                         unsigned char* d = half ? vd : kd;

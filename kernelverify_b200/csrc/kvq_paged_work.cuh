@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(Attend a, const u
     float o[V], l = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = 0.0f;
+    using Vec = typename std::conditional<V == 4, float4, float2>::type;
     for (uint32_t p0 = 0; p0 < u.parts; p0 += 32) {
         float w = 0.0f;
         if (p0 + lane < u.parts) {
@@ -127,12 +128,21 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(Attend a, const u
             l += w * part(p0 + lane)[COLS + col];
         }
         const uint32_t n = min(32u, u.parts - p0);
-#pragma unroll 8
-        for (uint32_t p = 0; p < n; ++p) {
-            const float f = __shfl_sync(0xffffffffu, w, p);
-            const float* s = part(p0 + p) + 2 * COLS + (size_t)col * DH + lane * V;
+        // sixteen parts' loads at a time
+        for (uint32_t q0 = 0; q0 < n; q0 += 16) {
+            Vec v[16];
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] += f * s[i];
+            for (int i = 0; i < 16; ++i)
+                if (q0 + i < n) v[i] = *reinterpret_cast<const Vec*>(part(p0 + q0 + i) + 2 * COLS + (size_t)col * DH + lane * V);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float f = __shfl_sync(0xffffffffu, w, (q0 + i) & 31);
+                if (q0 + i < n) {
+                    const float* x = reinterpret_cast<const float*>(&v[i]);
+#pragma unroll
+                    for (int d = 0; d < V; ++d) o[d] += f * x[d];
+                }
+            }
         }
     }
     l = warp_sum(l);

@@ -306,6 +306,22 @@ def test_attend_bad_pages_are_not_read(new):
             assert bool(((got[lo:hi].double() - want[lo:hi]).abs() <= tol[lo:hi]).all())
 
 
+@pytest.mark.parametrize("new, at", [(4, 2), (200, 130), (200, 3)])
+@pytest.mark.parametrize("what", ["nk", "nv"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_attend_keeps_later_tokens_out(new, at, what, value):
+    """A NaN or an infinity in an own entry reaches the tokens that see it and
+    none before it, nor another request."""
+    s = Step([60, 50], [new, 3], 2, 4, 128, 64, 16, F16, packed=False)
+    want, tol = s.reference()
+    getattr(s, what)[at, 1, 17] = value
+    got = s.call(paged)
+    off = (got.double() - want).abs() <= tol
+    assert bool(off[:at].all()) and bool(off[new:].all()) and bool(off[:new, :4].all())
+    if what == "nv" or value != value:
+        assert bool((~torch.isfinite(got[at:new, 4:])).any(-1).all())
+
+
 @pytest.mark.parametrize("new", [1, 70])
 def test_attend_cuts_to_its_bounds(new):
     """Lengths past max_ctx and negative ones are cut, not followed."""
