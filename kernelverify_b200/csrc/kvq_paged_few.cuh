@@ -459,31 +459,41 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
             if (valid > 0) {
                 float p[SUBS][NT][4];                      // rows g (0, 1) and g + 8, columns 2t, 2t + 1
                 float vs[SUBS][2][G], vz[SUBS][2][G];
+                // scores: blocks and groups are independent chains of MMAs, taken in turn
+                float sacc[SUBS][NT][G][4];
 #pragma unroll
-                for (int b = 0; b < SUBS; ++b) {
-                    const unsigned char* st = stage + b * C::BLOCK;
-                    float sacc[NT][G][4];
+                for (int b = 0; b < SUBS; ++b)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < G; ++i)
 #pragma unroll
-                            for (int c = 0; c < 4; ++c) sacc[nt][i][c] = 0.0f;
-                    const uint32_t* kw = reinterpret_cast<const uint32_t*>(st);
+                            for (int c = 0; c < 4; ++c) sacc[b][nt][i][c] = 0.0f;
+                constexpr int PER = C::SETS / G;           // runs of words per group
 #pragma unroll
-                    for (int u = 0; u < C::SETS; ++u) {
-                        const uint32_t wa = kw[g * C::W + word_of(u)], wb = kw[(g + 8) * C::W + word_of(u)];
+                for (int e = 0; e < PER; ++e)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint32_t f[4] = {nib<HALF>(wa, 2 * i), nib<HALF>(wb, 2 * i), nib<HALF>(wa, 2 * i + 1),
-                                                   nib<HALF>(wb, 2 * i + 1)};
+                    for (int b = 0; b < SUBS; ++b)
 #pragma unroll
-                            for (int x = 0; x < QP; ++x)
+                        for (int gi = 0; gi < G; ++gi) {
+                            const int u = gi * PER + e;
+                            static_assert(group_of(C::SETS - 1) == G - 1, "runs of a group are consecutive");
+                            const uint32_t* kw = reinterpret_cast<const uint32_t*>(stage + b * C::BLOCK);
+                            const uint32_t wa = kw[g * C::W + word_of(u)], wb = kw[(g + 8) * C::W + word_of(u)];
 #pragma unroll
-                                for (int nt = 0; nt < NT; ++nt)
-                                    mma<HALF>(sacc[nt][group_of(u)], f, qf[x][nt][u][2 * i], qf[x][nt][u][2 * i + 1]);
+                            for (int i = 0; i < 2; ++i) {
+                                const uint32_t f[4] = {nib<HALF>(wa, 2 * i), nib<HALF>(wb, 2 * i), nib<HALF>(wa, 2 * i + 1),
+                                                       nib<HALF>(wb, 2 * i + 1)};
+#pragma unroll
+                                for (int x = 0; x < QP; ++x)
+#pragma unroll
+                                    for (int nt = 0; nt < NT; ++nt)
+                                        mma<HALF>(sacc[b][nt][gi], f, qf[x][nt][u][2 * i], qf[x][nt][u][2 * i + 1]);
+                            }
                         }
-                    }
+#pragma unroll
+                for (int b = 0; b < SUBS; ++b) {
+                    const unsigned char* st = stage + b * C::BLOCK;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int at_pos = (g + 8 * h) * G;
@@ -503,10 +513,10 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                             for (int c = 0; c < 2; ++c) {
-                                float x = sacc[nt][0][2 * h + c] * ks[0], z = -ref[nt][c];
+                                float x = sacc[b][nt][0][2 * h + c] * ks[0], z = -ref[nt][c];
 #pragma unroll
                                 for (int i = 0; i < G; ++i) {
-                                    if (i) x = fmaf(sacc[nt][i][2 * h + c], ks[i], x);
+                                    if (i) x = fmaf(sacc[b][nt][i][2 * h + c], ks[i], x);
                                     z = fmaf(kz[i], qs[nt][c][i], z);
                                 }
                                 p[b][nt][2 * h + c] = fmaf(x, cs[nt][c], z);
@@ -607,18 +617,23 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                     for (int c2 = 0; c2 < DH / 64; ++c2) {
                         uint32_t w[4];              // 32 dims at positions 0..7 and 8..15, the next 32
                         ldsm_trans(va + 32 * c2, w);
+                        uint32_t f[4][4];
 #pragma unroll
-                        for (int c = 0; c < 2; ++c)
+                        for (int m = 0; m < 4; ++m) {
+                            const int c = m >> 1, j = m & 1;
+                            f[m][0] = nib<HALF>(w[2 * c], 2 * j);
+                            f[m][1] = nib<HALF>(w[2 * c], 2 * j + 1);
+                            f[m][2] = nib<HALF>(w[2 * c + 1], 2 * j);
+                            f[m][3] = nib<HALF>(w[2 * c + 1], 2 * j + 1);
+                        }
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                const uint32_t f[4] = {nib<HALF>(w[2 * c], 2 * j), nib<HALF>(w[2 * c], 2 * j + 1),
-                                                       nib<HALF>(w[2 * c + 1], 2 * j), nib<HALF>(w[2 * c + 1], 2 * j + 1)};
-                                const int i = (2 * c2 + c) * 32 / GROUP;
+                        for (int x = 0; x < PP; ++x)
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) {
+                                const int i = (2 * c2 + (m >> 1)) * 32 / GROUP;
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                    for (int x = 0; x < PP; ++x)
-                                        mma<HALF>(acc[4 * c2 + 2 * c + j][nt], f, bf[i][nt][x][0], bf[i][nt][x][1]);
+                                    mma<HALF>(acc[4 * c2 + m][nt], f[m], bf[i][nt][x][0], bf[i][nt][x][1]);
                             }
                     }
                 }
