@@ -46,11 +46,11 @@ Choice choose(const Attend& a) {
         for (uint64_t st : {a.q_token, a.q_head, a.k_token, a.k_head, a.v_token, a.v_head}) c.vec = c.vec && st * es % 16 == 0;
     }
     if (c.few_most) {
-        // no CTA for less than a round of its eight warps
+        // no CTA for less than a round of its warps
         const uint64_t few = c.few_most < a.max_new ? c.few_most : a.max_new, w = 8u * c.nt;
         const uint64_t tiles = rows * a.n_kv_heads * ((few * a.r + w - 1) / w) * ((uint64_t)a.max_ctx / 32 + 1);
         c.fits = c.fits && tiles < TOO_MANY;
-        c.few_grid = grid_for(tiles, 8, (a.dtype == KVQ_F16 && c.nt == 1 ? 2 : 1) * sms);
+        c.few_grid = grid_for(tiles, a.dtype == KVQ_F16 && c.nt == 1 ? 16 : 8, sms);
     }
     return c;
 }

@@ -5,8 +5,8 @@
 //
 // A warp takes 32 cached positions at a time, as two blocks of 16: it streams
 // them with cp.async.bulk into its own ring (a page holds whole blocks; no warp
-// waits for another), and keeps its own online softmax; the CTA's eight warps
-// are joined when a unit ends. With codes c, scales s, z = bias:
+// waits for another), and keeps its own online softmax; the CTA's warps are
+// joined when a unit ends. With codes c, scales s, z = bias:
 //
 //   scores   S^T[pos, col] = sum_g ks[pos,g] (sum_{d in g} c[pos,d] q[col,d])
 //                            + kz[pos,g] (sum_{d in g} q[col,d])
@@ -54,8 +54,6 @@ using mma4::mbar_init;
 using mma4::mbar_wait;
 using mma4::mma_f16;
 
-constexpr int CW = 8;                     // warps
-constexpr int THREADS = 32 * CW;
 constexpr int BLK = 16, SUBS = 2;          // positions per block, blocks per tile
 constexpr int TP = BLK * SUBS;
 constexpr float RAISE = 14.0f, START = 5.0f;   // log2 room above the reference
@@ -70,17 +68,21 @@ struct Cfg {
     static constexpr int MT = DH / 16;              // combine's 16-dim tiles
     static constexpr int QP = HALF ? 1 : 3, PP = HALF ? 2 : 3;
     static constexpr int COLS = 8 * NT;
+    // One CTA per SM: sixteen warps where 128 registers do, else eight. (Two CTAs
+    // of eight leave twice the parts to join, and the CTA that is launched later
+    // runs behind the other: 1 x 131072 took 60 us so.)
+    static constexpr int CW = HALF && NT == 1 ? 16 : 8, THREADS = 32 * CW;
+    static constexpr int HW = 8;                    // warps joined at once
     static constexpr int WB = BLK * W * 4, SB = BLK * G * (int)sizeof(T);
     static constexpr int VW = WB, KS = 2 * WB, KZ = KS + SB, VS = KZ + SB, VZ = VS + SB;
     static constexpr int BLOCK = VZ + SB;           // bytes of 16 positions
     static constexpr int STAGE = SUBS * BLOCK;
     static constexpr int NST = 2;                   // tiles per ring
     static constexpr int LD = DH + 4;               // floats per combined row (no bank conflicts)
-    static constexpr int COMB = CW * STAGE * NST;   // fp32 [CW][COLS][LD], then m and l [CW][COLS]
-    static constexpr int ML = COMB + CW * COLS * LD * 4;
+    static constexpr int COMB = CW * STAGE * NST;   // fp32 [HW][COLS][LD], then m and l [CW][COLS]
+    static constexpr int ML = COMB + HW * COLS * LD * 4;
     static constexpr int BAR = ML + 2 * CW * COLS * 4;
     static constexpr int BEFORE = BAR + CW * NST * 8 + 16;     // uint32 [rows + 1]
-    static constexpr int MIN_CTAS = NT == 1 && HALF ? 2 : 1;
     static_assert(STAGE % 16 == 0 && COMB % 16 == 0 && BAR % 8 == 0 && BEFORE % 16 == 0, "alignment");
 };
 
@@ -177,15 +179,18 @@ __device__ __forceinline__ void read8(const T* p, float (&x)[8]) {
 }
 
 template <typename T, int DH, int GROUP, int NT>
-__global__ void __launch_bounds__(THREADS, (Cfg<T, DH, GROUP, NT>::MIN_CTAS))
+__global__ void __launch_bounds__(Cfg<T, DH, GROUP, NT>::THREADS, 1)
 few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
     using C = Cfg<T, DH, GROUP, NT>;
-    constexpr int G = C::G, COLS = C::COLS, QP = C::QP, PP = C::PP;
+    constexpr int G = C::G, COLS = C::COLS, QP = C::QP, PP = C::PP, CW = C::CW, HW = C::HW, THREADS = C::THREADS;
     constexpr bool HALF = C::HALF;
     constexpr float UNIT = HALF ? 16777216.0f : 1.0f;      // a code in an MMA is c / UNIT, or 16 c / UNIT
     // exponents of the power of two above |vs|: from below what the quantizer
     // stores (its smallest step is 1e-7) to the type's largest
     constexpr int VEXP0 = HALF ? -14 : -30, VEXP1 = HALF ? 16 : 90;
+    // the join's CTAs may come as soon as there is room: none before these CTAs,
+    // which hold a whole SM's registers each, have left
+    pdl_launch_dependents();
     extern __shared__ __align__(128) unsigned char smem[];
     uint32_t* before = reinterpret_cast<uint32_t*>(smem + C::BEFORE);
     float* comb = reinterpret_cast<float*>(smem + C::COMB);
@@ -644,31 +649,69 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
 
         // ---- the warps' results of this part, joined ---------------------------------
         const float back = pow2(vexp) * UNIT;
+        float own_m[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int col = nt * 8 + 2 * t + c;
-                float bias[G], sum = l[nt][c];
+                float bias[G];
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                for (int o = 4; o < 32; o <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], o);
 #pragma unroll
                 for (int i = 0; i < G; ++i) {
                     bias[i] = ob[nt][c][i];
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) bias[i] += __shfl_xor_sync(0xffffffffu, bias[i], o);
                 }
-                if (g == 0) {
-                    comb_m[warp * COLS + col] = room[nt][c] == RAISE ? ref[nt][c] : -INFINITY;
-                    comb_l[warp * COLS + col] = sum;
-                }
+                own_m[nt][c] = room[nt][c] == RAISE ? ref[nt][c] : -INFINITY;
 #pragma unroll
                 for (int m = 0; m < C::MT; ++m)
 #pragma unroll
                     for (int hi = 0; hi < 2; ++hi)
-                        comb[(warp * COLS + col) * C::LD + dim_of(m, hi)] =
-                            acc[m][nt][2 * hi + c] * (hi ? back / 16.0f : back) + bias[(m >> 1) * 32 / GROUP];
+                        acc[m][nt][2 * hi + c] = acc[m][nt][2 * hi + c] * (hi ? back / 16.0f : back) + bias[(m >> 1) * 32 / GROUP];
             }
+        const auto leave = [&]() {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int col = nt * 8 + 2 * t + c;
+                    if (g == 0) {
+                        comb_m[warp * COLS + col] = own_m[nt][c];
+                        comb_l[warp * COLS + col] = l[nt][c];
+                    }
+#pragma unroll
+                    for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+                        for (int hi = 0; hi < 2; ++hi)
+                            comb[((warp % HW) * COLS + col) * C::LD + dim_of(m, hi)] = acc[m][nt][2 * hi + c];
+                }
+        };
+        if constexpr (CW > HW) {
+            // the upper half's results go to the lower half's warps first
+            if (warp >= HW) leave();
+            __syncthreads();
+            if (warp < HW) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int col = nt * 8 + 2 * t + c;
+                        const float m2 = comb_m[(warp + HW) * COLS + col], m = fmaxf(own_m[nt][c], m2);
+                        const float f = own_m[nt][c] == m ? 1.0f : ex2(own_m[nt][c] - m), f2 = m2 == m ? 1.0f : ex2(m2 - m);
+                        own_m[nt][c] = m;
+                        l[nt][c] = l[nt][c] * f + comb_l[(warp + HW) * COLS + col] * f2;
+#pragma unroll
+                        for (int k2 = 0; k2 < C::MT; ++k2)
+#pragma unroll
+                            for (int hi = 0; hi < 2; ++hi) {
+                                float& x = acc[k2][nt][2 * hi + c];
+                                x = x * f + comb[(warp * COLS + col) * C::LD + dim_of(k2, hi)] * f2;
+                            }
+                    }
+            }
+        }
+        if (warp < HW) leave();
         __syncthreads();
         const bool whole = u0 >= start && u1 <= end;
         float* slot = reinterpret_cast<float*>(ws + split_bytes(gridDim.x)) +
@@ -680,10 +723,10 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
             if (c >= n_cols) continue;
             float m = -INFINITY, sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < CW; ++w) m = fmaxf(m, comb_m[w * COLS + col]);
+            for (int w = 0; w < HW; ++w) m = fmaxf(m, comb_m[w * COLS + col]);
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < CW; ++w) {
+            for (int w = 0; w < HW; ++w) {
                 const float f = ex2(comb_m[w * COLS + col] - m);
                 const float4 x = *reinterpret_cast<const float4*>(&comb[(w * COLS + col) * C::LD + d]);
                 sum += f * comb_l[w * COLS + col];
@@ -714,7 +757,6 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
         __syncthreads();
         at = seg_end;
     }
-    pdl_launch_dependents();
 }
 
 template <typename T, int DH, int GROUP, int NT>
@@ -725,7 +767,7 @@ cudaError_t launch_few(const Attend& a, uint32_t most_new, uint32_t grid, void* 
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(kernel, C::BEFORE + (MAX_ROWS + 1) * 4, done);
     if (e != cudaSuccess) return e;
-    kernel<<<grid, THREADS, smem, stream>>>(a, most_new, static_cast<unsigned char*>(ws));
+    kernel<<<grid, C::THREADS, smem, stream>>>(a, most_new, static_cast<unsigned char*>(ws));
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     return launch_join<T, DH, C::COLS>(a, grid, static_cast<const unsigned char*>(ws), stream);

@@ -100,52 +100,91 @@ __device__ __forceinline__ uint32_t row_of_tile(const uint32_t* before, uint32_t
     return lo;
 }
 
-// A warp per (CTA of the split kernel, column): the unit's parts joined,
-// out = sum_p O_p 2^(m_p - m) / sum_p l_p 2^(m_p - m), m = max_p m_p in log2.
+// A block per (CTA of the split kernel, JOIN_COLS columns): the unit's parts
+// joined, out = sum_p O_p 2^(m_p - m) / sum_p l_p 2^(m_p - m), m = max_p m_p in
+// log2. A column's parts are shared out among several warps, whose loads do not
+// wait for the weights: a long sequence's unit has about 20 parts, and one warp
+// that walked them took 12 us.
 constexpr int JOIN_WARPS = 8;
 template <typename T, int DH, int COLS>
 __global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(Attend a, const unsigned char* __restrict__ ws) {
     constexpr int V = DH / 32;             // dims per lane
+    constexpr int PW = COLS > 32 ? 1 : 4;  // warps per column
+    constexpr int JC = JOIN_WARPS / PW;    // columns per block
+    constexpr int AHEAD = 5;               // parts a warp has in flight
     constexpr size_t SLOT = (size_t)COLS * (DH + 2);
+    using Vec = typename std::conditional<V == 4, float4, float2>::type;
+    __shared__ Vec sum_o[JOIN_WARPS][32];
+    __shared__ float sum_m[JOIN_WARPS], sum_l[JOIN_WARPS];
     pdl_wait();
-    const uint32_t cta = blockIdx.x, lane = threadIdx.x & 31, col = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5);
+    const uint32_t cta = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % PW;
+    const uint32_t col = blockIdx.y * JC + warp / PW;
     const Split u = reinterpret_cast<const Split*>(ws)[cta];
-    if (col >= COLS || u.parts == 0 || col >= u.cols) return;
+    if (u.parts == 0 || blockIdx.y * JC >= u.cols) return;
     const float* slots = reinterpret_cast<const float*>(ws + split_bytes(gridDim.x));
     // part 0 is this CTA's slot 1, part p > 0 CTA cta + p's slot 0
     const auto part = [&](uint32_t p) { return slots + (2 * (size_t)(cta + p) + (p == 0 ? 1 : 0)) * SLOT; };
-    float m = -INFINITY;
-    for (uint32_t p = lane; p < u.parts; p += 32) m = fmaxf(m, part(p)[col]);
-    m = warp_max(m);
-    float o[V], l = 0.0f;
+    float o[V], l = 0.0f, m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = 0.0f;
-    using Vec = typename std::conditional<V == 4, float4, float2>::type;
-    for (uint32_t p0 = 0; p0 < u.parts; p0 += 32) {
-        float w = 0.0f;
-        if (p0 + lane < u.parts) {
-            w = exp2f(part(p0 + lane)[col] - m);
-            l += w * part(p0 + lane)[COLS + col];
-        }
-        const uint32_t n = min(32u, u.parts - p0);
-        // sixteen parts' loads at a time
-        for (uint32_t q0 = 0; q0 < n; q0 += 16) {
-            Vec v[16];
+    if (col < u.cols)
+        for (uint32_t p0 = sub; p0 < u.parts; p0 += PW * AHEAD) {
+            Vec v[AHEAD];
+            float pm[AHEAD], pl[AHEAD], top = m;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (q0 + i < n) v[i] = *reinterpret_cast<const Vec*>(part(p0 + q0 + i) + 2 * COLS + (size_t)col * DH + lane * V);
+            for (int i = 0; i < AHEAD; ++i) {
+                const uint32_t p = p0 + i * PW;
+                pm[i] = -INFINITY;
+                if (p < u.parts) {
+                    const float* s = part(p);
+                    pm[i] = s[col];
+                    pl[i] = s[COLS + col];
+                    v[i] = *reinterpret_cast<const Vec*>(s + 2 * COLS + (size_t)col * DH + lane * V);
+                }
+            }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float f = __shfl_sync(0xffffffffu, w, (q0 + i) & 31);
-                if (q0 + i < n) {
+            for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, pm[i]);
+            const float keep = m == top ? 1.0f : exp2f(m - top);
+            m = top;
+            l *= keep;
+#pragma unroll
+            for (int d = 0; d < V; ++d) o[d] *= keep;
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                if (p0 + i * PW < u.parts) {
+                    const float f = exp2f(pm[i] - m);
                     const float* x = reinterpret_cast<const float*>(&v[i]);
+                    l += f * pl[i];
 #pragma unroll
                     for (int d = 0; d < V; ++d) o[d] += f * x[d];
                 }
-            }
+        }
+    if constexpr (PW > 1) {
+        sum_o[warp][lane] = *reinterpret_cast<const Vec*>(o);
+        if (lane == 0) {
+            sum_m[warp] = m;
+            sum_l[warp] = l;
+        }
+        __syncthreads();
+        if (sub != 0) return;
+        float top = m;
+#pragma unroll
+        for (int w = 1; w < PW; ++w) top = fmaxf(top, sum_m[warp + w]);
+        const float keep = exp2f(m - top);
+        l *= keep;
+#pragma unroll
+        for (int d = 0; d < V; ++d) o[d] *= keep;
+#pragma unroll
+        for (int w = 1; w < PW; ++w) {
+            const float f = exp2f(sum_m[warp + w] - top);
+            const Vec v = sum_o[warp + w][lane];
+            const float* x = reinterpret_cast<const float*>(&v);
+            l += f * sum_l[warp + w];
+#pragma unroll
+            for (int d = 0; d < V; ++d) o[d] += f * x[d];
         }
     }
-    l = warp_sum(l);
+    if (col >= u.cols) return;
     const uint32_t c = u.col0 + col, tok = u.token0 + c / a.r, head = u.hk * a.r + c % a.r;
     T* out = static_cast<T*>(a.out) + ((size_t)tok * a.n_heads + head) * DH + lane * V;
 #pragma unroll
@@ -172,7 +211,8 @@ cudaError_t allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
 template <typename T, int DH, int COLS>
 cudaError_t launch_join(const Attend& a, uint32_t grid, const unsigned char* ws, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid, (COLS + JOIN_WARPS - 1) / JOIN_WARPS);
+    constexpr int per_block = COLS > 32 ? JOIN_WARPS : JOIN_WARPS / 4;
+    cfg.gridDim = dim3(grid, (COLS + per_block - 1) / per_block);
     cfg.blockDim = dim3(32 * JOIN_WARPS);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
