@@ -4,8 +4,8 @@
 // bytes.
 //
 // A warp takes 32 cached positions at a time, as two blocks of 16: it streams
-// them with cp.async.bulk into its own ring (a page holds whole blocks; no warp
-// waits for another), and keeps its own online softmax; the CTA's warps are
+// them with 16-byte cp.async into its own ring (a page holds whole blocks; no
+// warp waits for another), and keeps its own online softmax; the CTA's warps are
 // joined when a unit ends. With codes c, scales s, z = bias:
 //
 //   scores   S^T[pos, col] = sum_g ks[pos,g] (sum_{d in g} c[pos,d] q[col,d])
@@ -46,12 +46,7 @@ namespace kvq {
 namespace paged {
 namespace few {
 
-using mma4::bulk_g2s;
 using mma4::ex2;
-using mma4::mbar_arrive;
-using mma4::mbar_expect_tx;
-using mma4::mbar_init;
-using mma4::mbar_wait;
 using mma4::mma_f16;
 
 constexpr int BLK = 16, SUBS = 2;          // positions per block, blocks per tile
@@ -81,9 +76,8 @@ struct Cfg {
     static constexpr int LD = DH + 4;               // floats per combined row (no bank conflicts)
     static constexpr int COMB = CW * STAGE * NST;   // fp32 [HW][COLS][LD], then m and l [CW][COLS]
     static constexpr int ML = COMB + HW * COLS * LD * 4;
-    static constexpr int BAR = ML + 2 * CW * COLS * 4;
-    static constexpr int BEFORE = BAR + CW * NST * 8 + 16;     // uint32 [rows + 1]
-    static_assert(STAGE % 16 == 0 && COMB % 16 == 0 && BAR % 8 == 0 && BEFORE % 16 == 0, "alignment");
+    static constexpr int BEFORE = ML + 2 * CW * COLS * 4;      // uint32 [rows + 1]
+    static_assert(STAGE % 16 == 0 && COMB % 16 == 0 && BEFORE % 16 == 0, "alignment");
 };
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
@@ -141,6 +135,9 @@ __device__ __forceinline__ void scales_of(const float* p, float (&x)[G]) {
 #pragma unroll
     for (int i = 0; i < G; ++i) x[i] = p[i];
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 // four 8 x 8 b16 tiles, transposed: lanes 8 i .. 8 i + 7 give tile i's rows;
 // lane (g, t) receives rows 2t (low half) and 2t + 1 of column g in x[i]
 __device__ __forceinline__ void ldsm_trans(uint32_t saddr, uint32_t (&x)[4]) {
@@ -196,19 +193,9 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
     float* comb = reinterpret_cast<float*>(smem + C::COMB);
     float* comb_m = reinterpret_cast<float*>(smem + C::ML);
     float* comb_l = comb_m + CW * COLS;
-    int* err = reinterpret_cast<int*>(smem + C::BEFORE - 16);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     unsigned char* ring = smem + warp * C::STAGE * C::NST;
-    uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::BAR) + warp * C::NST;
-
-    if (lane == 0) {
-        for (int s = 0; s < C::NST; ++s) mbar_init(&bar[s], 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (tid == 0) {
-        *err = 0;
-        reinterpret_cast<Split*>(ws)[blockIdx.x].parts = 0;
-    }
+    if (tid == 0) reinterpret_cast<Split*>(ws)[blockIdx.x].parts = 0;
     const uint32_t H = a.n_kv_heads;
     const auto tiles_in = [](uint32_t ctx) { return max(1u, (ctx + TP - 1) / TP); };
     const auto col_tiles = [&](const Request& r) { return r.n > most_new ? 0u : (r.n * a.r + COLS - 1) / COLS; };
@@ -248,30 +235,49 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
             row_at[i] = ((page * H + hk) << a.page_shift) + (pos & ((1u << a.page_shift) - 1));
         }
     };
-    // lanes 0..5 copy the first block's six runs, lanes 6..11 the second's
-    const int part = lane % 3, side = lane / 3 & 1, sub = lane / 6 & 1;
-    const Pool& pool = side ? a.v : a.k;
-    const unsigned char* src0 = part == 0 ? reinterpret_cast<const unsigned char*>(pool.words)
-                                          : static_cast<const unsigned char*>(part == 1 ? pool.scales : pool.biases);
-    const uint32_t row_bytes = part == 0 ? C::W * 4 : G * sizeof(T);
-    unsigned char* dst0 = ring + sub * C::BLOCK + (part == 0 ? side * C::WB : C::KS + (2 * side + part - 1) * C::SB);
-    const uint64_t policy = mma4::evict_first_policy();
+    // Every lane copies 16 bytes of each run. (A bulk copy per run takes its
+    // operands from uniform registers, so six lanes that issue one each are walked
+    // one after the other: 120 of 400 instructions per block.)
+    constexpr int WCH = C::WB / 16, SCH = C::SB / 16, ALL = 4 * SCH;   // chunks of a run, of the four scale runs
+    const unsigned char* kw0 = reinterpret_cast<const unsigned char*>(a.k.words) + lane * 16;
+    const unsigned char* vw0 = reinterpret_cast<const unsigned char*>(a.v.words) + lane * 16;
+    const unsigned char* sc0[(ALL + 31) / 32];
+#pragma unroll
+    for (int i = 0; i < (ALL + 31) / 32; ++i) {
+        const int chunk = lane + 32 * i, run = chunk / SCH;
+        const void* p = run == 0 ? a.k.scales : run == 1 ? a.k.biases : run == 2 ? a.v.scales : a.v.biases;
+        sc0[i] = static_cast<const unsigned char*>(p) + (chunk % SCH) * 16;
+    }
+    const uint32_t ring_at = mma4::s_addr(ring) + lane * 16;
     const uint32_t own = end - start > (uint32_t)warp ? (end - start - warp + CW - 1) / CW : 0;   // the warp's tiles
-    const auto fill = [&](uint32_t k) {
+    const auto fill_tile = [&](uint32_t k) {
         if (k >= own) return;
         if ((k & 31) == 0) look(k);
         const uint32_t r0 = __shfl_sync(0xffffffffu, row_at[0], k & 31), r1 = __shfl_sync(0xffffffffu, row_at[1], k & 31);
         const uint32_t what = __shfl_sync(0xffffffffu, held | bad_id << SUBS, k & 31);
         const uint32_t s = k % C::NST;
         bad = what >> SUBS ? bad | (1u << s) : bad & ~(1u << s);
-        const uint32_t n = __popc(what & ((1u << SUBS) - 1));
-        if (lane == 0) {
-            if (n) mbar_expect_tx(&bar[s], n * C::BLOCK);
-            else mbar_arrive(&bar[s]);
+#pragma unroll
+        for (int b = 0; b < SUBS; ++b) {
+            if (!(what >> b & 1)) break;
+            const uint64_t row = b ? r1 : r0;
+            const uint32_t to = ring_at + s * C::STAGE + b * C::BLOCK;
+#pragma unroll
+            for (int i = 0; i < (WCH + 31) / 32; ++i)
+                if (WCH >= 32 || lane < WCH) {
+                    copy16(to + 512 * i, kw0 + row * (C::W * 4) + 512 * i);
+                    copy16(to + C::VW + 512 * i, vw0 + row * (C::W * 4) + 512 * i);
+                }
+#pragma unroll
+            for (int i = 0; i < (ALL + 31) / 32; ++i)
+                if (lane + 32 * i < ALL) copy16(to + C::KS + 512 * i, sc0[i] + row * (G * sizeof(T)));
         }
-        __syncwarp();
-        if (lane < 6 * (int)n)
-            bulk_g2s(dst0 + s * C::STAGE, src0 + (uint64_t)(sub ? r1 : r0) * row_bytes, BLK * row_bytes, &bar[s], policy);
+    };
+    // one group of copies per tile, empty ones among them, so that a tile's copies
+    // are done when all but the last NST - 1 groups are
+    const auto fill = [&](uint32_t k) {
+        fill_tile(k);
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     for (int k = 0; k < C::NST; ++k) fill(k);
 
@@ -457,7 +463,8 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
         float vlim = pow2(vexp), vinv = pow2(-vexp);
         for (; k < own && start + warp + k * CW < seg_end; ++k) {
             const uint32_t s = k % C::NST;
-            if (!mbar_wait(&bar[s], (k / C::NST) & 1)) *err = 1;
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::NST - 1) : "memory");
+            __syncwarp();
             const unsigned char* stage = ring + s * C::STAGE;
             const uint32_t pos0 = (start + warp + k * CW - u0) * TP;
             const uint32_t valid = rq.ctx > pos0 ? rq.ctx - pos0 : 0;
@@ -716,7 +723,6 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
         const bool whole = u0 >= start && u1 <= end;
         float* slot = reinterpret_cast<float*>(ws + split_bytes(gridDim.x)) +
                       (2 * (size_t)blockIdx.x + (u0 >= start ? 1 : 0)) * slot_floats(COLS, DH);
-        const bool failed = *reinterpret_cast<volatile int*>(err) != 0;
         for (int i = tid; i < COLS * DH / 4; i += THREADS) {
             const int col = i / (DH / 4), d = i % (DH / 4) * 4;
             const uint32_t c = col0 + col;
@@ -735,7 +741,6 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                 o.z += f * x.z;
                 o.w += f * x.w;
             }
-            if (failed) o.x = o.y = o.z = o.w = NAN;
             if (whole) {
                 const uint32_t tok = rq.token0 + c / a.r, head = hk * a.r + c % a.r;
                 alignas(16) T v[4] = {from_f32<T>(o.x / sum), from_f32<T>(o.y / sum), from_f32<T>(o.z / sum),
