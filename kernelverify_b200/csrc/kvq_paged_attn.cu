@@ -13,7 +13,7 @@ namespace {
 
 struct Choice {
     uint32_t few_most;       // new tokens of a request up to which the few kernel takes it (0: none)
-    int nt;                  // its column tiles of 8
+    uint32_t cols;           // its query columns per pass
     uint32_t few_grid, many_grid;
     bool vec;
     bool fits;               // the tiles can be counted in 31 bits
@@ -30,11 +30,11 @@ Choice choose(const Attend& a) {
     const uint64_t cols = (uint64_t)a.max_new * a.r, sms = (uint64_t)sm_count();
     const uint64_t rows = a.rows < a.tokens ? a.rows : a.tokens;
     c.few_most = 0xFFFFFFFFu;
-    c.nt = a.dtype == KVQ_F16 && cols > 8 ? 2 : 1;
+    c.cols = a.dtype == KVQ_F32 ? 8 : cols <= 4 ? 4 : cols <= 8 ? 8 : 16;
     if (a.dtype == KVQ_F16 && a.r <= 128 && cols > 16) {
         // one request: the many kernel alone, whatever it brings
-        c.nt = 1;
-        c.few_most = a.rows == 1 ? 0 : (a.r >= 8 ? 1 : 8 / a.r);
+        c.cols = a.r <= 4 ? 4 : 8;
+        c.few_most = a.rows == 1 ? 0 : (a.r >= c.cols ? 1 : c.cols / a.r);
         // units have at most 256 query rows
         const uint64_t tu = 2 * (128 / a.r), units = (uint64_t)a.n_kv_heads * (a.tokens / tu + rows);
         const uint64_t tiles = units * (((uint64_t)a.max_ctx + a.max_new) / MANY_KEYS + 2);
@@ -46,18 +46,18 @@ Choice choose(const Attend& a) {
         for (uint64_t st : {a.q_token, a.q_head, a.k_token, a.k_head, a.v_token, a.v_head}) c.vec = c.vec && st * es % 16 == 0;
     }
     if (c.few_most) {
-        // no CTA for less than a round of its warps
-        const uint64_t few = c.few_most < a.max_new ? c.few_most : a.max_new, w = 8u * c.nt;
+        // no CTA for less than a tile per warp
+        const uint64_t few = c.few_most < a.max_new ? c.few_most : a.max_new, w = c.cols;
         const uint64_t tiles = rows * a.n_kv_heads * ((few * a.r + w - 1) / w) * ((uint64_t)a.max_ctx / 32 + 1);
         c.fits = c.fits && tiles < TOO_MANY;
-        c.few_grid = grid_for(tiles, a.dtype == KVQ_F16 && c.nt == 1 ? 16 : 8, sms);
+        c.few_grid = grid_for(tiles, a.dtype == KVQ_F16 && c.cols <= 8 ? 16 : 8, sms);
     }
     return c;
 }
 
 size_t few_bytes(const Attend& a, const Choice& c) {
     if (!c.few_most) return 0;
-    return (split_bytes(c.few_grid) + 2 * (size_t)c.few_grid * slot_floats(8u * c.nt, a.head_dim) * sizeof(float) + 255) / 256 * 256;
+    return (split_bytes(c.few_grid) + 2 * (size_t)c.few_grid * slot_floats(c.cols, a.head_dim) * sizeof(float) + 255) / 256 * 256;
 }
 size_t many_bytes(const Attend& a, const Choice& c) {
     if (!c.many_grid) return 0;
@@ -82,7 +82,7 @@ cudaError_t launch_attend(const Attend& a, void* ws, cudaStream_t s) {
         if (e != cudaSuccess) return e;
     }
     if (!c.few_most) return cudaSuccess;
-    if (a.dtype == KVQ_F16) return launch_few_f16(a, c.nt, c.few_most, c.few_grid, ws, s);
+    if (a.dtype == KVQ_F16) return launch_few_f16(a, c.cols, c.few_most, c.few_grid, ws, s);
     return launch_few_f32(a, c.few_most, c.few_grid, ws, s);
 }
 

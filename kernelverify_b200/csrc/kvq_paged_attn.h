@@ -7,9 +7,9 @@
 namespace kvq {
 namespace paged {
 
-// Requests with at most most_new new tokens, 8 nt query columns per pass over
-// the cache, on `grid` CTAs.
-cudaError_t launch_few_f16(const Attend& a, int nt, uint32_t most_new, uint32_t grid, void* ws, cudaStream_t s);
+// Requests with at most most_new new tokens, `cols` (4, 8 or 16; 8 for fp32)
+// query columns per pass over the cache, on `grid` CTAs.
+cudaError_t launch_few_f16(const Attend& a, uint32_t cols, uint32_t most_new, uint32_t grid, void* ws, cudaStream_t s);
 cudaError_t launch_few_f32(const Attend& a, uint32_t most_new, uint32_t grid, void* ws, cudaStream_t s);
 
 // Requests with at least least_new new tokens (at most 128 query heads per

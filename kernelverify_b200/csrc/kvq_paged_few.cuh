@@ -5,8 +5,10 @@
 //
 // A warp takes 32 cached positions at a time, as two blocks of 16: it streams
 // them with 16-byte cp.async into its own ring (a page holds whole blocks; no
-// warp waits for another), and keeps its own online softmax; the CTA's warps are
-// joined when a unit ends. With codes c, scales s, z = bias:
+// warp waits for another), and keeps its own online softmax. The CTA's share is
+// divided once more, into one run of tiles per warp: a unit inside one run is
+// finished by its warp, and the parts of the others are joined when the CTA's
+// warps are all done. With codes c, scales s, z = bias:
 //
 //   scores   S^T[pos, col] = sum_g ks[pos,g] (sum_{d in g} c[pos,d] q[col,d])
 //                            + kz[pos,g] (sum_{d in g} q[col,d])
@@ -26,6 +28,14 @@
 // a lane holds is free as long as both operands agree, and is chosen so that
 // the packed words are used where they are loaded. The weights p vs reach the
 // combine's B layout by one movmatrix per 8 x 8 block.
+//
+// Up to four columns (PAIR) leave half of an MMA's eight columns empty, and
+// with them half of every lane's softmax. They are then held twice: columns 0
+// to 3 stand for the tile's first block, 4 to 7 for its second. Scores are
+// taken from the MMAs of the one block or the other, everything from there to
+// the weights is done once for both, and the combine's MMAs of a block get the
+// other half's weights as zeros. The two halves are two online softmaxes, joined
+// at the end.
 //
 // Precision: products exact, sums fp32. The weights are carried as PP fp16
 // parts (2: 2^-22 relative, for fp16 steps; 3 for fp32 steps), held near the
@@ -53,8 +63,15 @@ constexpr int BLK = 16, SUBS = 2;          // positions per block, blocks per ti
 constexpr int TP = BLK * SUBS;
 constexpr float RAISE = 14.0f, START = 5.0f;   // log2 room above the reference
 
-template <typename T, int DH_, int GROUP_, int NT_>
+// A part of a unit that is not a warp's alone; cols = 0: none.
+struct Info {
+    uint32_t u0, u1, token0, hk, col0, cols;
+};
+
+template <typename T, int DH_, int GROUP_, int NT_, bool PAIR_>
 struct Cfg {
+    static constexpr bool PAIR = PAIR_;
+    static_assert(!PAIR_ || NT_ == 1, "paired columns are one tile");
     static constexpr int DH = DH_, GROUP = GROUP_, NT = NT_;
     static constexpr bool HALF = sizeof(T) == 2;
     static constexpr int G = DH / GROUP;
@@ -62,22 +79,25 @@ struct Cfg {
     static constexpr int SETS = DH / 32;            // runs of four words, one per lane of a quad
     static constexpr int MT = DH / 16;              // combine's 16-dim tiles
     static constexpr int QP = HALF ? 1 : 3, PP = HALF ? 2 : 3;
-    static constexpr int COLS = 8 * NT;
-    // One CTA per SM: sixteen warps where 128 registers do, else eight. (Two CTAs
-    // of eight leave twice the parts to join, and the CTA that is launched later
-    // runs behind the other: 1 x 131072 took 60 us so.)
-    static constexpr int CW = HALF && NT == 1 ? 16 : 8, THREADS = 32 * CW;
-    static constexpr int HW = 8;                    // warps joined at once
+    static constexpr int COLS = PAIR ? 4 : 8 * NT;
+    static constexpr int NB = PAIR ? 1 : SUBS;      // blocks whose weights a lane holds
+    // One CTA per SM, its warps as many as registers and shared memory allow. (Two
+    // CTAs of eight warps leave twice the parts to join, and the CTA that is
+    // launched later runs behind the other: 1 x 131072 took 60 us so.)
+    static constexpr int CW = HALF && NT == 1 ? (DH == 128 && G == 4 && !PAIR ? 12 : 16) : 8, THREADS = 32 * CW;
     static constexpr int WB = BLK * W * 4, SB = BLK * G * (int)sizeof(T);
     static constexpr int VW = WB, KS = 2 * WB, KZ = KS + SB, VS = KZ + SB, VZ = VS + SB;
     static constexpr int BLOCK = VZ + SB;           // bytes of 16 positions
     static constexpr int STAGE = SUBS * BLOCK;
     static constexpr int NST = 2;                   // tiles per ring
-    static constexpr int LD = DH + 4;               // floats per combined row (no bank conflicts)
-    static constexpr int COMB = CW * STAGE * NST;   // fp32 [HW][COLS][LD], then m and l [CW][COLS]
-    static constexpr int ML = COMB + HW * COLS * LD * 4;
-    static constexpr int BEFORE = ML + 2 * CW * COLS * 4;      // uint32 [rows + 1]
-    static_assert(STAGE % 16 == 0 && COMB % 16 == 0 && BEFORE % 16 == 0, "alignment");
+    static constexpr int PART = COLS * DH;          // floats of a part's O
+    static constexpr int HEADS = CW * STAGE * NST;  // fp32 [CW][COLS][DH]; the other parts lie in their warp's ring
+    static constexpr int ML = HEADS + CW * PART * 4;            // fp32 [2][CW][2][COLS]: m and l, head and tail
+    static constexpr int INFO = ML + 2 * CW * 2 * COLS * 4;     // Info [2][CW]
+    static constexpr int BEFORE = (INFO + 2 * CW * (int)sizeof(Info) + 15) / 16 * 16;   // uint32 [rows + 1]
+    static_assert(PART * 4 <= STAGE * NST, "a part fits a ring");
+    static_assert(BEFORE + (MAX_ROWS + 1) * 4 <= 232448, "shared memory");
+    static_assert(STAGE % 16 == 0 && HEADS % 16 == 0, "alignment");
 };
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
@@ -135,6 +155,10 @@ __device__ __forceinline__ void scales_of(const float* p, float (&x)[G]) {
 #pragma unroll
     for (int i = 0; i < G; ++i) x[i] = p[i];
 }
+__device__ __forceinline__ void store4(__half* p, float4 x) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack(x.x, x.y), pack(x.z, x.w));
+}
+__device__ __forceinline__ void store4(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -175,11 +199,12 @@ __device__ __forceinline__ void read8(const T* p, float (&x)[8]) {
     }
 }
 
-template <typename T, int DH, int GROUP, int NT>
-__global__ void __launch_bounds__(Cfg<T, DH, GROUP, NT>::THREADS, 1)
+template <typename T, int DH, int GROUP, int NT, bool PAIR>
+__global__ void __launch_bounds__(Cfg<T, DH, GROUP, NT, PAIR>::THREADS, 1)
 few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
-    using C = Cfg<T, DH, GROUP, NT>;
-    constexpr int G = C::G, COLS = C::COLS, QP = C::QP, PP = C::PP, CW = C::CW, HW = C::HW, THREADS = C::THREADS;
+    using C = Cfg<T, DH, GROUP, NT, PAIR>;
+    constexpr int NB = C::NB;
+    constexpr int G = C::G, COLS = C::COLS, QP = C::QP, PP = C::PP, CW = C::CW, THREADS = C::THREADS;
     constexpr bool HALF = C::HALF;
     constexpr float UNIT = HALF ? 16777216.0f : 1.0f;      // a code in an MMA is c / UNIT, or 16 c / UNIT
     // exponents of the power of two above |vs|: from below what the quantizer
@@ -190,9 +215,11 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
     pdl_launch_dependents();
     extern __shared__ __align__(128) unsigned char smem[];
     uint32_t* before = reinterpret_cast<uint32_t*>(smem + C::BEFORE);
-    float* comb = reinterpret_cast<float*>(smem + C::COMB);
-    float* comb_m = reinterpret_cast<float*>(smem + C::ML);
-    float* comb_l = comb_m + CW * COLS;
+    Info* info = reinterpret_cast<Info*>(smem + C::INFO);
+    const auto part_o = [&](int kind, int w) {      // kind 0: head (its unit began before the warp's run), 1: tail
+        return reinterpret_cast<float*>(kind ? smem + w * C::STAGE * C::NST : smem + C::HEADS + w * C::PART * 4);
+    };
+    const auto part_ml = [&](int kind, int w) { return reinterpret_cast<float*>(smem + C::ML) + (kind * CW + w) * 2 * COLS; };
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     unsigned char* ring = smem + warp * C::STAGE * C::NST;
     if (tid == 0) reinterpret_cast<Split*>(ws)[blockIdx.x].parts = 0;
@@ -203,11 +230,12 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
         const Request r = request_of(a, b);
         return (uint64_t)col_tiles(r) * H * tiles_in(r.ctx);
     });
-    // a whole round of the warps is the least a CTA takes
-    const uint32_t share = ((total + gridDim.x - 1) / gridDim.x + CW - 1) / CW * CW;
+    const uint32_t run = (total + gridDim.x * CW - 1) / (gridDim.x * CW), share = run * CW;   // tiles per warp and CTA
     const uint64_t start64 = (uint64_t)blockIdx.x * share;
     if (start64 >= total) return;
     const uint32_t start = (uint32_t)start64, end = min(total, start + share);
+    const uint32_t wstart = min(end, start + warp * run), wend = min(end, wstart + run), own = wend - wstart;
+    if (lane < 2) info[lane * CW + warp].cols = 0;
 
     // ---- the warp's stream of tiles -----------------------------------------
     // lane i looks up the batch's i-th tile: the cache row of each block, and per
@@ -215,10 +243,9 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
     uint32_t row_at[SUBS] = {0, 0}, held = 0, bad_id = 0;
     uint32_t bad = 0;                                  // stages with such a page
     const auto look = [&](uint32_t k0) {
-        const uint64_t x64 = (uint64_t)start + warp + (uint64_t)CW * (k0 + lane);
         held = bad_id = 0;
-        if (x64 >= end) return;
-        const uint32_t x = (uint32_t)x64;
+        if (k0 + lane >= own) return;
+        const uint32_t x = wstart + k0 + lane;
         const uint32_t b = row_of_tile(before, a.rows, x);
         const Request r = request_of(a, b);
         const uint32_t tiles = tiles_in(r.ctx), rem = x - before[b], unit = rem / tiles, hk = unit / col_tiles(r);
@@ -249,7 +276,6 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
         sc0[i] = static_cast<const unsigned char*>(p) + (chunk % SCH) * 16;
     }
     const uint32_t ring_at = mma4::s_addr(ring) + lane * 16;
-    const uint32_t own = end - start > (uint32_t)warp ? (end - start - warp + CW - 1) / CW : 0;   // the warp's tiles
     const auto fill_tile = [&](uint32_t k) {
         if (k >= own) return;
         if ((k & 31) == 0) look(k);
@@ -285,13 +311,13 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
     // this lane's row address for ldsm_trans: tiles (positions 0..7, 8..15) x (16 bytes, the next 16)
     const uint32_t v_at = mma4::s_addr(ring) + C::VW + (lane & 15) * (C::W * 4) + (lane >> 4) * 16;
     uint32_t k = 0;                                          // the warp's next tile
-    for (uint32_t at = start; at < end;) {
-        // ---- the unit this part of the share belongs to --------------------------
+    for (uint32_t at = wstart; at < wend;) {
+        // ---- the unit this part of the run belongs to ----------------------------
         const uint32_t b = row_of_tile(before, a.rows, at);
         const Request rq = request_of(a, b);
         const uint32_t tiles = tiles_in(rq.ctx), nct = col_tiles(rq);
         const uint32_t unit = (at - before[b]) / tiles, hk = unit / nct, col0 = (unit - hk * nct) * COLS;
-        const uint32_t u0 = before[b] + unit * tiles, u1 = u0 + tiles, seg_end = min(end, u1);
+        const uint32_t u0 = before[b] + unit * tiles, u1 = u0 + tiles, seg_end = min(wend, u1);
         const uint32_t n_cols = rq.n * a.r;
 
         // query fragments: lane (g, t) holds column g's dims of its words
@@ -301,7 +327,7 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
         constexpr auto group_of = [](int u) { return GROUP >= 64 ? (u >> 1) * 64 / GROUP : u; };
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const uint32_t c = col0 + nt * 8 + g;
+            const uint32_t c = col0 + nt * 8 + (PAIR ? g & 3 : g);
             float top = 0.0f, sum[G];
 #pragma unroll
             for (int i = 0; i < G; ++i) sum[i] = 0.0f;
@@ -390,13 +416,13 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
         // of the row's 16-bit unit; accumulators hold O UNIT / 2^vexp, times 16 for hi
         const auto dim_of = [&](int m, int hi) { return 32 * (m >> 1) + 4 * g + 2 * (m & 1) + hi; };
 
-        // ---- the step's own entries, in the share where the unit begins -----------
+        // ---- the step's own entries, in the run where the unit begins --------------
         // Entry j against every column: the quad's lanes hold column g's q.
         const auto own_entries = [&]() {
-            if (u0 < start) return;
+            if (u0 < wstart) return;
             const uint32_t last = min(rq.n, (col0 + COLS - 1) / a.r + 1);
             const float unit = pow2(-vexp) / UNIT;
-            for (uint32_t j = warp; j < last; j += CW) {
+            for (uint32_t j = 0; j < last; ++j) {
                 const T* nk = static_cast<const T*>(a.new_k) + (rq.token0 + j) * a.k_token + hk * a.k_head;
                 const T* nv = static_cast<const T*>(a.new_v) + (rq.token0 + j) * a.v_token + hk * a.v_head;
                 float dot[NT], dot16[NT];
@@ -433,8 +459,9 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                     for (int c = 0; c < 2; ++c) {
                         s[nt][c] = __shfl_sync(0xffffffffu, dot[nt], 8 * t + 4 * c) * (cs[nt][c] * (16.0f / UNIT)) - ref[nt][c];
                         const uint32_t col = col0 + nt * 8 + 2 * t + c;
-                        // columns past the last one are zero queries: any weight will do
-                        sees[nt][c] = col >= n_cols || j <= col / a.r;
+                        // columns past the last one are zero queries: any weight will do; a
+                        // paired column counts its own entries once
+                        sees[nt][c] = PAIR && t >= 2 ? false : col >= n_cols || j <= col / a.r;
                         if (!sees[nt][c]) s[nt][c] = -INFINITY;
                     }
 #pragma unroll
@@ -461,16 +488,16 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
 
         // ---- the cached tiles ------------------------------------------------------
         float vlim = pow2(vexp), vinv = pow2(-vexp);
-        for (; k < own && start + warp + k * CW < seg_end; ++k) {
+        for (; wstart + k < seg_end; ++k) {
             const uint32_t s = k % C::NST;
             asm volatile("cp.async.wait_group %0;" ::"n"(C::NST - 1) : "memory");
             __syncwarp();
             const unsigned char* stage = ring + s * C::STAGE;
-            const uint32_t pos0 = (start + warp + k * CW - u0) * TP;
+            const uint32_t pos0 = (wstart + k - u0) * TP;
             const uint32_t valid = rq.ctx > pos0 ? rq.ctx - pos0 : 0;
             if (valid > 0) {
-                float p[SUBS][NT][4];                      // rows g (0, 1) and g + 8, columns 2t, 2t + 1
-                float vs[SUBS][2][G], vz[SUBS][2][G];
+                float p[NB][NT][4];                      // rows g (0, 1) and g + 8, columns 2t, 2t + 1
+                float vs[NB][2][G], vz[NB][2][G];
                 // scores: blocks and groups are independent chains of MMAs, taken in turn
                 float sacc[SUBS][NT][G][4];
 #pragma unroll
@@ -504,8 +531,14 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                             }
                         }
 #pragma unroll
-                for (int b = 0; b < SUBS; ++b) {
-                    const unsigned char* st = stage + b * C::BLOCK;
+                for (int b = 0; b < NB; ++b) {
+                    const unsigned char* st = stage + (PAIR ? t >> 1 : b) * C::BLOCK;
+                    if (PAIR) {
+#pragma unroll
+                        for (int i = 0; i < G; ++i)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) sacc[0][0][i][c] = t < 2 ? sacc[0][0][i][c] : sacc[1][0][i][c];
+                    }
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int at_pos = (g + 8 * h) * G;
@@ -538,10 +571,10 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                 if (valid < TP) {
                     // rows past the length may hold anything
 #pragma unroll
-                    for (int b = 0; b < SUBS; ++b)
+                    for (int b = 0; b < NB; ++b)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            if ((uint32_t)(b * BLK + 8 * h + g) < valid) continue;
+                            if ((uint32_t)((PAIR ? t >> 1 : b) * BLK + 8 * h + g) < valid) continue;
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) p[b][nt][2 * h] = p[b][nt][2 * h + 1] = -INFINITY;
 #pragma unroll
@@ -550,7 +583,7 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                 }
                 if (bad & (1u << s)) {
 #pragma unroll
-                    for (int b = 0; b < SUBS; ++b)
+                    for (int b = 0; b < NB; ++b)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -562,7 +595,8 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        top[nt][c] = fmaxf(fmaxf(p[0][nt][c], p[0][nt][2 + c]), fmaxf(p[1][nt][c], p[1][nt][2 + c]));
+                        top[nt][c] = fmaxf(p[0][nt][c], p[0][nt][2 + c]);
+                        if (!PAIR) top[nt][c] = fmaxf(top[nt][c], fmaxf(p[NB - 1][nt][c], p[NB - 1][nt][2 + c]));
                         over |= top[nt][c] > room[nt][c];
                     }
                 if (__any_sync(0xffffffffu, over)) {
@@ -574,14 +608,14 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                             for (int o = 4; o < 32; o <<= 1) top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(0xffffffffu, top[nt][c], o));
                             const float by = raise(nt, c, top[nt][c]);
 #pragma unroll
-                            for (int b = 0; b < SUBS; ++b) {
+                            for (int b = 0; b < NB; ++b) {
                                 p[b][nt][c] -= by;
                                 p[b][nt][2 + c] -= by;
                             }
                         }
                 }
 #pragma unroll
-                for (int b = 0; b < SUBS; ++b)
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int i = 0; i < G; ++i) vtop = fmaxf(vtop, fmaxf(fabsf(vs[b][0][i]), fabsf(vs[b][1][i])));
                 if (__any_sync(0xffffffffu, vtop >= vlim)) {
@@ -599,8 +633,10 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                                 for (int c = 0; c < 4; ++c) acc[m][nt][c] *= f;
                     }
                 }
+                uint32_t bf[G][NT][PP][2];
 #pragma unroll
                 for (int b = 0; b < SUBS; ++b) {
+                    if (!PAIR || b == 0) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -608,7 +644,6 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                             p[b][nt][c] = ex2(p[b][nt][c]);
                             l[nt][c & 1] += p[b][nt][c];
                         }
-                    uint32_t bf[G][NT][PP][2];
 #pragma unroll
                     for (int i = 0; i < G; ++i)
 #pragma unroll
@@ -624,6 +659,16 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                                 for (int x = 0; x < PP; ++x) bf[i][nt][x][h] = movmatrix(f[x]);
                             }
                         }
+                    }
+                    uint32_t bm[G][NT][PP][2];              // the weights of this block
+#pragma unroll
+                    for (int i = 0; i < G; ++i)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int x = 0; x < PP; ++x)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) bm[i][nt][x][h] = !PAIR || (g >> 2) == b ? bf[i][nt][x][h] : 0u;
                     const uint32_t va = v_at + s * C::STAGE + b * C::BLOCK;
 #pragma unroll
                     for (int c2 = 0; c2 < DH / 64; ++c2) {
@@ -645,7 +690,7 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                                 const int i = (2 * c2 + (m >> 1)) * 32 / GROUP;
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt)
-                                    mma<HALF>(acc[4 * c2 + m][nt], f[m], bf[i][nt][x][0], bf[i][nt][x][1]);
+                                    mma<HALF>(acc[4 * c2 + m][nt], f[m], bm[i][nt][x][0], bm[i][nt][x][1]);
                             }
                     }
                 }
@@ -654,7 +699,7 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
             fill(k + C::NST);
         }
 
-        // ---- the warps' results of this part, joined ---------------------------------
+        // ---- the part's result -------------------------------------------------------
         const float back = pow2(vexp) * UNIT;
         float own_m[NT][2];
 #pragma unroll
@@ -677,77 +722,95 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                     for (int hi = 0; hi < 2; ++hi)
                         acc[m][nt][2 * hi + c] = acc[m][nt][2 * hi + c] * (hi ? back / 16.0f : back) + bias[(m >> 1) * 32 / GROUP];
             }
-        const auto leave = [&]() {
+        if (PAIR) {
+            // the second block's columns are two lanes on in the quad
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const float m2 = __shfl_xor_sync(0xffffffffu, own_m[0][c], 2), m = fmaxf(own_m[0][c], m2);
+                const float l2 = __shfl_xor_sync(0xffffffffu, l[0][c], 2);
+                const float f = own_m[0][c] == m ? 1.0f : ex2(own_m[0][c] - m), f2 = m2 == m ? 1.0f : ex2(m2 - m);
+                own_m[0][c] = m;
+                l[0][c] = l[0][c] * f + l2 * f2;
+#pragma unroll
+                for (int k2 = 0; k2 < C::MT; ++k2)
+#pragma unroll
+                    for (int hi = 0; hi < 2; ++hi) {
+                        float& x = acc[k2][0][2 * hi + c];
+                        const float y = __shfl_xor_sync(0xffffffffu, x, 2);
+                        x = x * f + y * f2;
+                    }
+            }
+        }
+        const bool writes = !PAIR || t < 2, head = u0 < wstart;
+        if (!head && u1 <= wend) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t cc = col0 + nt * 8 + 2 * t + c;
+                    if (!writes || cc >= n_cols) continue;
+                    const float inv = 1.0f / l[nt][c];
+                    T* out = static_cast<T*>(a.out) + ((size_t)(rq.token0 + cc / a.r) * a.n_heads + hk * a.r + cc % a.r) * DH;
+#pragma unroll
+                    for (int m = 0; m < C::MT; m += 2)
+                        store4(out + dim_of(m, 0), make_float4(acc[m][nt][c] * inv, acc[m][nt][2 + c] * inv,
+                                                               acc[m + 1][nt][c] * inv, acc[m + 1][nt][2 + c] * inv));
+                }
+        } else {
+            __syncwarp();                           // a tail lies in the ring, which is done with
+            float* o = part_o(!head, warp);
+            float* ml = part_ml(!head, warp);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const int col = nt * 8 + 2 * t + c;
+                    if (!writes) continue;
                     if (g == 0) {
-                        comb_m[warp * COLS + col] = own_m[nt][c];
-                        comb_l[warp * COLS + col] = l[nt][c];
+                        ml[col] = own_m[nt][c];
+                        ml[COLS + col] = l[nt][c];
                     }
 #pragma unroll
-                    for (int m = 0; m < C::MT; ++m)
-#pragma unroll
-                        for (int hi = 0; hi < 2; ++hi)
-                            comb[((warp % HW) * COLS + col) * C::LD + dim_of(m, hi)] = acc[m][nt][2 * hi + c];
+                    for (int m = 0; m < C::MT; m += 2)
+                        *reinterpret_cast<float4*>(&o[col * DH + dim_of(m, 0)]) =
+                            make_float4(acc[m][nt][c], acc[m][nt][2 + c], acc[m + 1][nt][c], acc[m + 1][nt][2 + c]);
                 }
-        };
-        if constexpr (CW > HW) {
-            // the upper half's results go to the lower half's warps first
-            if (warp >= HW) leave();
-            __syncthreads();
-            if (warp < HW) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int col = nt * 8 + 2 * t + c;
-                        const float m2 = comb_m[(warp + HW) * COLS + col], m = fmaxf(own_m[nt][c], m2);
-                        const float f = own_m[nt][c] == m ? 1.0f : ex2(own_m[nt][c] - m), f2 = m2 == m ? 1.0f : ex2(m2 - m);
-                        own_m[nt][c] = m;
-                        l[nt][c] = l[nt][c] * f + comb_l[(warp + HW) * COLS + col] * f2;
-#pragma unroll
-                        for (int k2 = 0; k2 < C::MT; ++k2)
-#pragma unroll
-                            for (int hi = 0; hi < 2; ++hi) {
-                                float& x = acc[k2][nt][2 * hi + c];
-                                x = x * f + comb[(warp * COLS + col) * C::LD + dim_of(k2, hi)] * f2;
-                            }
-                    }
-            }
+            if (lane == 0)
+                info[(head ? 0 : CW) + warp] = {u0, u1, rq.token0, hk, col0, min((uint32_t)COLS, n_cols - col0)};
         }
-        if (warp < HW) leave();
-        __syncthreads();
-        const bool whole = u0 >= start && u1 <= end;
-        float* slot = reinterpret_cast<float*>(ws + split_bytes(gridDim.x)) +
-                      (2 * (size_t)blockIdx.x + (u0 >= start ? 1 : 0)) * slot_floats(COLS, DH);
-        for (int i = tid; i < COLS * DH / 4; i += THREADS) {
+        at = seg_end;
+    }
+
+    // ---- the parts of units that several warps shared, joined in their order ----------
+    __syncthreads();
+    float* slots = reinterpret_cast<float*>(ws + split_bytes(gridDim.x)) + 2 * (size_t)blockIdx.x * slot_floats(COLS, DH);
+    for (int first = -1; first < CW; ++first) {
+        // a unit's first part here: warp 0's head (the unit began before the share) or a tail
+        const Info u = info[first < 0 ? 0 : CW + first];
+        if (u.cols == 0) continue;
+        const int w0 = max(first, 0), w1 = (int)((min(u.u1, end) - 1 - start) / run);
+        const bool whole = u.u0 >= start && u.u1 <= end;
+        float* slot = slots + (u.u0 >= start ? slot_floats(COLS, DH) : 0);
+        for (int i = tid; i < (int)u.cols * (DH / 4); i += THREADS) {
             const int col = i / (DH / 4), d = i % (DH / 4) * 4;
-            const uint32_t c = col0 + col;
-            if (c >= n_cols) continue;
-            float m = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < HW; ++w) m = fmaxf(m, comb_m[w * COLS + col]);
+            float m = part_ml(first >= 0, w0)[col];
+            for (int w = w0 + 1; w <= w1; ++w) m = fmaxf(m, part_ml(0, w)[col]);
+            float sum = 0.0f;
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int w = 0; w < HW; ++w) {
-                const float f = ex2(comb_m[w * COLS + col] - m);
-                const float4 x = *reinterpret_cast<const float4*>(&comb[(w * COLS + col) * C::LD + d]);
-                sum += f * comb_l[w * COLS + col];
+            for (int w = w0; w <= w1; ++w) {
+                const int kind = w == w0 && first >= 0;
+                const float f = ex2(part_ml(kind, w)[col] - m);
+                const float4 x = *reinterpret_cast<const float4*>(&part_o(kind, w)[col * DH + d]);
+                sum += f * part_ml(kind, w)[COLS + col];
                 o.x += f * x.x;
                 o.y += f * x.y;
                 o.z += f * x.z;
                 o.w += f * x.w;
             }
             if (whole) {
-                const uint32_t tok = rq.token0 + c / a.r, head = hk * a.r + c % a.r;
-                alignas(16) T v[4] = {from_f32<T>(o.x / sum), from_f32<T>(o.y / sum), from_f32<T>(o.z / sum),
-                                      from_f32<T>(o.w / sum)};
-                T* dst = static_cast<T*>(a.out) + ((size_t)tok * a.n_heads + head) * DH + d;
-                if constexpr (HALF) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(v);
-                else *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+                const uint32_t c = u.col0 + col, tok = u.token0 + c / a.r, hd = u.hk * a.r + c % a.r;
+                store4(static_cast<T*>(a.out) + ((size_t)tok * a.n_heads + hd) * DH + d,
+                       make_float4(o.x / sum, o.y / sum, o.z / sum, o.w / sum));
             } else {
                 *reinterpret_cast<float4*>(&slot[2 * COLS + col * DH + d]) = o;
                 if (d == 0) {
@@ -756,19 +819,16 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                 }
             }
         }
-        if (tid == 0 && u0 >= start && u1 > end)
-            reinterpret_cast<Split*>(ws)[blockIdx.x] = {(u1 - 1) / share - blockIdx.x + 1, rq.token0, hk, col0,
-                                                        min((uint32_t)COLS, n_cols - col0)};
-        __syncthreads();
-        at = seg_end;
+        if (tid == 0 && u.u0 >= start && u.u1 > end)
+            reinterpret_cast<Split*>(ws)[blockIdx.x] = {(u.u1 - 1) / share - blockIdx.x + 1, u.token0, u.hk, u.col0, u.cols};
     }
 }
 
-template <typename T, int DH, int GROUP, int NT>
+template <typename T, int DH, int GROUP, int NT, bool PAIR>
 cudaError_t launch_few(const Attend& a, uint32_t most_new, uint32_t grid, void* ws, cudaStream_t stream) {
-    using C = Cfg<T, DH, GROUP, NT>;
+    using C = Cfg<T, DH, GROUP, NT, PAIR>;
     const size_t smem = C::BEFORE + ((size_t)a.rows + 1) * 4;
-    auto kernel = few_kernel<T, DH, GROUP, NT>;
+    auto kernel = few_kernel<T, DH, GROUP, NT, PAIR>;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(kernel, C::BEFORE + (MAX_ROWS + 1) * 4, done);
     if (e != cudaSuccess) return e;
