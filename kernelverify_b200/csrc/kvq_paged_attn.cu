@@ -50,7 +50,7 @@ Choice choose(const Attend& a) {
         const uint64_t few = c.few_most < a.max_new ? c.few_most : a.max_new, w = c.cols;
         const uint64_t tiles = rows * a.n_kv_heads * ((few * a.r + w - 1) / w) * ((uint64_t)a.max_ctx / 32 + 1);
         c.fits = c.fits && tiles < TOO_MANY;
-        c.few_grid = grid_for(tiles, a.dtype == KVQ_F16 && c.cols <= 8 ? 16 : 8, sms);
+        c.few_grid = grid_for(tiles, a.dtype == KVQ_F16 && c.cols <= 8 ? 12 : 8, sms);
     }
     return c;
 }

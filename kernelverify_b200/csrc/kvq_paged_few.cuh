@@ -84,7 +84,7 @@ struct Cfg {
     // One CTA per SM, its warps as many as registers and shared memory allow. (Two
     // CTAs of eight warps leave twice the parts to join, and the CTA that is
     // launched later runs behind the other: 1 x 131072 took 60 us so.)
-    static constexpr int CW = HALF && NT == 1 ? (DH == 128 && G == 4 && !PAIR ? 12 : 16) : 8, THREADS = 32 * CW;
+    static constexpr int CW = HALF && NT == 1 ? 12 : 8, THREADS = 32 * CW;
     static constexpr int WB = BLK * W * 4, SB = BLK * G * (int)sizeof(T);
     static constexpr int VW = WB, KS = 2 * WB, KZ = KS + SB, VS = KZ + SB, VZ = VS + SB;
     static constexpr int BLOCK = VZ + SB;           // bytes of 16 positions
