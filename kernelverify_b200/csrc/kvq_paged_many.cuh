@@ -16,14 +16,13 @@
 //         an online softmax whose reference moves (and rescales O) only when
 //         the row's maximum passed it by 2^14, P back to tensor memory; at the
 //         end O / l to the output, or the unit's part to the workspace
-//   2     loads: a thread per key; 4-bit rows become fp16 by one HFMA2 per two
-//         codes, stored with the 128-byte swizzle the MMAs read
+//   2     loads: cached rows a thread per key, the next tile's words on their way
+//         while this one's become fp16; own entries by 16-byte asynchronous
+//         copies; all stored with the 128-byte swizzle the MMAs read
 //   3     one thread issues the MMAs
 // While one M tile is in its softmax the tensor cores work for the other. K
 // and V tiles have the same layout, rows of keys: K is read as a K-major
-// operand, V as an MN-major one. Within each run of eight dims, operands hold
-// them in the order 0 4 1 5 2 6 3 7 that unpacking a word gives; scores do not
-// depend on it and the output is put back in order.
+// operand, V as an MN-major one.
 //
 // Rounded to fp16: the dequantized K and V (as a cache held in fp16 would be)
 // and the weights P; everything else is fp32. P is at most 2^14 and its sum is
@@ -149,26 +148,24 @@ __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile in
     *err = 1;
 }
 
-// eight fp16 in natural order -> the operands' order 0 4 1 5 2 6 3 7
-__device__ __forceinline__ uint4 reorder(uint4 x) {
-    return make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410),
-                      __byte_perm(x.y, x.w, 0x7632));
-}
-// a word's eight codes -> fp16 scale * code + bias, rounded once: 1024 + c (or
-// 1024 + 16 c) is exact, and so is c after one subtraction (or multiply-add)
+// a word's eight codes -> fp16 scale * code + bias, rounded once. A byte in both
+// halves gives codes 2k and 2k + 1 as 1024 + c and 1024 + 16 c', exact, one
+// HFMA2 makes them c and c', exact, and another the values.
 __device__ __forceinline__ uint4 values_of(uint32_t w, __half2 s, __half2 z) {
-    const __half2 big = __half2half2(__ushort_as_half(0x6400)), one16 = __half2half2(__ushort_as_half(0x2C00)),
-                  m64 = __half2half2(__ushort_as_half(0xD400));
-    uint32_t x[4] = {and_or<0x000F000Fu, 0x64006400u>(w), and_or<0x00F000F0u, 0x64006400u>(w),
-                     and_or<0x000F000Fu, 0x64006400u>(w >> 8), and_or<0x00F000F0u, 0x64006400u>(w >> 8)};
+    const __half2 mul = __halves2half2(__ushort_as_half(0x3C00), __ushort_as_half(0x2C00));    // 1, 1/16
+    const __half2 sub = __halves2half2(__ushort_as_half(0xE400), __ushort_as_half(0xD400));    // -1024, -64
+    uint32_t x[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        __half2 h = *reinterpret_cast<__half2*>(&x[i]);
-        h = i & 1 ? __hfma2(h, one16, m64) : __hsub2(h, big);
-        h = __hfma2(h, s, z);
-        x[i] = *reinterpret_cast<uint32_t*>(&h);
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t b = and_or<0x00F0000Fu, 0x64006400u>(__byte_perm(w, 0, k * 0x0101));
+        const __half2 v = __hfma2(__hfma2(*reinterpret_cast<const __half2*>(&b), mul, sub), s, z);
+        x[k] = *reinterpret_cast<const uint32_t*>(&v);
     }
     return make_uint4(x[0], x[1], x[2], x[3]);
+}
+// 16 bytes to shared memory, or 16 zeros
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
 // sum_{i=0}^{n-1} floor((a i + b) / 128)
@@ -327,7 +324,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                             x = *reinterpret_cast<const uint4*>(h);
                         }
                     }
-                    *reinterpret_cast<uint4*>(dst + (c >> 3) * C::PANEL + swizzled(row, c & 7)) = reorder(x);
+                    *reinterpret_cast<uint4*>(dst + (c >> 3) * C::PANEL + swizzled(row, c & 7)) = x;
                 }
                 fence_async_smem();
                 __syncwarp();
@@ -413,10 +410,9 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
                     if (!live) break;
-                    // columns hold dims 0 4 1 5 2 6 3 7
                     float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[(e >> 1) + 4 * (e & 1)] = __uint_as_float(o[i + e]) * inv;
+                    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(o[i + e]) * inv;
                     if (whole) {
                         alignas(16) __half2 h[4];
 #pragma unroll
@@ -442,121 +438,132 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
         // ------------------------------ loads -------------------------------------
         regs_dec<REG_LOAD>();
         const uint32_t row = tid & 127;
+        const auto filled = [&](uint64_t* bar) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
         uint32_t done = 0;
         for (uint32_t at = start; at < end;) {
             const Part p = part_at(a, before, least_new, at, end);
             at = p.hi;
-            for (uint32_t j = p.lo; j < p.hi; ++j, ++done) {
-                const uint32_t st = done % STAGES, use = done / STAGES, tile = j - p.u0;
+            // ---- cached tiles: this thread's key of each -----------------------------
+            const uint32_t t0 = p.lo - p.u0, tn = min(p.hi - p.u0, p.s.past);      // tiles [t0, tn)
+            const int32_t* table = a.block_tables + (size_t)p.b * a.width;
+            const auto page_of = [&](uint32_t tile) {                      // 0 past the length: not used
+                const uint32_t pos = tile * KT + row;
+                return tile < tn && pos < p.s.rq.ctx ? (uint32_t)table[pos >> a.page_shift] : 0u;
+            };
+            // a key's packed row, and whether there is one (0 none, 1 a row, 2 a page id
+            // outside the pool)
+            uint4 kw[W / 4], vw[W / 4];
+            __half ks[G], kz[G], vs[G], vz[G];
+            const auto row_of = [&](uint32_t tile, uint32_t page, uint32_t& kind) {
+                const uint32_t pos = tile * KT + row;
+                kind = tile < tn && pos < p.s.rq.ctx ? (page < a.pages ? 1 : 2) : 0;
+                return (((kind == 1 ? page : 0u) * a.n_kv_heads + p.hk) << a.page_shift) + (pos & ((1u << a.page_shift) - 1));
+            };
+            const auto read = [&](uint32_t kind, uint64_t r, const Pool& pool, uint4 (&w)[W / 4], __half (&s)[G], __half (&z)[G]) {
+                // keys past the length: zeros, which the mask (K) and the zero weights (V)
+                // leave without effect
+#pragma unroll
+                for (int i = 0; i < W / 4; ++i) w[i] = kind ? reinterpret_cast<const uint4*>(pool.words + r * W)[i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                for (int i = 0; i < G; ++i) {
+                    s[i] = kind ? static_cast<const __half*>(pool.scales)[r * G + i] : __ushort_as_half(0);
+                    z[i] = kind ? static_cast<const __half*>(pool.biases)[r * G + i] : __ushort_as_half(0);
+                }
+            };
+            const auto put = [&](unsigned char* d, const uint4 (&w)[W / 4], const __half (&s)[G], const __half (&z)[G]) {
+#pragma unroll
+                for (int c = 0; c < W; ++c) {
+                    const uint32_t word = c % 4 == 0 ? w[c / 4].x : c % 4 == 1 ? w[c / 4].y : c % 4 == 2 ? w[c / 4].z : w[c / 4].w;
+                    *reinterpret_cast<uint4*>(d + (c >> 3) * C::PANEL + swizzled(row, c & 7)) =
+                        values_of(word, __half2half2(s[c * 8 / GROUP]), __half2half2(z[c * 8 / GROUP]));
+                }
+            };
+            uint32_t kind, page = page_of(t0);
+            uint32_t r = row_of(t0, page, kind);
+            page = page_of(t0 + 1);
+            read(kind, r, a.k, kw, ks, kz);
+            read(kind, r, a.v, vw, vs, vz);
+            for (uint32_t tile = t0; tile < tn; ++tile, ++done) {
+                const uint32_t st = done % STAGES, use = done / STAGES;
+                if (kind == 2) {
+#pragma unroll
+                    for (int i = 0; i < G; ++i) kz[i] = __ushort_as_half(0x7FFF);
+                }
+                if (use) wait(&k_empty[st], (use - 1) & 1, err);
+                put(smem + C::K + st * C::TILE, kw, ks, kz);
+                filled(&k_full[st]);
+                r = row_of(tile + 1, page, kind);
+                read(kind, r, a.k, kw, ks, kz);
+                page = page_of(tile + 2);
+                if (use) wait(&v_empty[st], (use - 1) & 1, err);
+                put(smem + C::V + st * C::TILE, vw, vs, vz);
+                filled(&v_full[st]);
+                read(kind, r, a.v, vw, vs, vz);
+            }
+            // ---- own entries: W lanes copy a row, a warp RPW rows at a time ---------------
+            // (A thread per row left each load of a warp in 32 lines: 18,000 cycles a tile.)
+            constexpr int RPW = 32 / W, STEPS = KT / (4 * RPW);
+            const uint32_t c = lane % W, r0 = (warp & 3) * RPW + lane / W;
+            for (uint32_t tile = max(t0, p.s.past); tile < p.hi - p.u0; ++tile, ++done) {
+                const uint32_t st = done % STAGES, use = done / STAGES, key0 = (tile - p.s.past) * KT;
+                const auto copy_rows = [&](const void* base, uint64_t token, uint64_t head, unsigned char* tile_at) {
+                    const __half* src = static_cast<const __half*>(base) + (p.s.rq.token0 + key0 + r0) * token + p.hk * head + 8 * c;
+                    const uint32_t d = mma4::s_addr(tile_at) + (c >> 3) * C::PANEL;
+#pragma unroll 4
+                    for (int i = 0; i < STEPS; ++i) {
+                        const uint32_t rr = r0 + 4 * RPW * i;
+                        const bool live = key0 + rr < p.s.rq.n;
+                        const __half* from = live ? src + (uint64_t)(4 * RPW * i) * token : static_cast<const __half*>(base);
+                        if (vec) {
+                            copy16(d + swizzled(rr, c & 7), from, live);
+                        } else {
+                            __half h[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) h[e] = live ? from[e] : __ushort_as_half(0);
+                            *reinterpret_cast<uint4*>(tile_at + (c >> 3) * C::PANEL + swizzled(rr, c & 7)) = *reinterpret_cast<const uint4*>(h);
+                        }
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                };
                 unsigned char* kd = smem + C::K + st * C::TILE;
                 unsigned char* vd = smem + C::V + st * C::TILE;
-                if (tile < p.s.past) {
-                    const uint32_t pos = tile * KT + row;
-                    const bool live = pos < p.s.rq.ctx;
-                    bool bad = false;
-                    uint4 kw[W / 4], vw[W / 4];
-                    __half sc[4][G];
-                    if (live) {
-                        uint32_t page = (uint32_t)a.block_tables[(size_t)p.b * a.width + (pos >> a.page_shift)];
-                        bad = page >= a.pages;
-                        if (bad) page = 0;
-                        const uint64_t r = (((uint64_t)page * a.n_kv_heads + p.hk) << a.page_shift) + (pos & ((1u << a.page_shift) - 1));
-#pragma unroll
-                        for (int i = 0; i < W / 4; ++i) {
-                            kw[i] = reinterpret_cast<const uint4*>(a.k.words + r * W)[i];
-                            vw[i] = reinterpret_cast<const uint4*>(a.v.words + r * W)[i];
-                        }
-#pragma unroll
-                        for (int i = 0; i < G; ++i) {
-                            sc[0][i] = static_cast<const __half*>(a.k.scales)[r * G + i];
-                            sc[1][i] = static_cast<const __half*>(a.k.biases)[r * G + i];
-                            sc[2][i] = static_cast<const __half*>(a.v.scales)[r * G + i];
-                            sc[3][i] = static_cast<const __half*>(a.v.biases)[r * G + i];
-                        }
-                    } else {
-                        // keys past the length: zeros, which the mask (K) and the zero
-                        // weights (V) leave without effect
-#pragma unroll
-                        for (int i = 0; i < W / 4; ++i) kw[i] = vw[i] = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                        for (int i = 0; i < G; ++i)
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) sc[x][i] = __ushort_as_half(0);
-                    }
-                    if (bad) {
-#pragma unroll
-                        for (int i = 0; i < G; ++i) sc[1][i] = __ushort_as_half(0x7FFF);
-                    }
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        if (use) wait(half ? &v_empty[st] : &k_empty[st], (use - 1) & 1, err);
-                        unsigned char* d = half ? vd : kd;
-                        const uint4* w = half ? vw : kw;
-#pragma unroll
-                        for (int c = 0; c < W; ++c) {
-                            const uint32_t word = c % 4 == 0 ? w[c / 4].x : c % 4 == 1 ? w[c / 4].y : c % 4 == 2 ? w[c / 4].z : w[c / 4].w;
-                            *reinterpret_cast<uint4*>(d + (c >> 3) * C::PANEL + swizzled(row, c & 7)) =
-                                values_of(word, __half2half2(sc[2 * half][c * 8 / GROUP]), __half2half2(sc[2 * half + 1][c * 8 / GROUP]));
-                        }
-                        fence_async_smem();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(half ? &v_full[st] : &k_full[st]);
-                    }
-                } else {
-                    const uint32_t own = (tile - p.s.past) * KT + row;
-                    const bool live = own < p.s.rq.n;
-                    const auto read_row = [&](const void* base, uint64_t token, uint64_t head, uint4 (&x)[W]) {
-                        const __half* src = static_cast<const __half*>(base) + (p.s.rq.token0 + own) * token + p.hk * head;
-#pragma unroll
-                        for (int c = 0; c < W; ++c) {
-                            x[c] = make_uint4(0u, 0u, 0u, 0u);
-                            if (live) {
-                                if (vec) {
-                                    x[c] = reinterpret_cast<const uint4*>(src)[c];
-                                } else {
-                                    __half h[8];
-#pragma unroll
-                                    for (int i = 0; i < 8; ++i) h[i] = src[8 * c + i];
-                                    x[c] = *reinterpret_cast<const uint4*>(h);
-                                }
-                            }
-                        }
-                    };
-                    // A weight of zero does not keep an infinite or NaN value out of the
-                    // rows that are masked from it: such a value row is taken as zeros, and
-                    // its key as NaN, which reaches the rows that see it and no other.
-                    bool wild = false;
-                    {
-                        uint4 x[W];
-                        read_row(a.new_v, a.v_token, a.v_head, x);
-                        __half2 top = __half2half2(__ushort_as_half(0));
-#pragma unroll
-                        for (int c = 0; c < W; ++c) {
-                            const __half2* h = reinterpret_cast<const __half2*>(&x[c]);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) top = __hmax2_nan(top, __habs2(h[i]));
-                        }
-                        wild = !(__low2float(top) <= 65504.0f && __high2float(top) <= 65504.0f);
-                    }
-#pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
-                        uint4 x[W];
-                        if (half) read_row(a.new_v, a.v_token, a.v_head, x);
-                        else read_row(a.new_k, a.k_token, a.k_head, x);
-                        if (wild) {
-#pragma unroll
-                            for (int c = 0; c < W; ++c) x[c].x = x[c].y = x[c].z = x[c].w = half ? 0u : 0x7FFF7FFFu;
-                        }
-                        if (use) wait(half ? &v_empty[st] : &k_empty[st], (use - 1) & 1, err);
-                        unsigned char* d = half ? vd : kd;
-#pragma unroll
-                        for (int c = 0; c < W; ++c)
-                            *reinterpret_cast<uint4*>(d + (c >> 3) * C::PANEL + swizzled(row, c & 7)) = reorder(x[c]);
-                        fence_async_smem();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(half ? &v_full[st] : &k_full[st]);
+                if (use) wait(&k_empty[st], (use - 1) & 1, err);
+                copy_rows(a.new_k, a.k_token, a.k_head, kd);
+                if (key0 + KT - 1 <= p.tok0) {                 // every row sees every key
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    filled(&k_full[st]);
+                    if (use) wait(&v_empty[st], (use - 1) & 1, err);
+                    copy_rows(a.new_v, a.v_token, a.v_head, vd);
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    filled(&v_full[st]);
+                    continue;
+                }
+                // A weight of zero does not keep an infinite or NaN value out of the rows that
+                // are masked from it. Such a value row is taken as zeros, and its key as NaN,
+                // which reaches the rows that see it and no other.
+                if (use) wait(&v_empty[st], (use - 1) & 1, err);
+                copy_rows(a.new_v, a.v_token, a.v_head, vd);
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                __syncwarp();
+#pragma unroll 4
+                for (int i = 0; i < STEPS; ++i) {
+                    const uint32_t off = (c >> 3) * C::PANEL + swizzled(r0 + 4 * RPW * i, c & 7);
+                    const uint4 x = *reinterpret_cast<const uint4*>(vd + off);
+                    const __half2* h = reinterpret_cast<const __half2*>(&x);
+                    const __half2 top = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+                    const bool here = !(__low2float(top) <= 65504.0f && __high2float(top) <= 65504.0f);
+                    const uint32_t who = __ballot_sync(0xffffffffu, here) >> (lane / W * W);
+                    if (who & (uint32_t)((1ull << W) - 1)) {
+                        *reinterpret_cast<uint4*>(vd + off) = make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4*>(kd + off) = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
                     }
                 }
+                filled(&k_full[st]);
+                filled(&v_full[st]);
             }
         }
     } else {
