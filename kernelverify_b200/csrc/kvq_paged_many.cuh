@@ -5,13 +5,13 @@
 // 128 rows, a row being one (token, query head), the R heads of a token side
 // by side, so the R heads share every key they read. Keys come in tiles of
 // 128: the cached positions first, dequantized to fp16, then the step's own
-// entries under the causal mask. Both products are tcgen05.mma kind::f16 of
-// 128 x 128 x DH:
+// entries under the causal mask. They are worked off in steps of 64 keys, and both
+// products are tcgen05.mma kind::f16:
 //
 //   S_i = Q_i K^T   (both operands in shared memory, fp32 S in tensor memory)
-//   O_i += P_i V    (P_i fp16 in tensor memory over S_i's columns)
+//   O_i += P_i V    (P_i fp16 in tensor memory over its S_i's columns)
 //
-// Sixteen warps in four warpgroups, registers re-split with setmaxnreg:
+// Sixteen warps in four warpgroups:
 //   0, 1  softmax of M tile 0 and 1, a thread per row: S from tensor memory,
 //         an online softmax whose reference moves (and rescales O) only when
 //         the row's maximum passed it by 2^14, P back to tensor memory; at the
@@ -19,10 +19,13 @@
 //   2     loads: cached rows a thread per key, the next tile's words on their way
 //         while this one's become fp16; own entries by 16-byte asynchronous
 //         copies; all stored with the 128-byte swizzle the MMAs read
-//   3     one thread issues the MMAs
-// While one M tile is in its softmax the tensor cores work for the other. K
-// and V tiles have the same layout, rows of keys: K is read as a K-major
-// operand, V as an MN-major one.
+//   3     a warp per M tile whose elected lane issues its MMAs (one warp for both
+//         spent 2,400 cycles on a step of 64 keys, waiting and issuing in turn)
+// Each M tile has two S buffers, so that the scores of a step are there before
+// the softmax is done with the one in front. (With one buffer of 128 keys the
+// softmax of an M tile waited for its own PV and S: 4,850 cycles per 128 keys,
+// 2,830 of them softmax.) K and V tiles have the same layout, rows of keys: K is
+// read as a K-major operand, V as an MN-major one.
 //
 // Rounded to fp16: the dequantized K and V (as a cache held in fp16 would be)
 // and the weights P; everything else is fp32. P is at most 2^14 and its sum is
@@ -56,15 +59,13 @@ using umma::umma;
 using umma::umma_commit;
 
 constexpr int THREADS = 512;
-constexpr int KT = 128;                    // keys per tile
+constexpr int KT = 128;                    // keys per tile in shared memory
+constexpr int KS = 64;                     // keys per step
 constexpr int ROWS = 128;                  // query rows per M tile
 constexpr int COLS = 2 * ROWS;             // query rows per unit
 constexpr int STAGES = 2;                  // K and V tiles in shared memory, each
 constexpr float RAISE = 14.0f, START = 4.0f;   // log2 room above the reference
-// registers per thread at launch and after the re-split; the sum over the four
-// warpgroups must stay the launch's (a larger one would wait forever)
-constexpr int REG_LAUNCH = 128, REG_SOFTMAX = 176, REG_LOAD = 112, REG_MMA = 48;
-static_assert(2 * REG_SOFTMAX + REG_LOAD + REG_MMA <= 4 * REG_LAUNCH, "register re-split over the launch budget");
+constexpr uint32_t SUSPEND_NS = 20000;
 constexpr long long WAIT_CYCLES = 2000000000ll;      // about a second
 
 template <int DH>
@@ -76,12 +77,12 @@ struct Cfg {
     static constexpr int K = 2 * TILE;
     static constexpr int V = K + STAGES * TILE;
     static constexpr int BAR = V + STAGES * TILE;
-    // q_full[2], s_full[2], p_full[2], o_full[2], then k_full, k_empty, v_full,
-    // v_empty [STAGES] each, and the MMA thread's last one
-    static constexpr int NBAR = 8 + 4 * STAGES + 2;
+    // q_full[2], pv_done[2], s_full[2][2], p_full[2][2] (M tile, buffer), then k_full,
+    // k_empty, v_full, v_empty [STAGES] each, and the MMA warp's last one
+    static constexpr int NBAR = 12 + 4 * STAGES + 2;
     static constexpr int MISC = BAR + NBAR * 8;        // TMEM address, error flag
     static constexpr int BEFORE = MISC + 16;           // uint32 [rows + 1]
-    static constexpr uint32_t S0 = 0, O0 = 256;        // TMEM columns: S_i at 128 i, O_i at 256 + 128 i
+    static constexpr uint32_t S0 = 0, O0 = 256;        // TMEM columns: S_i's buffer b at 128 i + 64 b, O_i at 256 + 128 i
     static_assert(PANEL % 1024 == 0, "swizzle atoms are 1024-byte aligned");
 };
 
@@ -122,11 +123,6 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
     return p != 0;
 }
-template <int N>
-__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-
 // Descriptor of an operand with the 128-byte swizzle: rows of 128 bytes, eight
 // to a 1024-byte atom. K-major (Q, K): the rows are M or N, atoms along them
 // 1024 bytes apart. MN-major (V): the rows are K, atoms along them 1024 bytes
@@ -138,14 +134,30 @@ __device__ __forceinline__ uint64_t desc128(uint32_t saddr, uint32_t leading) {
 // byte offset of 16-byte chunk c (eight dims) of row r in a panel
 __device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
+// A test of a phase that may suspend the thread until it completes: a warp that
+// polls takes issue slots from the others.
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(SUSPEND_NS)
+        : "memory");
+    return ok != 0;
+}
 // Every wait ends: after WAIT_CYCLES, or once another wait gave up.
-__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* err) {
-    if (mbar_try_wait(bar, parity)) return;
+__device__ __forceinline__ void wait_long(uint32_t bar, uint32_t parity, volatile int* err) {
     const long long t0 = clock64();
-    do {
-        if (mbar_try_wait(bar, parity) || *err) return;
-    } while (clock64() - t0 < WAIT_CYCLES);
+    while (clock64() - t0 < WAIT_CYCLES) {
+        if (try_wait(bar, parity) || *err) return;
+    }
     *err = 1;
+}
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* err) {
+    const uint32_t at = mma4::s_addr(bar);
+    if (!try_wait(at, parity)) wait_long(at, parity, err);
 }
 
 // a word's eight codes -> fp16 scale * code + bias, rounded once. A byte in both
@@ -246,8 +258,8 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (mma4::s_addr(smem_raw) & 1023u)) & 1023u);
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::BAR);
-    uint64_t *q_full = bar, *s_full = bar + 2, *p_full = bar + 4, *o_full = bar + 6;
-    uint64_t *k_full = bar + 8, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES;
+    uint64_t *q_full = bar, *pv_done = bar + 2, *s_full = bar + 4, *p_full = bar + 8;
+    uint64_t *k_full = bar + 12, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES;
     uint64_t* drained = v_empty + STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::MISC);
     volatile int* err = reinterpret_cast<volatile int*>(smem + C::MISC + 4);
@@ -257,17 +269,20 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 4);
+            mbar_init(&pv_done[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
-            mbar_init(&o_full[i], 1);
         }
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(&k_full[i], 4);
-            mbar_init(&k_empty[i], 1);
+            mbar_init(&k_empty[i], 2);
             mbar_init(&v_full[i], 4);
-            mbar_init(&v_empty[i], 1);
+            mbar_init(&v_empty[i], 2);
         }
-        mbar_init(drained, 1);
+        mbar_init(&drained[0], 1);
+        mbar_init(&drained[1], 1);
         *err = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         reinterpret_cast<Split*>(ws)[blockIdx.x].parts = 0;
@@ -292,14 +307,13 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
 
     if (wg < 2) {
         // ---------------------------- softmax ------------------------------------
-        regs_inc<REG_SOFTMAX>();
         const int mt = wg, row = tid & 127;
         const uint32_t tokm = ROWS / a.r;
         const uint32_t rt = row / a.r, rh = row - rt * a.r;          // the row's token of the M tile, head
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // TMEM lane 32 (warp % 4), bits 16 up
         const uint32_t s_at = tmem + lanes + C::S0 + 128 * mt, o_at = tmem + lanes + C::O0 + 128 * mt;
         const float scale2 = a.scale * 1.4426950408889634f;
-        uint32_t tiles_done = 0, parts_done = 0;
+        uint32_t done = 0;                                           // steps
         for (uint32_t at = start; at < end;) {
             const Part p = part_at(a, before, least_new, at, end);
             at = p.hi;
@@ -331,27 +345,28 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                 if (lane == 0) mbar_arrive(&q_full[mt]);
             }
             float ref = -INFINITY, l = 0.0f;
-            for (uint32_t j = p.lo; j < p.hi; ++j, ++tiles_done) {
-                wait(&s_full[mt], tiles_done & 1, err);
+            const uint32_t steps = (p.hi - p.lo) * (KT / KS);
+            for (uint32_t q = 0; q < steps; ++q, ++done) {
+                const uint32_t buf = done & 1, s_buf = s_at + KS * buf;
+                wait(&s_full[2 * mt + buf], (done >> 1) & 1, err);
                 __syncwarp();
                 tc_fence_after();
-                uint32_t s[KT];
-#pragma unroll
-                for (int c = 0; c < KT; c += 32) ld32(s_at + c, s + c);
+                uint32_t s[KS];
+                ld32(s_buf, s);
+                ld32(s_buf + 32, s + 32);
                 tmem_wait_ld();
-                // visible keys of the tile: the cached ones up to the length, of the
-                // step's own those up to the row's token
-                const uint32_t tile = j - p.u0;
-                const int lim = tile < p.s.past ? (int)min((uint32_t)KT, p.s.rq.ctx - tile * KT)
-                                                : (int)tok - (int)((tile - p.s.past) * KT) + 1;
-                if (__any_sync(0xffffffffu, lim < KT)) {
+                // visible keys of the step: the cached ones up to the length, of the step's
+                // own those up to the row's token
+                const uint32_t tile = p.lo - p.u0 + q / 2, key = (tile < p.s.past ? tile : tile - p.s.past) * KT + (q & 1) * KS;
+                const int lim = tile < p.s.past ? (int)p.s.rq.ctx - (int)key : (int)tok - (int)key + 1;
+                if (__any_sync(0xffffffffu, lim < KS)) {
 #pragma unroll
-                    for (int c = 0; c < KT; ++c)
+                    for (int c = 0; c < KS; ++c)
                         if (c >= lim) s[c] = 0xff800000u;
                 }
                 float top = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < KT; c += 2) top = fmaxf(top, fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])));
+                for (int c = 0; c < KS; c += 2) top = fmaxf(top, fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])));
                 top *= scale2;
                 const bool over = top - ref > RAISE;
                 if (__any_sync(0xffffffffu, over)) {
@@ -360,7 +375,10 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                     const float f = ref == -INFINITY ? 0.0f : ex2(ref - to);
                     ref = to;
                     l *= f;
-                    if (j > p.lo) {
+                    if (q > 0) {
+                        wait(&pv_done[mt], (done - 1) & 1, err);
+                        __syncwarp();
+                        tc_fence_after();
 #pragma unroll
                         for (int c = 0; c < DH; c += 16) {
                             uint32_t o[16];
@@ -373,25 +391,29 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                     }
                 }
                 const float sub = ref == -INFINITY ? 0.0f : ref;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const float2 mul2 = make_float2(scale2, scale2), sub2 = make_float2(-sub, -sub);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-                for (int c = 0; c < KT; c += 2) {
-                    const float x = ex2(fmaf(__uint_as_float(s[c]), scale2, -sub));
-                    const float y = ex2(fmaf(__uint_as_float(s[c + 1]), scale2, -sub));
-                    sum[(c >> 1) & 3] += x + y;
-                    const __half2 h = __floats2half2_rn(x, y);
+                for (int c = 0; c < KS; c += 2) {
+                    float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), mul2, sub2);
+                    x.x = ex2(x.x);
+                    x.y = ex2(x.y);
+                    sum[(c >> 1) & 1] = __fadd2_rn(sum[(c >> 1) & 1], x);
+                    const __half2 h = __floats2half2_rn(x.x, x.y);
                     s[c >> 1] = *reinterpret_cast<const uint32_t*>(&h);
-                    if (c % 64 == 62) st32(s_at + c / 2 - 31, s + c / 2 - 31);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                st32(s_buf, s);
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
                 tc_fence_before();
+                // every step's combine is waited for before the next one is let go (it has long
+                // been done by then): a parity tells only neighbouring phases apart
+                if (q > 0) wait(&pv_done[mt], (done - 1) & 1, err);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[mt]);
+                if (lane == 0) mbar_arrive(&p_full[2 * mt + buf]);
             }
             // ---- the part's result ------------------------------------------------
-            wait(&o_full[mt], parts_done & 1, err);
-            ++parts_done;
+            wait(&pv_done[mt], (done - 1) & 1, err);
             __syncwarp();
             tc_fence_after();
             const bool whole = p.u0 >= start && p.u1 <= end;
@@ -436,7 +458,6 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
         }
     } else if (wg == 2) {
         // ------------------------------ loads -------------------------------------
-        regs_dec<REG_LOAD>();
         const uint32_t row = tid & 127;
         const auto filled = [&](uint64_t* bar) {
             fence_async_smem();
@@ -568,62 +589,76 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
         }
     } else {
         // --------------------------- the MMAs -----------------------------------------
-        regs_dec<REG_MMA>();
-        if (warp == 12) {
-            // The whole warp walks the tiles and one elected lane issues, so that
-            // the operands' descriptors stay in uniform registers: under a
-            // condition on the lane number each MMA took 190 cycles to issue
-            // against the 64 it runs.
-            constexpr uint32_t ID_S = idesc(false, false, false, KT, ROWS);
+        if (warp < 14) {
+            // The whole warp walks the steps and one elected lane issues, so that the
+            // operands' descriptors stay in uniform registers: under a condition on the
+            // lane number each MMA took 190 cycles to issue against the 64 it runs.
+            constexpr uint32_t ID_S = idesc(false, false, false, KS, ROWS);
             constexpr uint32_t ID_O = idesc(false, false, true, DH, ROWS);
-            const uint32_t base = mma4::s_addr(smem);
-            uint32_t done = 0, parts[2] = {0, 0}, tiles[2] = {0, 0};
+            const int mt = warp - 12;
+            const uint32_t base = mma4::s_addr(smem), q_at = base + C::Q + mt * C::TILE;
+            const uint32_t s_at = tmem + C::S0 + 128 * mt, o_at = tmem + C::O0 + 128 * mt;
+            uint32_t tiles = 0, parts = 0, steps = 0;              // done in front of this part
             for (uint32_t at = start; at < end;) {
                 const Part p = part_at(a, before, least_new, at, end);
                 at = p.hi;
-                const int n = p.second ? 2 : 1;
-                for (int i = 0; i < n; ++i) wait(&q_full[i], parts[i] & 1, err);
-                for (uint32_t j = p.lo; j <= p.hi; ++j) {
-                    const uint32_t st = done % STAGES, pst = (done - 1) % STAGES;
-                    if (j < p.hi) wait(&k_full[st], (done / STAGES) & 1, err);
-                    if (j > p.lo) wait(&v_full[pst], ((done - 1) / STAGES) & 1, err);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        if (i == n) break;
-                        if (j > p.lo) wait(&p_full[i], (tiles[i] - 1) & 1, err);
+                const uint32_t n = (p.hi - p.lo) * (KT / KS), tile0 = tiles;
+                tiles += p.hi - p.lo;
+                if (mt == 1 && !p.second) {
+                    // nothing to do in this part but to follow its tiles: a parity tells only
+                    // neighbouring phases apart, and a tile is free once both warps say so
+                    for (uint32_t kt = tile0; kt < tiles; ++kt) {
+                        wait(&k_full[kt % STAGES], (kt / STAGES) & 1, err);
                         __syncwarp();
-                        tc_fence_after();
-                        if (elect_one()) {
-                            if (j > p.lo) {
-                                const uint64_t v = desc128(base + C::V + pst * C::TILE, C::PANEL);
-#pragma unroll
-                                for (int k = 0; k < KT / 16; ++k)
-                                    umma_ts(tmem + C::O0 + 128 * i, tmem + C::S0 + 128 * i + 8 * k, v + k * (2048 >> 4), ID_O,
-                                            j - 1 > p.lo || k > 0);
-                                if (j == p.hi) umma_commit(&o_full[i]);
-                                if (i == n - 1) umma_commit(&v_empty[pst]);
-                            }
-                            if (j < p.hi) {
-                                const uint64_t q = desc128(base + C::Q + i * C::TILE, 16), kd = desc128(base + C::K + st * C::TILE, 16);
-#pragma unroll
-                                for (int k = 0; k < DH / 16; ++k) {
-                                    const uint32_t off = ((k >> 2) * C::PANEL + (k & 3) * 32) >> 4;
-                                    umma(tmem + C::S0 + 128 * i, q + off, kd + off, ID_S, k > 0);
-                                }
-                                umma_commit(&s_full[i]);
-                                if (i == n - 1) umma_commit(&k_empty[st]);
-                            }
-                        }
+                        if (lane == 0) mbar_arrive(&k_empty[kt % STAGES]);
+                        wait(&v_full[kt % STAGES], (kt / STAGES) & 1, err);
                         __syncwarp();
-                        if (j < p.hi) ++tiles[i];
+                        if (lane == 0) mbar_arrive(&v_empty[kt % STAGES]);
                     }
-                    if (j < p.hi) ++done;
+                    continue;
                 }
-                for (int i = 0; i < n; ++i) ++parts[i];
+                wait(&q_full[mt], parts & 1, err);
+                ++parts;
+                // scores of step q, two steps ahead of the combine of step q - 2 whose buffer
+                // they take
+                for (uint32_t q = 0; q < n + 2; ++q) {
+                    const uint32_t kt = tile0 + q / 2, vt = kt - 1, half = q & 1, g = steps + q, buf = g & 1;
+                    const uint32_t s_buf = s_at + KS * buf;
+                    if (q < n && half == 0) wait(&k_full[kt % STAGES], (kt / STAGES) & 1, err);
+                    if (q >= 2) {
+                        if (half == 0) wait(&v_full[vt % STAGES], (vt / STAGES) & 1, err);
+                        wait(&p_full[2 * mt + buf], ((g - 2) >> 1) & 1, err);
+                    }
+                    __syncwarp();
+                    tc_fence_after();
+                    if (elect_one()) {
+                        if (q >= 2) {
+                            const uint64_t v = desc128(base + C::V + (vt % STAGES) * C::TILE + half * (KS * 128), C::PANEL);
+#pragma unroll
+                            for (int k = 0; k < KS / 16; ++k) umma_ts(o_at, s_buf + 8 * k, v + k * (2048 >> 4), ID_O, q > 2 || k > 0);
+                            // in front of the scores' commit: whoever sees step q's scores knows
+                            // that all combines up to step q - 2 are done and counted
+                            umma_commit(&pv_done[mt]);
+                            if (half) umma_commit(&v_empty[vt % STAGES]);
+                        }
+                        if (q < n) {
+                            const uint64_t qd = desc128(q_at, 16), kd = desc128(base + C::K + (kt % STAGES) * C::TILE + half * (KS * 128), 16);
+#pragma unroll
+                            for (int k = 0; k < DH / 16; ++k) {
+                                const uint32_t off = ((k >> 2) * C::PANEL + (k & 3) * 32) >> 4;
+                                umma(s_buf, qd + off, kd + off, ID_S, k > 0);
+                            }
+                            umma_commit(&s_full[2 * mt + buf]);
+                            if (half) umma_commit(&k_empty[kt % STAGES]);
+                        }
+                    }
+                    __syncwarp();
+                }
+                steps += n;
             }
             // nothing of this CTA's is in flight when its tensor memory goes
-            if (elect_one()) umma_commit(drained);
-            for (const long long t0 = clock64(); !mbar_try_wait(drained, 0) && clock64() - t0 < WAIT_CYCLES;) {}
+            if (elect_one()) umma_commit(&drained[mt]);
+            for (const long long t0 = clock64(); !mbar_try_wait(&drained[mt], 0) && clock64() - t0 < WAIT_CYCLES;) {}
         }
     }
     tc_fence_before();
@@ -640,12 +675,6 @@ cudaError_t launch_many(const Attend& a, uint32_t least_new, bool vec, uint32_t 
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(kernel, 1024 + C::BEFORE + (MAX_ROWS + 1) * 4, done);
     if (e != cudaSuccess) return e;
-    // the register re-split assumes the launch's count (host-side constant of the build)
-    static const int regs = [&] {
-        cudaFuncAttributes f{};
-        return cudaFuncGetAttributes(&f, kernel) == cudaSuccess ? f.numRegs : 0;
-    }();
-    if (regs != REG_LAUNCH) return cudaErrorInvalidConfiguration;
     const size_t smem = 1024 + C::BEFORE + ((size_t)a.rows + 1) * 4;
     kernel<<<grid, THREADS, smem, stream>>>(a, least_new, vec, static_cast<unsigned char*>(ws));
     e = cudaGetLastError();
