@@ -77,9 +77,9 @@ struct Cfg {
     static constexpr int K = 2 * TILE;
     static constexpr int V = K + STAGES * TILE;
     static constexpr int BAR = V + STAGES * TILE;
-    // q_full[2], pv_done[2], s_full[2][2], p_full[2][2] (M tile, buffer), then k_full,
-    // k_empty, v_full, v_empty [STAGES] each, and the MMA warp's last one
-    static constexpr int NBAR = 12 + 4 * STAGES + 2;
+    // q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2] (M tile, buffer), then k_full,
+    // k_empty, v_full, v_empty [STAGES] each, and the MMA warps' last ones
+    static constexpr int NBAR = 14 + 4 * STAGES + 2;
     static constexpr int MISC = BAR + NBAR * 8;        // TMEM address, error flag
     static constexpr int BEFORE = MISC + 16;           // uint32 [rows + 1]
     static constexpr uint32_t S0 = 0, O0 = 256;        // TMEM columns: S_i's buffer b at 128 i + 64 b, O_i at 256 + 128 i
@@ -123,6 +123,31 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
     return p != 0;
 }
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^x of two values on the FMA pipe: x = n + r with |r| <= 1/2 by adding and
+// taking away 1.5 * 2^23, a polynomial for 2^r (fitted to it in relative error:
+// 5.5e-6 at most), n added to the exponent. Below -126 as at -126, which is 0 in
+// fp16; not for NaN. The special-function unit gives 16 exponentials a cycle to
+// an SM and is what the softmax waits for: POLY of eight pairs are taken off it.
+constexpr int POLY = 3;
+constexpr float P0 = 0.99999803f, P1 = 0.69313157f, P2 = 0.24027981f, P3 = 0.055894606f, P4 = 0.0094680814f;
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    const auto both = [](float v) { return make_float2(v, v); };
+    x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+    const float2 t = __fadd2_rn(x, both(12582912.0f));
+    const float2 r = __fadd2_rn(x, __ffma2_rn(t, both(-1.0f), both(12582912.0f)));
+    float2 p = __ffma2_rn(r, both(P4), both(P3));
+    p = __ffma2_rn(p, r, both(P2));
+    p = __ffma2_rn(p, r, both(P1));
+    p = __ffma2_rn(p, r, both(P0));
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
 // Descriptor of an operand with the 128-byte swizzle: rows of 128 bytes, eight
 // to a 1024-byte atom. K-major (Q, K): the rows are M or N, atoms along them
 // 1024 bytes apart. MN-major (V): the rows are K, atoms along them 1024 bytes
@@ -258,8 +283,8 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (mma4::s_addr(smem_raw) & 1023u)) & 1023u);
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::BAR);
-    uint64_t *q_full = bar, *pv_done = bar + 2, *s_full = bar + 4, *p_full = bar + 8;
-    uint64_t *k_full = bar + 12, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES;
+    uint64_t *q_full = bar, *s_full = bar + 2, *p_full = bar + 6, *pv_done = bar + 10;
+    uint64_t *k_full = bar + 14, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES;
     uint64_t* drained = v_empty + STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::MISC);
     volatile int* err = reinterpret_cast<volatile int*>(smem + C::MISC + 4);
@@ -269,9 +294,9 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 4);
-            mbar_init(&pv_done[i], 1);
         }
         for (int i = 0; i < 4; ++i) {
+            mbar_init(&pv_done[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
         }
@@ -314,6 +339,10 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
         const uint32_t s_at = tmem + lanes + C::S0 + 128 * mt, o_at = tmem + lanes + C::O0 + 128 * mt;
         const float scale2 = a.scale * 1.4426950408889634f;
         uint32_t done = 0;                                           // steps
+        // step g's combine is done. Asked of the last step in front of one whose scores
+        // were seen, or of that one: those of two steps before are done then, so that
+        // the barrier of g's buffer is at g's phase or just behind it.
+        const auto combined = [&](uint32_t g) { wait(&pv_done[2 * mt + (g & 1)], (g >> 1) & 1, err); };
         for (uint32_t at = start; at < end;) {
             const Part p = part_at(a, before, least_new, at, end);
             at = p.hi;
@@ -364,10 +393,12 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                     for (int c = 0; c < KS; ++c)
                         if (c >= lim) s[c] = 0xff800000u;
                 }
-                float top = -INFINITY;
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < KS; c += 2) top = fmaxf(top, fmaxf(__uint_as_float(s[c]), __uint_as_float(s[c + 1])));
-                top *= scale2;
+                for (int c = 0; c < KS; c += 2)
+                    tops[c / 2 % 4] = max_nan(tops[c / 2 % 4], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+                const float top = max_nan(max_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]) * scale2;
+                if (top != top) l = NAN;               // a NaN among the scores it sees: so is the row
                 const bool over = top - ref > RAISE;
                 if (__any_sync(0xffffffffu, over)) {
                     const float to = over ? top - START : ref;
@@ -376,7 +407,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                     ref = to;
                     l *= f;
                     if (q > 0) {
-                        wait(&pv_done[mt], (done - 1) & 1, err);
+                        combined(done - 1);
                         __syncwarp();
                         tc_fence_after();
 #pragma unroll
@@ -396,8 +427,12 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
 #pragma unroll
                 for (int c = 0; c < KS; c += 2) {
                     float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), mul2, sub2);
-                    x.x = ex2(x.x);
-                    x.y = ex2(x.y);
+                    if (c / 2 % 8 < POLY) {
+                        x = exp2_poly(x);
+                    } else {
+                        x.x = ex2(x.x);
+                        x.y = ex2(x.y);
+                    }
                     sum[(c >> 1) & 1] = __fadd2_rn(sum[(c >> 1) & 1], x);
                     const __half2 h = __floats2half2_rn(x.x, x.y);
                     s[c >> 1] = *reinterpret_cast<const uint32_t*>(&h);
@@ -406,14 +441,11 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
                 tc_fence_before();
-                // every step's combine is waited for before the next one is let go (it has long
-                // been done by then): a parity tells only neighbouring phases apart
-                if (q > 0) wait(&pv_done[mt], (done - 1) & 1, err);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[2 * mt + buf]);
             }
             // ---- the part's result ------------------------------------------------
-            wait(&pv_done[mt], (done - 1) & 1, err);
+            combined(done - 1);
             __syncwarp();
             tc_fence_after();
             const bool whole = p.u0 >= start && p.u1 <= end;
@@ -638,7 +670,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                             for (int k = 0; k < KS / 16; ++k) umma_ts(o_at, s_buf + 8 * k, v + k * (2048 >> 4), ID_O, q > 2 || k > 0);
                             // in front of the scores' commit: whoever sees step q's scores knows
                             // that all combines up to step q - 2 are done and counted
-                            umma_commit(&pv_done[mt]);
+                            umma_commit(&pv_done[2 * mt + buf]);
                             if (half) umma_commit(&v_empty[vt % STAGES]);
                         }
                         if (q < n) {
