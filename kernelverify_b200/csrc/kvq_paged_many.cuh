@@ -205,18 +205,19 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
-// sum_{i=0}^{n-1} floor((a i + b) / 128)
-__device__ __forceinline__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+// sum_{i=0}^{n-1} floor((a i + b) / m), by steps of Euclid's algorithm
+__device__ __forceinline__ uint64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
     uint64_t s = 0;
     while (n > 0) {
-        s += n * (n - 1) / 2 * (a / m) + n * (b / m);
-        a %= m;
-        b %= m;
-        const uint64_t y = a * n + b;
+        const uint32_t qa = a / m, qb = b / m;
+        s += (uint64_t)n * (n - 1) / 2 * qa + (uint64_t)n * qb;
+        a -= qa * m;
+        b -= qb * m;
+        const uint64_t y = (uint64_t)a * n + b;
         if (y < m) break;
-        n = y / m;
-        b = y % m;
-        const uint64_t t = a;
+        n = (uint32_t)y / m;                // y < 2^31: a < m <= 128, and at most 2^23 units
+        b = (uint32_t)y - n * m;
+        const uint32_t t = a;
         a = m;
         m = t;
     }
@@ -228,10 +229,12 @@ __device__ __forceinline__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a
 struct Shape {
     Request rq;
     uint32_t tu, units, past;          // tokens per unit, units per cache head, cached tiles
+    __device__ __forceinline__ uint32_t tiles(uint32_t i) const { return past + (min((i + 1) * tu, rq.n) + KT - 1) / KT; }
     // key tiles of the units in front of unit i
     __device__ __forceinline__ uint32_t in_front(uint32_t i) const {
-        if (i < units) return i * past + (uint32_t)floor_sum(i, KT, tu, tu + KT - 1);
-        return i * past + (uint32_t)floor_sum(i - 1, KT, tu, tu + KT - 1) + (rq.n + KT - 1) / KT;
+        const uint32_t full = i < units ? i : units - 1;
+        const uint32_t s = full * past + (uint32_t)floor_sum(full, KT, tu, tu + KT - 1);
+        return i < units ? s : s + tiles(full);
     }
 };
 __device__ __forceinline__ Shape shape_of(const Attend& a, uint32_t b, uint32_t least_new) {
@@ -249,8 +252,33 @@ struct Part {
     uint32_t b, hk, unit, u0, u1, lo, hi;
     uint32_t tok0, n_tok;              // the unit's tokens
     bool second;                       // its second M tile has any
+    __device__ __forceinline__ void settle(uint32_t end) {
+        u1 = u0 + s.tiles(unit);
+        hi = min(end, u1);
+        tok0 = unit * s.tu;
+        n_tok = min(s.tu, s.rq.n - tok0);
+        second = n_tok > s.tu / 2;
+    }
+    // the part behind this one; false at the end of the share
+    __device__ __forceinline__ bool next(const Attend& a, const uint32_t* before, uint32_t least_new, uint32_t end) {
+        if (hi >= end) return false;
+        lo = u0 = u1;
+        if (++unit == s.units) {
+            unit = 0;
+            if (++hk == a.n_kv_heads) {
+                hk = 0;
+                do ++b;
+                while (before[b + 1] == u0);       // requests without a unit
+                s = shape_of(a, b, least_new);
+            }
+        }
+        settle(end);
+        return true;
+    }
 };
-__device__ __forceinline__ Part part_at(const Attend& a, const uint32_t* before, uint32_t least_new, uint32_t at, uint32_t end) {
+// The part in which the share begins: found once (the arithmetic of the search
+// is worth several tiles), the others follow from it.
+__device__ __forceinline__ Part first_part(const Attend& a, const uint32_t* before, uint32_t least_new, uint32_t at, uint32_t end) {
     Part p;
     p.b = row_of_tile(before, a.rows, at);
     p.s = shape_of(a, p.b, least_new);
@@ -266,12 +294,8 @@ __device__ __forceinline__ Part part_at(const Attend& a, const uint32_t* before,
     }
     p.unit = lo;
     p.u0 = before[p.b] + p.hk * per_head + p.s.in_front(lo);
-    p.u1 = before[p.b] + p.hk * per_head + p.s.in_front(lo + 1);
     p.lo = at;
-    p.hi = min(end, p.u1);
-    p.tok0 = lo * p.s.tu;
-    p.n_tok = min(p.s.tu, p.s.rq.n - p.tok0);
-    p.second = p.n_tok > p.s.tu / 2;
+    p.settle(end);
     return p;
 }
 
@@ -321,6 +345,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
     if (start64 >= total) return;
     const uint32_t start = (uint32_t)start64, end = min(total, start + share);
 
+    Part p = first_part(a, before, least_new, start, end);
     if (warp == 12) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
@@ -343,9 +368,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
         // were seen, or of that one: those of two steps before are done then, so that
         // the barrier of g's buffer is at g's phase or just behind it.
         const auto combined = [&](uint32_t g) { wait(&pv_done[2 * mt + (g & 1)], (g >> 1) & 1, err); };
-        for (uint32_t at = start; at < end;) {
-            const Part p = part_at(a, before, least_new, at, end);
-            at = p.hi;
+        do {
             if (mt == 1 && !p.second) continue;
             const uint32_t tok = p.tok0 + mt * tokm + rt;           // of the request
             const bool live = rt < tokm && tok < p.s.rq.n;
@@ -487,7 +510,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                 reinterpret_cast<Split*>(ws)[blockIdx.x] = {(p.u1 - 1) / share - blockIdx.x + 1, p.s.rq.token0, p.hk,
                                                             p.tok0 * a.r, p.n_tok * a.r};
             tc_fence_before();
-        }
+        } while (p.next(a, before, least_new, end));
     } else if (wg == 2) {
         // ------------------------------ loads -------------------------------------
         const uint32_t row = tid & 127;
@@ -497,9 +520,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
             if (lane == 0) mbar_arrive(bar);
         };
         uint32_t done = 0;
-        for (uint32_t at = start; at < end;) {
-            const Part p = part_at(a, before, least_new, at, end);
-            at = p.hi;
+        do {
             // ---- cached tiles: this thread's key of each -----------------------------
             const uint32_t t0 = p.lo - p.u0, tn = min(p.hi - p.u0, p.s.past);      // tiles [t0, tn)
             const int32_t* table = a.block_tables + (size_t)p.b * a.width;
@@ -561,45 +582,59 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
             // (A thread per row left each load of a warp in 32 lines: 18,000 cycles a tile.)
             constexpr int RPW = 32 / W, STEPS = KT / (4 * RPW);
             const uint32_t c = lane % W, r0 = (warp & 3) * RPW + lane / W;
+            const auto copy_rows = [&](const void* base, uint64_t token, uint64_t head, uint32_t key0, unsigned char* tile_at) {
+                const __half* src = static_cast<const __half*>(base) + (p.s.rq.token0 + key0 + r0) * token + p.hk * head + 8 * c;
+                const uint32_t d = mma4::s_addr(tile_at) + (c >> 3) * C::PANEL;
+#pragma unroll 4
+                for (int i = 0; i < STEPS; ++i) {
+                    const uint32_t rr = r0 + 4 * RPW * i;
+                    const bool live = key0 + rr < p.s.rq.n;
+                    const __half* from = live ? src + (uint64_t)(4 * RPW * i) * token : static_cast<const __half*>(base);
+                    if (vec) {
+                        copy16(d + swizzled(rr, c & 7), from, live);
+                    } else {
+                        __half h[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) h[e] = live ? from[e] : __ushort_as_half(0);
+                        *reinterpret_cast<uint4*>(tile_at + (c >> 3) * C::PANEL + swizzled(rr, c & 7)) = *reinterpret_cast<const uint4*>(h);
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            // K and V copies are groups in turn; each is handed over when the one behind it
+            // is on its way
+            uint64_t* pending = nullptr;                        // the V in flight
+            const auto settle = [&]() {
+                if (pending == nullptr) return;
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                filled(pending);
+                pending = nullptr;
+            };
             for (uint32_t tile = max(t0, p.s.past); tile < p.hi - p.u0; ++tile, ++done) {
                 const uint32_t st = done % STAGES, use = done / STAGES, key0 = (tile - p.s.past) * KT;
-                const auto copy_rows = [&](const void* base, uint64_t token, uint64_t head, unsigned char* tile_at) {
-                    const __half* src = static_cast<const __half*>(base) + (p.s.rq.token0 + key0 + r0) * token + p.hk * head + 8 * c;
-                    const uint32_t d = mma4::s_addr(tile_at) + (c >> 3) * C::PANEL;
-#pragma unroll 4
-                    for (int i = 0; i < STEPS; ++i) {
-                        const uint32_t rr = r0 + 4 * RPW * i;
-                        const bool live = key0 + rr < p.s.rq.n;
-                        const __half* from = live ? src + (uint64_t)(4 * RPW * i) * token : static_cast<const __half*>(base);
-                        if (vec) {
-                            copy16(d + swizzled(rr, c & 7), from, live);
-                        } else {
-                            __half h[8];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) h[e] = live ? from[e] : __ushort_as_half(0);
-                            *reinterpret_cast<uint4*>(tile_at + (c >> 3) * C::PANEL + swizzled(rr, c & 7)) = *reinterpret_cast<const uint4*>(h);
-                        }
-                    }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                };
                 unsigned char* kd = smem + C::K + st * C::TILE;
                 unsigned char* vd = smem + C::V + st * C::TILE;
+                const bool all_see = key0 + KT - 1 <= p.tok0;   // every row sees every key
+                if (!all_see) settle();
                 if (use) wait(&k_empty[st], (use - 1) & 1, err);
-                copy_rows(a.new_k, a.k_token, a.k_head, kd);
-                if (key0 + KT - 1 <= p.tok0) {                 // every row sees every key
-                    asm volatile("cp.async.wait_group 0;" ::: "memory");
-                    filled(&k_full[st]);
+                copy_rows(a.new_k, a.k_token, a.k_head, key0, kd);
+                if (all_see) {
+                    if (pending != nullptr) {
+                        asm volatile("cp.async.wait_group 1;" ::: "memory");
+                        filled(pending);
+                    }
                     if (use) wait(&v_empty[st], (use - 1) & 1, err);
-                    copy_rows(a.new_v, a.v_token, a.v_head, vd);
-                    asm volatile("cp.async.wait_group 0;" ::: "memory");
-                    filled(&v_full[st]);
+                    copy_rows(a.new_v, a.v_token, a.v_head, key0, vd);
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    filled(&k_full[st]);
+                    pending = &v_full[st];
                     continue;
                 }
                 // A weight of zero does not keep an infinite or NaN value out of the rows that
                 // are masked from it. Such a value row is taken as zeros, and its key as NaN,
                 // which reaches the rows that see it and no other.
                 if (use) wait(&v_empty[st], (use - 1) & 1, err);
-                copy_rows(a.new_v, a.v_token, a.v_head, vd);
+                copy_rows(a.new_v, a.v_token, a.v_head, key0, vd);
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
                 __syncwarp();
 #pragma unroll 4
@@ -618,7 +653,8 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                 filled(&k_full[st]);
                 filled(&v_full[st]);
             }
-        }
+            settle();
+        } while (p.next(a, before, least_new, end));
     } else {
         // --------------------------- the MMAs -----------------------------------------
         if (warp < 14) {
@@ -631,9 +667,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
             const uint32_t base = mma4::s_addr(smem), q_at = base + C::Q + mt * C::TILE;
             const uint32_t s_at = tmem + C::S0 + 128 * mt, o_at = tmem + C::O0 + 128 * mt;
             uint32_t tiles = 0, parts = 0, steps = 0;              // done in front of this part
-            for (uint32_t at = start; at < end;) {
-                const Part p = part_at(a, before, least_new, at, end);
-                at = p.hi;
+            do {
                 const uint32_t n = (p.hi - p.lo) * (KT / KS), tile0 = tiles;
                 tiles += p.hi - p.lo;
                 if (mt == 1 && !p.second) {
@@ -687,7 +721,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                     __syncwarp();
                 }
                 steps += n;
-            }
+            } while (p.next(a, before, least_new, end));
             // nothing of this CTA's is in flight when its tensor memory goes
             if (elect_one()) umma_commit(&drained[mt]);
             for (const long long t0 = clock64(); !mbar_try_wait(&drained[mt], 0) && clock64() - t0 < WAIT_CYCLES;) {}
