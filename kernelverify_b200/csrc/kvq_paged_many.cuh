@@ -65,7 +65,6 @@ constexpr int ROWS = 128;                  // query rows per M tile
 constexpr int COLS = 2 * ROWS;             // query rows per unit
 constexpr int STAGES = 2;                  // K and V tiles in shared memory, each
 constexpr float RAISE = 14.0f, START = 4.0f;   // log2 room above the reference
-constexpr uint32_t SUSPEND_NS = 20000;
 constexpr long long WAIT_CYCLES = 2000000000ll;      // about a second
 
 template <int DH>
@@ -159,30 +158,15 @@ __device__ __forceinline__ uint64_t desc128(uint32_t saddr, uint32_t leading) {
 // byte offset of 16-byte chunk c (eight dims) of row r in a panel
 __device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
-// A test of a phase that may suspend the thread until it completes: a warp that
-// polls takes issue slots from the others.
-__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity), "r"(SUSPEND_NS)
-        : "memory");
-    return ok != 0;
-}
-// Every wait ends: after WAIT_CYCLES, or once another wait gave up.
-__device__ __forceinline__ void wait_long(uint32_t bar, uint32_t parity, volatile int* err) {
-    const long long t0 = clock64();
-    while (clock64() - t0 < WAIT_CYCLES) {
-        if (try_wait(bar, parity) || *err) return;
-    }
-    *err = 1;
-}
+// Every wait ends: after WAIT_CYCLES, or once another wait gave up. (Tests with a
+// time to suspend for woke up late: a part of one tile took 60 us.)
 __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* err) {
-    const uint32_t at = mma4::s_addr(bar);
-    if (!try_wait(at, parity)) wait_long(at, parity, err);
+    if (mbar_try_wait(bar, parity)) return;
+    const long long t0 = clock64();
+    do {
+        if (mbar_try_wait(bar, parity) || *err) return;
+    } while (clock64() - t0 < WAIT_CYCLES);
+    *err = 1;
 }
 
 // a word's eight codes -> fp16 scale * code + bias, rounded once. A byte in both
@@ -359,14 +343,17 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
         // ---------------------------- softmax ------------------------------------
         const int mt = wg, row = tid & 127;
         const uint32_t tokm = ROWS / a.r;
-        const uint32_t rt = row / a.r, rh = row - rt * a.r;          // the row's token of the M tile, head
+        const uint32_t rt = row / a.r;                               // the row's token of the M tile
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // TMEM lane 32 (warp % 4), bits 16 up
         const uint32_t s_at = tmem + lanes + C::S0 + 128 * mt, o_at = tmem + lanes + C::O0 + 128 * mt;
         const float scale2 = a.scale * 1.4426950408889634f;
+        // rows go in and out in whole lines: W lanes a row, RPW of the warp's 32 rows at once
+        constexpr int RPW = 32 / W;
+        const uint32_t r0 = (warp & 3) * 32 + lane / W, c0 = lane % W;
         uint32_t done = 0;                                           // steps
-        // step g's combine is done. Asked of the last step in front of one whose scores
-        // were seen, or of that one: those of two steps before are done then, so that
-        // the barrier of g's buffer is at g's phase or just behind it.
+        // step g's combine is done. A parity tells only neighbouring phases apart, and
+        // arrivals at different barriers may pass one another, so every phase of either
+        // buffer's barrier is waited for in turn (two steps behind, when it is long over).
         const auto combined = [&](uint32_t g) { wait(&pv_done[2 * mt + (g & 1)], (g >> 1) & 1, err); };
         do {
             if (mt == 1 && !p.second) continue;
@@ -374,28 +361,28 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
             const bool live = rt < tokm && tok < p.s.rq.n;
             // this M tile's queries (the last MMA that read the buffer is done: its
             // scores have been read)
-            {
-                unsigned char* dst = smem + C::Q + mt * C::TILE;
-                const __half* q = static_cast<const __half*>(a.q) + (p.s.rq.token0 + tok) * a.q_token + (p.hk * a.r + rh) * a.q_head;
+            unsigned char* q_tile = smem + C::Q + mt * C::TILE;
+            __syncwarp();
+#pragma unroll 4
+            for (int i = 0; i < 32 / RPW; ++i) {
+                const uint32_t r = r0 + RPW * i, t = r / a.r, h = r - t * a.r, of = p.tok0 + mt * tokm + t;
+                const bool has = t < tokm && of < p.s.rq.n;
+                const __half* from = static_cast<const __half*>(a.q) +
+                                     (has ? (p.s.rq.token0 + of) * a.q_token + (p.hk * a.r + h) * a.q_head + 8 * c0 : 0);
+                unsigned char* to = q_tile + (c0 >> 3) * C::PANEL + swizzled(r, c0 & 7);
+                if (vec) {
+                    copy16(mma4::s_addr(to), from, has);
+                } else {
+                    __half x[8];
 #pragma unroll
-                for (int c = 0; c < W; ++c) {
-                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                    if (live) {
-                        if (vec) {
-                            x = reinterpret_cast<const uint4*>(q)[c];
-                        } else {
-                            __half h[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) h[i] = q[8 * c + i];
-                            x = *reinterpret_cast<const uint4*>(h);
-                        }
-                    }
-                    *reinterpret_cast<uint4*>(dst + (c >> 3) * C::PANEL + swizzled(row, c & 7)) = x;
+                    for (int e = 0; e < 8; ++e) x[e] = has ? from[e] : __ushort_as_half(0);
+                    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(x);
                 }
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[mt]);
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[mt]);
             float ref = -INFINITY, l = 0.0f;
             const uint32_t steps = (p.hi - p.lo) * (KT / KS);
             for (uint32_t q = 0; q < steps; ++q, ++done) {
@@ -464,10 +451,12 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
                 tc_fence_before();
+                if (q >= 2) combined(done - 2);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[2 * mt + buf]);
             }
             // ---- the part's result ------------------------------------------------
+            combined(done - 2);
             combined(done - 1);
             __syncwarp();
             tc_fence_after();
@@ -475,31 +464,46 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
             const uint32_t col = mt * tokm * a.r + row;                 // row of the unit
             float* slot = reinterpret_cast<float*>(ws + split_bytes(gridDim.x)) +
                           (2 * (size_t)blockIdx.x + (p.u0 >= start ? 1 : 0)) * slot_floats(COLS, DH);
-            __half* out = static_cast<__half*>(a.out) +
-                          ((size_t)(p.s.rq.token0 + tok) * a.n_heads + p.hk * a.r + rh) * DH;
             const float inv = *err ? NAN : (whole ? 1.0f / l : 1.0f);
-#pragma unroll
-            for (int c = 0; c < DH; c += 32) {
-                uint32_t o[32];
+            // through this M tile's query buffer, whose MMAs are done, as rows of 2 DH bytes:
+            // the fp16 result, or the two halves of an fp32 part one after the other. Each
+            // warp uses the rows that it loads queries into: others may be at the next part.
+#pragma unroll 1
+            for (int half = 0; half < (whole ? 1 : 2); ++half) {
                 __syncwarp();
-                ld32(o_at + c, o);
-                tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    if (!live) break;
-                    float x[8];
+                for (int c = 0; c < DH; c += 32) {
+                    if (!whole && c / (DH / 2) != half) continue;
+                    uint32_t o[32];
+                    ld32(o_at + c, o);
+                    tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(o[i + e]) * inv;
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
                     if (whole) {
-                        alignas(16) __half2 h[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) h[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
-                        *reinterpret_cast<uint4*>(out + c + i) = *reinterpret_cast<const uint4*>(h);
-                    } else {
-                        float4* d = reinterpret_cast<float4*>(slot + 2 * COLS + (size_t)col * DH + c + i);
-                        d[0] = make_float4(x[0], x[1], x[2], x[3]);
-                        d[1] = make_float4(x[4], x[5], x[6], x[7]);
+                        for (int i = 0; i < 32; i += 2) {
+                            const __half2 h = __floats2half2_rn(__uint_as_float(o[i]), __uint_as_float(o[i + 1]));
+                            o[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
                     }
+                    const int first = whole ? c / 8 : (c % (DH / 2)) / 4;        // 16-byte chunk of the row
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (!whole || i < 4)
+                            *reinterpret_cast<uint4*>(q_tile + ((first + i) >> 3) * C::PANEL + swizzled(row, (first + i) & 7)) =
+                                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                }
+                __syncwarp();
+#pragma unroll 4
+                for (int i = 0; i < 32 / RPW; ++i) {
+                    const uint32_t r = r0 + RPW * i, t = r / a.r, h = r - t * a.r, of = p.tok0 + mt * tokm + t;
+                    if (t >= tokm || of >= p.s.rq.n) continue;
+                    const uint4 x = *reinterpret_cast<const uint4*>(q_tile + (c0 >> 3) * C::PANEL + swizzled(r, c0 & 7));
+                    if (whole)
+                        *reinterpret_cast<uint4*>(static_cast<__half*>(a.out) +
+                                                  ((size_t)(p.s.rq.token0 + of) * a.n_heads + p.hk * a.r + h) * DH + 8 * c0) = x;
+                    else
+                        *reinterpret_cast<uint4*>(slot + 2 * COLS + (size_t)(mt * tokm * a.r + r) * DH + half * (DH / 2) + 4 * c0) = x;
                 }
             }
             if (!whole && live) {
@@ -702,8 +706,6 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                             const uint64_t v = desc128(base + C::V + (vt % STAGES) * C::TILE + half * (KS * 128), C::PANEL);
 #pragma unroll
                             for (int k = 0; k < KS / 16; ++k) umma_ts(o_at, s_buf + 8 * k, v + k * (2048 >> 4), ID_O, q > 2 || k > 0);
-                            // in front of the scores' commit: whoever sees step q's scores knows
-                            // that all combines up to step q - 2 are done and counted
                             umma_commit(&pv_done[2 * mt + buf]);
                             if (half) umma_commit(&v_empty[vt % STAGES]);
                         }

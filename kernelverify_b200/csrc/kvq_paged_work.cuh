@@ -107,7 +107,7 @@ __device__ __forceinline__ uint32_t row_of_tile(const uint32_t* before, uint32_t
 // that walked them took 12 us.
 constexpr int JOIN_WARPS = 8;
 template <typename T, int DH, int COLS>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(Attend a, const unsigned char* __restrict__ ws) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(Attend a, const unsigned char* ws) {
     constexpr int V = DH / 32;             // dims per lane
     constexpr int PW = COLS > 32 ? 1 : 4;  // warps per column
     constexpr int JC = JOIN_WARPS / PW;    // columns per block
@@ -119,7 +119,13 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(Attend a, const u
     pdl_wait();
     const uint32_t cta = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % PW;
     const uint32_t col = blockIdx.y * JC + warp / PW;
-    const Split u = reinterpret_cast<const Split*>(ws)[cta];
+    // this grid may have been launched while the one that wrote the parts still ran:
+    // they are read through L2, past lines an SM may have cached
+    Split u;
+    {
+        const uint32_t* s = reinterpret_cast<const uint32_t*>(reinterpret_cast<const Split*>(ws) + cta);
+        u = {__ldcg(s), __ldcg(s + 1), __ldcg(s + 2), __ldcg(s + 3), __ldcg(s + 4)};
+    }
     if (u.parts == 0 || blockIdx.y * JC >= u.cols) return;
     const float* slots = reinterpret_cast<const float*>(ws + split_bytes(gridDim.x));
     // part 0 is this CTA's slot 1, part p > 0 CTA cta + p's slot 0
@@ -137,9 +143,9 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) join_kernel(Attend a, const u
                 pm[i] = -INFINITY;
                 if (p < u.parts) {
                     const float* s = part(p);
-                    pm[i] = s[col];
-                    pl[i] = s[COLS + col];
-                    v[i] = *reinterpret_cast<const Vec*>(s + 2 * COLS + (size_t)col * DH + lane * V);
+                    pm[i] = __ldcg(s + col);
+                    pl[i] = __ldcg(s + COLS + col);
+                    v[i] = __ldcg(reinterpret_cast<const Vec*>(s + 2 * COLS + (size_t)col * DH + lane * V));
                 }
             }
 #pragma unroll

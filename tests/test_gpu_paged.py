@@ -360,6 +360,19 @@ def test_attend_is_repeatable_and_streams_do_not_share():
         assert all(torch.equal(x, w) for x in g)
 
 
+@pytest.mark.parametrize("case", [([60, 50], [200, 3], 2, 4), ([700, 0, 33], [130, 64, 9], 4, 2), ([300], [5], 8, 8)])
+def test_attend_same_bits_many_times(case):
+    """Short units of several lengths behind one another in every CTA's share,
+    call after call: a buffer taken over too early shows as a differing bit."""
+    s = Step(*case, 128, 64, 16, F16, packed=False)
+    want = s.call(paged).clone()
+    s.check(want)
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(400):
+        differ += (s.call(paged) != want).sum()
+    assert differ.item() == 0
+
+
 def test_attend_captured_step_follows_lengths():
     """One captured step replayed for other lengths within its bounds, beside
     a second graph of the same tensors."""
