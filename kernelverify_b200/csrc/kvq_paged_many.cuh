@@ -127,26 +127,6 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// 2^x of two values on the FMA pipe: x = n + r with |r| <= 1/2 by adding and
-// taking away 1.5 * 2^23, a polynomial for 2^r (fitted to it in relative error:
-// 5.5e-6 at most), n added to the exponent. Below -126 as at -126, which is 0 in
-// fp16; not for NaN. The special-function unit gives 16 exponentials a cycle to
-// an SM and is what the softmax waits for: POLY of eight pairs are taken off it.
-constexpr int POLY = 3;
-constexpr float P0 = 0.99999803f, P1 = 0.69313157f, P2 = 0.24027981f, P3 = 0.055894606f, P4 = 0.0094680814f;
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    const auto both = [](float v) { return make_float2(v, v); };
-    x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
-    const float2 t = __fadd2_rn(x, both(12582912.0f));
-    const float2 r = __fadd2_rn(x, __ffma2_rn(t, both(-1.0f), both(12582912.0f)));
-    float2 p = __ffma2_rn(r, both(P4), both(P3));
-    p = __ffma2_rn(p, r, both(P2));
-    p = __ffma2_rn(p, r, both(P1));
-    p = __ffma2_rn(p, r, both(P0));
-    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                       __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
-}
-
 // Descriptor of an operand with the 128-byte swizzle: rows of 128 bytes, eight
 // to a 1024-byte atom. K-major (Q, K): the rows are M or N, atoms along them
 // 1024 bytes apart. MN-major (V): the rows are K, atoms along them 1024 bytes
@@ -160,10 +140,13 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t c) { return r 
 
 // Every wait ends: after WAIT_CYCLES, or once another wait gave up. (Tests with a
 // time to suspend for woke up late: a part of one tile took 60 us.)
+template <bool SLACK = false>
 __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* err) {
     if (mbar_try_wait(bar, parity)) return;
     const long long t0 = clock64();
     do {
+        // a role that is tiles ahead leaves the issue slots to the others
+        if (SLACK) __nanosleep(100);
         if (mbar_try_wait(bar, parity) || *err) return;
     } while (clock64() - t0 < WAIT_CYCLES);
     *err = 1;
@@ -343,7 +326,11 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
         // ---------------------------- softmax ------------------------------------
         const int mt = wg, row = tid & 127;
         const uint32_t tokm = ROWS / a.r;
-        const uint32_t rt = row / a.r;                               // the row's token of the M tile
+        // x / R by a multiplication: exact for x < 128, R <= 128 (the excess stays below
+        // 128 / 65536 < 1 / R)
+        const uint32_t inv_r = (65536u + a.r - 1) / a.r;
+        const auto token_of = [&](uint32_t x) { return x * inv_r >> 16; };
+        const uint32_t rt = token_of(row);                           // the row's token of the M tile
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // TMEM lane 32 (warp % 4), bits 16 up
         const uint32_t s_at = tmem + lanes + C::S0 + 128 * mt, o_at = tmem + lanes + C::O0 + 128 * mt;
         const float scale2 = a.scale * 1.4426950408889634f;
@@ -365,7 +352,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
             __syncwarp();
 #pragma unroll 4
             for (int i = 0; i < 32 / RPW; ++i) {
-                const uint32_t r = r0 + RPW * i, t = r / a.r, h = r - t * a.r, of = p.tok0 + mt * tokm + t;
+                const uint32_t r = r0 + RPW * i, t = token_of(r), h = r - t * a.r, of = p.tok0 + mt * tokm + t;
                 const bool has = t < tokm && of < p.s.rq.n;
                 const __half* from = static_cast<const __half*>(a.q) +
                                      (has ? (p.s.rq.token0 + of) * a.q_token + (p.hk * a.r + h) * a.q_head + 8 * c0 : 0);
@@ -437,12 +424,8 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
 #pragma unroll
                 for (int c = 0; c < KS; c += 2) {
                     float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), mul2, sub2);
-                    if (c / 2 % 8 < POLY) {
-                        x = exp2_poly(x);
-                    } else {
-                        x.x = ex2(x.x);
-                        x.y = ex2(x.y);
-                    }
+                    x.x = ex2(x.x);
+                    x.y = ex2(x.y);
                     sum[(c >> 1) & 1] = __fadd2_rn(sum[(c >> 1) & 1], x);
                     const __half2 h = __floats2half2_rn(x.x, x.y);
                     s[c >> 1] = *reinterpret_cast<const uint32_t*>(&h);
@@ -496,7 +479,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                 __syncwarp();
 #pragma unroll 4
                 for (int i = 0; i < 32 / RPW; ++i) {
-                    const uint32_t r = r0 + RPW * i, t = r / a.r, h = r - t * a.r, of = p.tok0 + mt * tokm + t;
+                    const uint32_t r = r0 + RPW * i, t = token_of(r), h = r - t * a.r, of = p.tok0 + mt * tokm + t;
                     if (t >= tokm || of >= p.s.rq.n) continue;
                     const uint4 x = *reinterpret_cast<const uint4*>(q_tile + (c0 >> 3) * C::PANEL + swizzled(r, c0 & 7));
                     if (whole)
@@ -571,13 +554,13 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
 #pragma unroll
                     for (int i = 0; i < G; ++i) kz[i] = __ushort_as_half(0x7FFF);
                 }
-                if (use) wait(&k_empty[st], (use - 1) & 1, err);
+                if (use) wait<true>(&k_empty[st], (use - 1) & 1, err);
                 put(smem + C::K + st * C::TILE, kw, ks, kz);
                 filled(&k_full[st]);
                 r = row_of(tile + 1, page, kind);
                 read(kind, r, a.k, kw, ks, kz);
                 page = page_of(tile + 2);
-                if (use) wait(&v_empty[st], (use - 1) & 1, err);
+                if (use) wait<true>(&v_empty[st], (use - 1) & 1, err);
                 put(smem + C::V + st * C::TILE, vw, vs, vz);
                 filled(&v_full[st]);
                 read(kind, r, a.v, vw, vs, vz);
@@ -620,14 +603,14 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                 unsigned char* vd = smem + C::V + st * C::TILE;
                 const bool all_see = key0 + KT - 1 <= p.tok0;   // every row sees every key
                 if (!all_see) settle();
-                if (use) wait(&k_empty[st], (use - 1) & 1, err);
+                if (use) wait<true>(&k_empty[st], (use - 1) & 1, err);
                 copy_rows(a.new_k, a.k_token, a.k_head, key0, kd);
                 if (all_see) {
                     if (pending != nullptr) {
                         asm volatile("cp.async.wait_group 1;" ::: "memory");
                         filled(pending);
                     }
-                    if (use) wait(&v_empty[st], (use - 1) & 1, err);
+                    if (use) wait<true>(&v_empty[st], (use - 1) & 1, err);
                     copy_rows(a.new_v, a.v_token, a.v_head, key0, vd);
                     asm volatile("cp.async.wait_group 1;" ::: "memory");
                     filled(&k_full[st]);
@@ -637,7 +620,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                 // A weight of zero does not keep an infinite or NaN value out of the rows that
                 // are masked from it. Such a value row is taken as zeros, and its key as NaN,
                 // which reaches the rows that see it and no other.
-                if (use) wait(&v_empty[st], (use - 1) & 1, err);
+                if (use) wait<true>(&v_empty[st], (use - 1) & 1, err);
                 copy_rows(a.new_v, a.v_token, a.v_head, key0, vd);
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
                 __syncwarp();
