@@ -6,8 +6,9 @@
 // packed word) of a row, so a group's minimum and maximum are shuffles over
 // GROUP / 8 lanes and a row is read and written once, whole sectors at a time.
 // The CTA's warps take consecutive tokens of one cache head, which lie side by
-// side in a page. Bound by the bytes moved once the step is long, by the launch
-// for a few tokens.
+// side in a page. Bound by instructions once the step is long (so the arithmetic
+// below is what it is), by the launch for a few tokens. Four tokens per lane,
+// loaded ahead, were slower: 33 us against 25 for 8192 tokens of 8 heads.
 #include "kvq_common.cuh"
 #include "kvq_paged.h"
 
@@ -21,24 +22,39 @@ __device__ __forceinline__ float half_away(float x) {
     return copysignf(floorf(__fadd_rn(fabsf(x), 0.5f)), x);
 }
 
-// min(half_away(x / step), 15) as the canonical quantizer has it, mostly
-// without its division. y = x * (1 / step) with both factors rounded is within
-// 3 * 2^-24 of the rounded quotient relatively, so within 2^-18 below 16, and
-// the rounded sum with 0.5 adds 2^-21 at most: where |y| + 0.5 stands further
-// than 2^-17 from a whole number (from 16 up every value gives 15), the
-// quotient's floor is the same. The rest, about one value in 2^16 of smooth
-// data, divides; so do NaN and infinities, which fail the comparison.
-__device__ __forceinline__ uint32_t code_of(float x, float step, float inv) {
-    const float y = __fmul_rn(x, inv);
-    const float s = __fadd_rn(fabsf(y), 0.5f);
-    const float f = floorf(s), d = s - f;
-    if (d > 7.62939453125e-6f && d < 1.0f - 7.62939453125e-6f) return (uint32_t)fminf(copysignf(f, y) + 0.0f, 15.0f);
-    return (uint32_t)(int)fminf(half_away(__fdiv_rn(x, step)), 15.0f);
+// The codes min(half_away((x - bias) / step), 15) of eight values as the
+// canonical quantizer has them, mostly without its division. y = (x - bias) *
+// (1 / step) with the last two rounded is within 3 * 2^-24 of the rounded
+// quotient relatively, so within 2^-18 below 16, and the rounded sum with 0.5
+// adds 2^-21 at most: where s = |y| + 0.5 stands further than 2^-17 from a whole
+// number, the quotient's floor is the same (from 15.75 up every value gives 15,
+// and so does NaN, here as there). If one of the eight stands nearer, about one
+// lane in 2^13 of smooth data, all of them divide. The floor is the low bits of
+// s + 2^23 rounded down, and the eight are put together in one word with those
+// of 2^23, whose sum is taken off at the end.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float bias, float step) {
+    const float inv = __frcp_rn(step);
+    uint32_t word = 0;
+    float worst = 0.0f;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {
+        const float s = fminf(__fadd_rn(fabsf(__fmul_rn(__fsub_rn(x[i], bias), inv)), 0.5f), 15.75f);
+        const float t = __fadd_rd(s, 8388608.0f);
+        worst = fmaxf(worst, fabsf(__fsub_rn(__fsub_rn(s, 0.5f), __fsub_rn(t, 8388608.0f))));
+        word = word * 16u + __float_as_uint(t);
+    }
+    word -= 0x4B000000u * 0x11111111u;
+    if (worst < 0.5f - 7.62939453125e-6f) return word;
+    word = 0;
+#pragma unroll 1
+    for (int i = 7; i >= 0; --i)
+        word = word * 16u + (uint32_t)(int)fminf(half_away(__fdiv_rn(__fsub_rn(x[i], bias), step)), 15.0f);
+    return word;
 }
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8]) {
-    if (vec) {
+template <bool VEC, typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+    if constexpr (VEC) {
         constexpr int N = 8 * sizeof(T) / 16;
         uint4 raw[N];
 #pragma unroll
@@ -52,7 +68,7 @@ __device__ __forceinline__ void load8(const T* p, bool vec, float (&x)[8]) {
     }
 }
 
-template <typename T, int DH, int GROUP>
+template <typename T, int DH, int GROUP, bool VEC>
 __global__ void __launch_bounds__(THREADS) append_kernel(Rows r) {
     constexpr int LANES = DH / 8;                  // lanes of a row
     constexpr int GL = GROUP / 8;                  // lanes of a group
@@ -68,8 +84,8 @@ __global__ void __launch_bounds__(THREADS) append_kernel(Rows r) {
 
     float x[8];
     if (live)
-        load8(static_cast<const T*>(r.src[side]) + tok * r.token_stride[side] +
-                  head * r.head_stride[side] + lane * 8, r.vec, x);
+        load8<VEC>(static_cast<const T*>(r.src[side]) + tok * r.token_stride[side] +
+                       head * r.head_stride[side] + lane * 8, x);
     else
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = 0.0f;
@@ -94,10 +110,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(Rows r) {
     if (!degenerate) step = __fdiv_rn(edge, n_edge);
     const float bias = degenerate ? 0.0f : edge;
 
-    const float inv = __frcp_rn(step);
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) word |= code_of(__fsub_rn(x[i], bias), step, inv) << (4 * i);
+    const uint32_t word = codes_of(x, bias, step);
     if (!live) return;
     const uint64_t page = (uint64_t)slot >> r.page_shift;
     const uint64_t row = ((page * r.heads + head) << r.page_shift) + ((uint64_t)slot & ((1u << r.page_shift) - 1));
@@ -112,9 +125,9 @@ __global__ void __launch_bounds__(THREADS) append_kernel(Rows r) {
 
 // Values scale * code + bias (a rounded multiply, a rounded add, then the
 // output type's rounding); zeros for a slot that is not in the pool.
-template <typename T, typename TO>
+template <typename T, typename TO, int DH, int GROUP>
 __global__ void __launch_bounds__(THREADS) gather_kernel(Rows r) {
-    const uint32_t lanes = r.head_dim / 8, rows = THREADS / lanes;
+    constexpr uint32_t lanes = DH / 8, rows = THREADS / lanes;
     const uint32_t lane = threadIdx.x % lanes;
     const uint32_t tok = blockIdx.x * rows + threadIdx.x / lanes;
     const uint32_t head = blockIdx.y >> 1, side = blockIdx.y & 1;
@@ -127,36 +140,61 @@ __global__ void __launch_bounds__(THREADS) gather_kernel(Rows r) {
         const uint64_t page = (uint64_t)slot >> r.page_shift;
         const uint64_t row = ((page * r.heads + head) << r.page_shift) + ((uint64_t)slot & ((1u << r.page_shift) - 1));
         const Pool& p = r.pool[side];
-        const uint64_t g = row * (r.head_dim / r.group) + lane * 8 / r.group;
+        const uint64_t g = row * (DH / GROUP) + lane * 8 / GROUP;
         const uint32_t w = p.words[row * lanes + lane];
         const float s = to_f32(static_cast<const T*>(p.scales)[g]);
         const float b = to_f32(static_cast<const T*>(p.biases)[g]);
+        // codes i and i + 4 as fp16 1024 + c (even i) or 1024 + 16 c; s * c is one
+        // rounded multiply-add of that, as 1024 s and s / 16 are exact
+        const float s16 = s * 0.0625f, m1024 = s * -1024.0f, m64 = s * -64.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = from_f32<TO>(dequant(s, (w >> (4 * i)) & 15u, b));
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t h = ((i & 2 ? w >> 8 : w) & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;
+            const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&h));
+            v[i] = from_f32<TO>(__fadd_rn(i & 1 ? fmaf(c.x, s16, m64) : fmaf(c.x, s, m1024), b));
+            v[i + 4] = from_f32<TO>(__fadd_rn(i & 1 ? fmaf(c.y, s16, m64) : fmaf(c.y, s, m1024), b));
+        }
     }
-    TO* out = static_cast<TO*>(r.dst[side]) + ((uint64_t)tok * r.heads + head) * r.head_dim + lane * 8;
+    TO* out = static_cast<TO*>(r.dst[side]) + ((uint64_t)tok * r.heads + head) * DH + lane * 8;
 #pragma unroll
     for (int i = 0; i < (int)(8 * sizeof(TO) / 16); ++i)
         reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(v)[i];
 }
 
-template <typename T, int DH, int GROUP>
-static cudaError_t append_one(const Rows& r, cudaStream_t stream) {
-    constexpr uint32_t ROWS = THREADS / (DH / 8);
-    append_kernel<T, DH, GROUP><<<dim3((r.tokens + ROWS - 1) / ROWS, 2 * r.heads), THREADS, 0, stream>>>(r);
-    return cudaGetLastError();
+// f(head_dim, group) as constants
+template <typename F>
+static cudaError_t by_format(const Rows& r, F&& f) {
+    using std::integral_constant;
+    switch (r.head_dim * 1000 + r.group) {
+        case 64032: return f(integral_constant<int, 64>{}, integral_constant<int, 32>{});
+        case 64064: return f(integral_constant<int, 64>{}, integral_constant<int, 64>{});
+        case 128032: return f(integral_constant<int, 128>{}, integral_constant<int, 32>{});
+        case 128064: return f(integral_constant<int, 128>{}, integral_constant<int, 64>{});
+        case 128128: return f(integral_constant<int, 128>{}, integral_constant<int, 128>{});
+    }
+    return cudaErrorInvalidValue;
+}
+
+static dim3 grid_of(const Rows& r) {
+    const uint32_t rows = THREADS / (r.head_dim / 8);
+    return dim3((r.tokens + rows - 1) / rows, 2 * r.heads);
 }
 
 template <typename T>
 static cudaError_t append_typed(const Rows& r, cudaStream_t stream) {
-    switch (r.head_dim * 1000 + r.group) {
-        case 64032: return append_one<T, 64, 32>(r, stream);
-        case 64064: return append_one<T, 64, 64>(r, stream);
-        case 128032: return append_one<T, 128, 32>(r, stream);
-        case 128064: return append_one<T, 128, 64>(r, stream);
-        case 128128: return append_one<T, 128, 128>(r, stream);
-    }
-    return cudaErrorInvalidValue;
+    return by_format(r, [&](auto dh, auto group) {
+        if (r.vec) append_kernel<T, dh.value, group.value, true><<<grid_of(r), THREADS, 0, stream>>>(r);
+        else append_kernel<T, dh.value, group.value, false><<<grid_of(r), THREADS, 0, stream>>>(r);
+        return cudaGetLastError();
+    });
+}
+
+template <typename T, typename TO>
+static cudaError_t gather_typed(const Rows& r, cudaStream_t stream) {
+    return by_format(r, [&](auto dh, auto group) {
+        gather_kernel<T, TO, dh.value, group.value><<<grid_of(r), THREADS, 0, stream>>>(r);
+        return cudaGetLastError();
+    });
 }
 
 cudaError_t launch_append(const Rows& r, cudaStream_t stream) {
@@ -164,15 +202,8 @@ cudaError_t launch_append(const Rows& r, cudaStream_t stream) {
 }
 
 cudaError_t launch_gather(const Rows& r, cudaStream_t stream) {
-    const uint32_t rows = THREADS / (r.head_dim / 8);
-    const dim3 grid((r.tokens + rows - 1) / rows, 2 * r.heads);
-    if (r.dtype == KVQ_F32)
-        gather_kernel<float, float><<<grid, THREADS, 0, stream>>>(r);
-    else if (r.out_dtype == KVQ_F32)
-        gather_kernel<__half, float><<<grid, THREADS, 0, stream>>>(r);
-    else
-        gather_kernel<__half, __half><<<grid, THREADS, 0, stream>>>(r);
-    return cudaGetLastError();
+    if (r.dtype == KVQ_F32) return gather_typed<float, float>(r, stream);
+    return r.out_dtype == KVQ_F32 ? gather_typed<__half, float>(r, stream) : gather_typed<__half, __half>(r, stream);
 }
 
 }  // namespace paged

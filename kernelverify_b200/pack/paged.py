@@ -58,22 +58,23 @@ class PageBatch(NamedTuple):
 
 
 def _check(name, ten, shape, dtype, device) -> None:
-    """A contiguous tensor of exactly this shape, dtype and device (the library
-    indexes it by its address alone)."""
+    """A contiguous tensor of exactly this shape and dtype on CUDA device
+    `device` (its index; the library indexes it by its address alone)."""
     if ten.shape != shape:
         raise ValueError(f"{name} has shape {tuple(ten.shape)}, expected {tuple(shape)}")
     if ten.dtype != dtype:
         raise ValueError(f"{name} is {ten.dtype}, expected {dtype}")
     if not ten.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    if ten.device != device:
-        raise ValueError(f"{name} is on {ten.device}, expected {device}")
+    if ten.get_device() != device:
+        raise ValueError(f"{name} is on {ten.device}, expected cuda:{device}")
 
 
-def _cuda_device(name, ten):
-    if not ten.is_cuda:
+def _cuda_device(name, ten) -> int:
+    device = ten.get_device()
+    if device < 0:
         raise ValueError(f"{name} must be a CUDA tensor")
-    return ten.device
+    return device
 
 
 def _page_size(page_size: int) -> int:
@@ -86,21 +87,23 @@ def _call(entry, device, stream, *args) -> None:
     """entry(*args, stream handle) with `device` current, so a tensor's device
     decides where the kernel runs, not the caller's current one."""
     torch = _torch()
-    if torch.cuda.current_device() == device.index:
-        s = stream if stream is not None else torch.cuda.current_stream()
-        _native.check(entry(*args, s.cuda_stream))
+    if torch._C._cuda_getDevice() == device:
+        _native.check(entry(*args, stream.cuda_stream if stream is not None
+                            else torch._C._cuda_getCurrentRawStream(device)))
         return
     with torch.cuda.device(device):
-        s = stream if stream is not None else torch.cuda.current_stream(device)
-        _native.check(entry(*args, s.cuda_stream))
+        _native.check(entry(*args, stream.cuda_stream if stream is not None
+                            else torch._C._cuda_getCurrentRawStream(device)))
 
 
-def _on_stream(stream, make):
-    """make() with its allocations belonging to `stream` (None: the current)."""
+def _empty(stream, shape, dtype, device):
+    """An unwritten tensor whose memory belongs to `stream` (None: the current
+    one), so that it is reused after that stream's work."""
+    torch = _torch()
     if stream is None:
-        return make()
-    with _torch().cuda.stream(stream):
-        return make()
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _tables(lens, step, block_tables, free_pages, n_free, page_size):
@@ -124,14 +127,13 @@ def _tables(lens, step, block_tables, free_pages, n_free, page_size):
     return device, rows, width, pool
 
 
-def empty_batch(rows: int, max_tokens: int, device) -> PageBatch:
+def empty_batch(rows: int, max_tokens: int, device, stream=None) -> PageBatch:
     """Unwritten buffers of a step's tables, for `build_tables(out=...)`."""
     torch = _torch()
-    i32 = torch.int32
-    one = torch.empty(2 * rows + 3 + max_tokens, dtype=i32, device=device)
-    cu, lens, n_free, status, pos = one.split([rows + 1, rows, 1, 1, max_tokens])
-    return PageBatch(cu, torch.empty(max_tokens, dtype=torch.int64, device=device), pos, lens,
-                     n_free, status)
+    cu, lens, n_free, status, pos = _empty(
+        stream, 2 * rows + 3 + max_tokens, torch.int32, device).split_with_sizes(
+            [rows + 1, rows, 1, 1, max_tokens])
+    return PageBatch(cu, _empty(stream, max_tokens, torch.int64, device), pos, lens, n_free, status)
 
 
 def build_tables(lens, new_lens, block_tables, free_pages, n_free, *, page_size: int,
@@ -151,7 +153,7 @@ def build_tables(lens, new_lens, block_tables, free_pages, n_free, *, page_size:
     if max_tokens < 0:
         raise ValueError(f"max_tokens {max_tokens} is negative")
     if out is None:
-        out = _on_stream(stream, lambda: empty_batch(rows, max_tokens, device))
+        out = empty_batch(rows, max_tokens, lens.device, stream)
     else:
         torch = _torch()
         _check("out.slots", out.slots, (max_tokens,), torch.int64, device)
@@ -177,8 +179,7 @@ def truncate(lens, keep, block_tables, free_pages, n_free, *, page_size: int, ou
     device, rows, width, pool = _tables(lens, keep, block_tables, free_pages, n_free, page_size)
     torch = _torch()
     if out is None:
-        lens_out, n_out = _on_stream(stream, lambda: torch.empty(
-            rows + 1, dtype=torch.int32, device=device).split([rows, 1]))
+        lens_out, n_out = _empty(stream, rows + 1, torch.int32, lens.device).split_with_sizes([rows, 1])
     else:
         lens_out, n_out = out
         _check("out[0]", lens_out, (rows,), torch.int32, device)
@@ -207,11 +208,13 @@ def _pools(k_wq, k_scales, k_biases, v_wq, v_scales, v_biases):
         raise ValueError(f"page_size {page} not in {PAGE_SIZES}")
     if groups == 0 or head_dim % groups or head_dim // groups not in SUPPORTED_GROUPS:
         raise ValueError(f"{groups} groups per row: group_size must be one of {SUPPORTED_GROUPS}")
-    dtype, wdt, lead = k_scales.dtype, k_wq.dtype, (pages, heads, page, groups)
+    dtype, wdt, shape, lead = k_scales.dtype, k_wq.dtype, k_wq.shape, k_scales.shape
     if wdt != torch.int32 and wdt != torch.uint32:
         raise ValueError("packed words must be int32/uint32 tensors")
-    _check("k_wq", k_wq, k_wq.shape, wdt, device)
-    _check("v_wq", v_wq, k_wq.shape, wdt, device)
+    if lead[:3] != shape[:3]:
+        raise ValueError(f"k_scales has shape {tuple(lead)}, expected {tuple(shape[:3])} first")
+    _check("k_wq", k_wq, shape, wdt, device)
+    _check("v_wq", v_wq, shape, wdt, device)
     _check("k_scales", k_scales, lead, dtype, device)
     _check("k_biases", k_biases, lead, dtype, device)
     _check("v_scales", v_scales, lead, dtype, device)
@@ -228,8 +231,8 @@ def _rows(name, ten, shape, dtype, device):
         raise ValueError(f"{name} has shape {tuple(ten.shape)}, expected {tuple(shape)}")
     if ten.dtype != dtype:
         raise ValueError(f"{name} is {ten.dtype}; the cache holds {dtype}")
-    if ten.device != device:
-        raise ValueError(f"{name} is on {ten.device}, expected {device}")
+    if ten.get_device() != device:
+        raise ValueError(f"{name} is on {ten.device}, expected cuda:{device}")
     token, head, dim = ten.stride()
     if dim != 1:
         raise ValueError(f"{name}'s head_dim must be contiguous")
@@ -272,7 +275,7 @@ def gather(k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, slots, *, dtype=N
     dtype = held if dtype is None else dtype
     if dtype != held and dtype != torch.float32:
         raise ValueError(f"dtype {dtype}: the cache's {held} or float32")
-    out = _on_stream(stream, lambda: torch.empty((2, n, heads, head_dim), dtype=dtype, device=device))
+    out = _empty(stream, (2, n, heads, head_dim), dtype, k_wq.device)
     keys, values = out.unbind(0)
     a = KvqPagedRows(*pool, keys.data_ptr(), values.data_ptr(), slots.data_ptr(), 0, 0, 0, 0, n,
                      heads, head_dim, group, pages, page, _dtype_code(held), _dtype_code(dtype))
@@ -324,7 +327,7 @@ def attend(q, k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, new_k, new_v, 
     if max_new < 0:
         raise ValueError(f"max_new {max_new} is negative")
     if out is None:
-        out = _on_stream(stream, lambda: torch.empty((n, n_heads, head_dim), dtype=dtype, device=device))
+        out = _empty(stream, (n, n_heads, head_dim), dtype, q.device)
     else:
         _check("out", out, (n, n_heads, head_dim), dtype, device)
     a = KvqPagedArgs(qp, kp, vp, *pool, block_tables.data_ptr(), ctx_lens.data_ptr(),
@@ -338,9 +341,9 @@ def attend(q, k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, new_k, new_v, 
         # a buffer of the call's own unless the caller keeps one: the allocator
         # orders its reuse after this call, and a captured step's is its graph's
         if workspace is None:
-            buf, have = _on_stream(stream, lambda: torch.empty(need, dtype=torch.uint8, device=device)), need
+            buf, have = _empty(stream, need, torch.uint8, q.device), need
         else:
-            buf, have = workspace.get(need, device, stream)
+            buf, have = workspace.get(need, q.device, stream)
         ws = buf.data_ptr()
     _call(lib.kvq_paged_attend, device, stream, ref, out.data_ptr(), ws, have)
     return out
