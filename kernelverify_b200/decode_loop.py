@@ -21,6 +21,11 @@ torch/cuBLAS, so only the attention arm differs between A and B.
 
     python -m kernelverify_b200.decode_loop --smoke
     python -m kernelverify_b200.decode_loop --ab [--bits 4 8] [--prompt 512 896]
+    python -m kernelverify_b200.decode_loop --paged [--prompt 512 896] [--batch 8]
+
+--paged runs the same decoder over a paged 4-bit cache: prompts of different
+lengths prefilled in one ragged step, then a captured decode step of the whole
+batch (tables, append, attention and the greedy pick on the device).
 """
 
 from __future__ import annotations
@@ -33,7 +38,8 @@ import time
 from dataclasses import dataclass
 
 from kernelverify_b200.pack import kv_attention as kva
-from kernelverify_b200.serving import (DecodeRouter, FullPrecisionKVCache, QuantizedKVCache)
+from kernelverify_b200.serving import (DecodeRouter, FullPrecisionKVCache, PagedKVCache,
+                                       PagedSequences, QuantizedKVCache, stock_paged_attention)
 
 GROUP_SIZE = 64
 
@@ -115,10 +121,11 @@ class Decoder:
         x1, x2 = x.chunk(2, dim=-1)
         return x * cos + torch.cat([-x2, x1], dim=-1) * sin
 
-    def run(self, tokens, cos, sin, attend):
-        """tokens [B, L] -> last-position logits [B, vocab]. attend(i, q, k, v)
-        is layer i's attention on post-RoPE q [B, H, L, DH], k / v
-        [B, HKV, L, DH] (it owns the cache update)."""
+    def run(self, tokens, cos, sin, attend, last=None):
+        """tokens [B, L] -> last-position logits [B, vocab], or with `last`
+        (indices into the L positions of a ragged batch, B = 1) the logits of
+        those positions. attend(i, q, k, v) is layer i's attention on post-RoPE
+        q [B, H, L, DH], k / v [B, HKV, L, DH] (it owns the cache update)."""
         torch = _torch()
         F = torch.nn.functional
         s = self.shape
@@ -136,7 +143,7 @@ class Decoder:
             h = F.rms_norm(x, (s.hidden,), lw["n_post"], s.eps)
             gate, up = F.linear(h, lw["wgu"]).chunk(2, dim=-1)
             x = x + F.linear(F.silu(gate) * up, lw["wd"])
-        x = F.rms_norm(x[:, -1], (s.hidden,), self.n_final, s.eps)
+        x = F.rms_norm(x[:, -1] if last is None else x[0, last], (s.hidden,), self.n_final, s.eps)
         return F.linear(x, self.embed)
 
     def forward(self, tokens, caches, router):
@@ -374,6 +381,164 @@ def ab_graph(model: Decoder, batch: int, prompt: int, steps: int, bits: int = 4,
     return row
 
 
+class PagedDecode:
+    """Greedy generation of a batch of requests of any lengths over a paged
+    4-bit cache (`serving.PagedSequences`, one `PagedKVCache` per layer).
+
+    `prefill(prompts)` takes a list of token lists, one per row (an empty list
+    leaves its row empty), in one ragged step; `step()` decodes a token of
+    every live row, eagerly or, after `capture()`, as one graph replay that
+    needs nothing from the host. `release(rows)` ends requests and returns
+    their pages. `tok` [B] holds each row's latest token. With `shadow` (eager
+    steps only) every attention is also taken through the stock composition;
+    `shadow_gap` is the largest distance between the two, `shadow_mag` the
+    largest magnitude."""
+
+    def __init__(self, model: Decoder, batch: int, max_len: int, pages: int | None = None,
+                 page_size: int = 64, group_size: int = GROUP_SIZE, shadow: bool = False):
+        torch = _torch()
+        s = model.shape
+        pages = batch * -(-max_len // page_size) if pages is None else pages
+        self.model, self.batch, self.max_len = model, batch, max_len
+        self.seqs = PagedSequences(batch, pages, max_len, page_size, model.device)
+        self.caches = [PagedKVCache(self.seqs, s.n_kv_heads, s.head_dim, group_size, model.dtype)
+                       for _ in range(s.n_layers)]
+        self.tok = torch.zeros(batch, dtype=torch.long, device=model.device)
+        self.live = torch.zeros(batch, dtype=torch.int32, device=model.device)
+        self.workspace = kva.Workspace()
+        self.graph = None
+        self.shadow, self.shadow_gap, self.shadow_mag = shadow, 0.0, 0.0
+
+    def _run(self, tokens, batch, max_new):
+        """Logits [B, vocab] of each row's last new token: one ragged pass."""
+        model = self.model
+        cos, sin = model.rope_tables(batch.positions.float()[None])
+
+        def attend(i, q, k, v):
+            q, k, v = (x[0].transpose(0, 1) for x in (q, k, v))
+            cache = self.caches[i]
+            cache.append(k, v, batch)
+            out = cache.attend(q, k, v, batch, max_new, workspace=self.workspace)
+            if self.shadow:
+                new = batch.cu_new.diff().tolist()
+                ref = stock_paged_attention(q, k, v, cache, self.seqs.lens.tolist(), new)[:sum(new)]
+                gap = (out[:sum(new)].float() - ref.float()).abs().max()
+                self.shadow_gap = max(self.shadow_gap, float(gap))
+                self.shadow_mag = max(self.shadow_mag, float(ref.abs().max()))
+            return out.transpose(0, 1)[None]
+
+        last = (batch.cu_new[1:] - 1).clamp(min=0).long()
+        return model.run(tokens[None], cos, sin, attend, last=last)
+
+    def prefill(self, prompts) -> None:
+        torch = _torch()
+        if len(prompts) != self.batch:
+            raise ValueError(f"{len(prompts)} prompts for a batch of {self.batch}")
+        new = [len(p) for p in prompts]
+        total = sum(new)
+        if total == 0:
+            return
+        device = self.model.device
+        tokens = torch.tensor([t for p in prompts for t in p], dtype=torch.long, device=device)
+        new_lens = torch.tensor(new, dtype=torch.int32, device=device)
+        with torch.inference_mode():
+            batch = self.seqs.begin(new_lens, total)
+            if batch.status.item():
+                raise ValueError(f"the prompts do not fit the cache (status {batch.status.item()})")
+            logits = self._run(tokens, batch, max(new))
+            self.seqs.commit(batch)
+            took = new_lens > 0
+            self.tok.copy_(torch.where(took, logits.argmax(-1), self.tok))
+            self.live.copy_(torch.where(took, torch.ones_like(self.live), self.live))
+
+    def step(self):
+        """One token of every live row (eager). Returns the step's status
+        tensor: a step that did not fit decodes nothing."""
+        torch = _torch()
+        with torch.inference_mode():
+            batch = self.seqs.begin(self.live, self.batch)
+            tokens = torch.zeros_like(self.tok)
+            at = batch.cu_new[:-1].long().clamp(max=self.batch - 1)
+            # dead rows' writes land on a position that a live row owns or on padding
+            order = torch.where(self.live > 0, at, torch.full_like(at, self.batch))
+            tokens = torch.cat([tokens, tokens[:1]]).scatter_(0, order, self.tok)[:-1]
+            logits = self._run(tokens, batch, 1)
+            went = (self.live > 0) & (batch.status == 0)
+            self.tok.copy_(torch.where(went, logits.argmax(-1), self.tok))
+            self.seqs.commit(batch)
+            return batch.status
+
+    def capture(self, warmup: int = 2) -> None:
+        """Capture one step; the state is what it was before."""
+        torch = _torch()
+        s, device = self.seqs, self.model.device
+        saved = [x.clone() for x in (self.tok, s.lens, s.n_free, s.block_tables)]
+        side = torch.cuda.Stream(device)
+        side.wait_stream(torch.cuda.current_stream(device))
+        with torch.cuda.stream(side):
+            for _ in range(warmup):
+                self.step()
+        torch.cuda.current_stream(device).wait_stream(side)
+        # a workspace of its own: no other call may replace the graph's buffer
+        self.workspace = kva.Workspace()
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph):
+            self.status = self.step()
+        for x, y in zip((self.tok, s.lens, s.n_free, s.block_tables), saved):
+            x.copy_(y)
+        self._graph_workspace, self.workspace = self.workspace, kva.Workspace()
+
+    def replay(self):
+        """One captured step."""
+        if self.graph is None:
+            self.capture()
+        self.graph.replay()
+        return self.status
+
+    def release(self, rows) -> None:
+        """End the requests of `rows`: their pages go back, their rows are empty."""
+        torch = _torch()
+        keep = torch.full((self.batch,), 2 ** 31 - 1, dtype=torch.int32, device=self.model.device)
+        keep[list(rows)] = 0
+        self.seqs.truncate(keep)
+        self.live[list(rows)] = 0
+
+
+def paged_run(model: Decoder, lengths, steps: int, page_size: int = 64, seed: int = 0) -> dict:
+    """Prompts of `lengths` prefilled in one ragged step, then `steps` captured
+    decode steps of the batch: decode tokens/s (CUDA events), the pages held, and
+    how far the fused attention is from the stock composition over a prefill and
+    two eager steps of the same requests."""
+    torch = _torch()
+    check = PagedDecode(model, len(lengths), max(lengths) + 2, page_size=page_size, shadow=True)
+    check.prefill([make_prompt(model, 1, n, seed + i)[0].tolist() for i, n in enumerate(lengths)])
+    for _ in range(2):
+        check.step()
+    gap, gate = check.shadow_gap, 4e-3 * max(1.0, check.shadow_mag)
+    del check
+    d = PagedDecode(model, len(lengths), max(lengths) + steps + 2, page_size=page_size)
+    prompts = [make_prompt(model, 1, n, seed + i)[0].tolist() for i, n in enumerate(lengths)]
+    t0 = time.perf_counter()
+    d.prefill(prompts)
+    torch.cuda.synchronize(model.device)
+    prefill_s = time.perf_counter() - t0
+    d.capture()
+    start, stop = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    for _ in range(steps):
+        d.replay()
+    stop.record()
+    stop.synchronize()
+    held = d.seqs.pages - int(d.seqs.n_free.item())
+    row = {"mode": "paged", "bits": 4, "prompt": list(lengths), "steps": steps,
+           "prefill_s": round(prefill_s, 4),
+           "tps": round(steps * len(lengths) / (start.elapsed_time(stop) / 1e3), 1),
+           "pages_held": held, "status": int(d.status.item()),
+           "lens": d.seqs.lens.tolist(), "shadow_gap": gap, "gate": gate, "ok": gap <= gate}
+    d.graph = None
+    return row
+
+
 def make_prompt(model: Decoder, batch: int, length: int, seed: int = 0):
     torch = _torch()
     g = torch.Generator(device="cpu")
@@ -457,6 +622,8 @@ def main(argv=None) -> int:
     mode.add_argument("--ab", action="store_true")
     mode.add_argument("--ab-graph", action="store_true",
                       help="the captured-step A/B (GPU-bound tokens/s)")
+    mode.add_argument("--paged", action="store_true",
+                      help="a paged 4-bit cache: ragged prefill, captured decode steps")
     ap.add_argument("--tiny", action="store_true", help="a 2-layer decoder instead of Qwen3-4B")
     ap.add_argument("--bits", type=int, nargs="*", default=[4, 8])
     ap.add_argument("--prompt", type=int, nargs="*", default=[512, 896])
@@ -469,6 +636,11 @@ def main(argv=None) -> int:
         report = smoke(model)
         print(json.dumps(report))
         return 0 if report["ok"] else 1
+    if args.paged:
+        lengths = [args.prompt[i % len(args.prompt)] for i in range(max(args.batch, len(args.prompt)))]
+        row = paged_run(model, lengths, args.steps)
+        print(json.dumps(row))
+        return 0 if row["ok"] and row["status"] == 0 else 1
     if args.ab_graph:
         for bits in args.bits:
             for p in args.prompt:

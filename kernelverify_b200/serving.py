@@ -39,6 +39,7 @@ import math
 from dataclasses import dataclass, field
 
 from kernelverify_b200.pack import kv_attention as kva
+from kernelverify_b200.pack import paged
 
 
 ROW_ALIGN = 64
@@ -141,6 +142,125 @@ class QuantizedKVCache:
             return kva.dequant(*sl, self.bits)
 
         return deq(self.keys), deq(self.values)
+
+
+class PagedSequences:
+    """The requests of a continuous batch and the pages they hold, one for all
+    layers: `lens` int32 [B], `block_tables` int32 [B, W], the stack
+    `free_pages` / `n_free`, all on the device. A request of length 0 is an
+    empty row of the batch.
+
+    A step is `begin(new_lens, max_tokens)`, the layers' `append` and `attend`
+    with the batch it returns, then `commit(batch)`. Nothing here asks the
+    device for a length, so a step can be captured; `batch.status` tells a step
+    that did not fit (it takes no page and writes nothing)."""
+
+    def __init__(self, batch: int, pages: int, max_len: int, page_size: int = 64, device="cuda"):
+        torch = _torch()
+        if page_size not in paged.PAGE_SIZES:
+            raise ValueError(f"page_size {page_size} not in {paged.PAGE_SIZES}")
+        if not 1 <= batch <= paged.MAX_ROWS:
+            raise ValueError(f"{batch} requests: 1 to {paged.MAX_ROWS}")
+        if pages < 1 or max_len < 1:
+            raise ValueError("pages and max_len must be >= 1")
+        self.batch, self.pages, self.page_size = batch, pages, page_size
+        self.width = -(-max_len // page_size)
+        i32 = torch.int32
+        self.lens = torch.zeros(batch, dtype=i32, device=device)
+        self.block_tables = torch.full((batch, self.width), -1, dtype=i32, device=device)
+        self.free_pages = torch.arange(pages, dtype=i32, device=device)
+        self.n_free = torch.full((1,), pages, dtype=i32, device=device)
+
+    def begin(self, new_lens, max_tokens: int, out=None):
+        """The step's PageBatch for new_lens (int32 [B], on the device)."""
+        return paged.build_tables(self.lens, new_lens, self.block_tables, self.free_pages,
+                                  self.n_free, page_size=self.page_size, max_tokens=max_tokens,
+                                  out=out)
+
+    def commit(self, batch) -> None:
+        """Take the step's tokens into the lengths, once its layers are done."""
+        self.lens.copy_(batch.lens)
+        self.n_free.copy_(batch.n_free)
+
+    def truncate(self, keep) -> None:
+        """Cut request b to keep[b] positions (int32 [B], on the device; 0 ends
+        it) and return the pages behind them."""
+        lens, n_free = paged.truncate(self.lens, keep, self.block_tables, self.free_pages,
+                                      self.n_free, page_size=self.page_size)
+        self.lens.copy_(lens)
+        self.n_free.copy_(n_free)
+
+
+class PagedKVCache:
+    """One layer's packed 4-bit K/V pools for a `PagedSequences`: keys / values
+    are (words int32 [pages, HKV, page_size, DH/8], scales [pages, HKV,
+    page_size, DH/group], biases)."""
+
+    def __init__(self, sequences: PagedSequences, n_kv_heads: int, head_dim: int,
+                 group_size: int = 64, dtype=None):
+        torch = _torch()
+        dtype = torch.float16 if dtype is None else dtype
+        if head_dim not in kva.SUPPORTED_DH:
+            raise ValueError(f"head_dim {head_dim} not in {kva.SUPPORTED_DH}")
+        if group_size not in kva.SUPPORTED_GROUPS or head_dim % group_size:
+            raise ValueError(f"group_size {group_size} not in {kva.SUPPORTED_GROUPS}")
+        self.sequences, self.dtype = sequences, dtype
+        self.n_kv_heads, self.head_dim, self.group_size = n_kv_heads, head_dim, group_size
+        lead = (sequences.pages, n_kv_heads, sequences.page_size)
+        device = sequences.lens.device
+
+        def triplet():
+            return (torch.zeros(lead + (head_dim // 8,), dtype=torch.int32, device=device),
+                    torch.zeros(lead + (head_dim // group_size,), dtype=dtype, device=device),
+                    torch.zeros(lead + (head_dim // group_size,), dtype=dtype, device=device))
+
+        self.keys, self.values = triplet(), triplet()
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in self.keys + self.values)
+
+    def append(self, keys, values, batch) -> None:
+        """Quantize the step's keys / values [N, HKV, DH] into its slots."""
+        paged.append(keys, values, *self.keys, *self.values, batch.slots)
+
+    def attend(self, queries, keys, values, batch, max_new: int, max_ctx: int | None = None,
+               workspace=None):
+        """The step's attention [N, H, DH] over the positions cached before it
+        and its own keys / values; call it before `commit`."""
+        s = self.sequences
+        return paged.attend(queries, *self.keys, *self.values, keys, values,
+                            block_tables=s.block_tables, ctx_lens=s.lens, cu_new=batch.cu_new,
+                            max_new=max_new, max_ctx=max_ctx, workspace=workspace)
+
+    def dequantized(self, row: int, length: int):
+        """(K, V) [length, HKV, DH] in the cache dtype: request `row`'s first
+        positions, read back (what the stock composition attends over)."""
+        torch = _torch()
+        s = self.sequences
+        pos = torch.arange(length, device=s.lens.device)
+        slots = s.block_tables[row, pos // s.page_size].long() * s.page_size + pos % s.page_size
+        return paged.gather(*self.keys, *self.values, slots)
+
+
+def stock_paged_attention(queries, keys, values, cache: PagedKVCache, lens, new_lens):
+    """The stock composition of a paged step: request by request, its cached
+    positions read back and torch attention over them and the step's own
+    entries. lens / new_lens: host lists. [N, H, DH] -> [N, H, DH]."""
+    torch = _torch()
+    out, at = torch.empty_like(queries), 0
+    for row, (length, n) in enumerate(zip(lens, new_lens)):
+        sl = slice(at, at + n)
+        at += n
+        if n == 0:
+            continue
+        k, v = cache.dequantized(row, length)
+        k, v = (torch.cat([x, y[sl]]).transpose(0, 1)[None] for x, y in ((k, keys), (v, values)))
+        o = torch.nn.functional.scaled_dot_product_attention(
+            queries[sl].transpose(0, 1)[None], k, v,
+            attn_mask=_causal_mask(n, length + n, queries.device),
+            enable_gqa=k.shape[1] != queries.shape[1])
+        out[sl] = o[0].transpose(0, 1)
+    return out
 
 
 class FullPrecisionKVCache:

@@ -152,3 +152,18 @@ def test_python_refuses_cpu_tensors():
     s = torch.zeros(1, 1, 16, 2, dtype=torch.float16)
     with pytest.raises(ValueError, match="CUDA"):
         paged.gather(w, s, s, w, s, s, torch.zeros(1, dtype=torch.int64))
+
+
+def test_serving_classes_check_their_arguments():
+    from kernelverify_b200 import serving
+    seqs = serving.PagedSequences(3, 10, 100, 16, device="cpu")
+    assert seqs.width == 7 and seqs.n_free.item() == 10 and seqs.block_tables.shape == (3, 7)
+    cache = serving.PagedKVCache(seqs, 2, 64, 32)
+    assert cache.keys[0].shape == (10, 2, 16, 8) and cache.values[1].shape == (10, 2, 16, 2)
+    assert cache.nbytes() == 10 * 2 * 16 * 2 * (32 + 2 * 2 * 2)
+    for bad in (dict(batch=0), dict(pages=0), dict(max_len=0), dict(page_size=20), dict(batch=5000)):
+        with pytest.raises(ValueError):
+            serving.PagedSequences(**(dict(batch=3, pages=10, max_len=100, device="cpu") | bad))
+    for bad in (dict(head_dim=96), dict(head_dim=64, group_size=128)):
+        with pytest.raises(ValueError):
+            serving.PagedKVCache(seqs, **(dict(n_kv_heads=2, head_dim=64) | bad))
