@@ -23,11 +23,10 @@ No reference counterpart: its cache is one padded buffer per sequence
 
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import NamedTuple
 
 from kernelverify_b200 import _native
-from kernelverify_b200._native import KvqPagedArgs, KvqPagedRows, KvqTables
 from kernelverify_b200.pack.kv_attention import (SUPPORTED_DH, SUPPORTED_GROUPS, Workspace,
                                                  _dtype_code)
 
@@ -37,10 +36,22 @@ MAX_ROWS = 4096
 # bits of PageBatch.status
 POOL_EMPTY, ROW_FULL, TOO_MANY_TOKENS = 1, 2, 4
 
+# The C argument blocks (kvq_tables, kvq_paged_rows, kvq_paged_args), packed in
+# one go: a step makes two of these calls per layer, and the host's part of a
+# call is most of a small step's time.
+_TABLES = struct.Struct("@11Q5I4x")
+_ROWS = struct.Struct("@13Q8I")
+_ARGS = struct.Struct("@18Q12I")
+
+_torch_module = None
+
 
 def _torch():
-    import torch
-    return torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
 
 
 class PageBatch(NamedTuple):
@@ -96,14 +107,13 @@ def _call(entry, device, stream, *args) -> None:
                             else torch._C._cuda_getCurrentRawStream(device)))
 
 
-def _empty(stream, shape, dtype, device):
-    """An unwritten tensor whose memory belongs to `stream` (None: the current
-    one), so that it is reused after that stream's work."""
-    torch = _torch()
+def _empty(stream, like, shape, dtype):
+    """An unwritten tensor on `like`'s device whose memory belongs to `stream`
+    (None: the current one), so that it is reused after that stream's work."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
+    with _torch().cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
 
 
 def _tables(lens, step, block_tables, free_pages, n_free, page_size):
@@ -118,22 +128,33 @@ def _tables(lens, step, block_tables, free_pages, n_free, page_size):
     if block_tables.dim() != 2 or free_pages.dim() != 1:
         raise ValueError("block_tables must be [B, W] and free_pages [pages]")
     width, pool = block_tables.shape[1], free_pages.shape[0]
-    _check("lens", lens, (rows,), i32, device)
-    _check("block_tables", block_tables, (rows, width), i32, device)
-    _check("free_pages", free_pages, (pool,), i32, device)
-    _check("n_free", n_free, (1,), i32, device)
-    _check("new_lens or keep", step, (rows,), i32, device)
+    if not (step.shape == (rows,) and n_free.shape == (1,) and block_tables.shape[0] == rows
+            and lens.dtype == step.dtype == block_tables.dtype == free_pages.dtype == n_free.dtype == i32
+            and lens.is_contiguous() and step.is_contiguous() and block_tables.is_contiguous()
+            and free_pages.is_contiguous()
+            and step.get_device() == block_tables.get_device() == free_pages.get_device()
+            == n_free.get_device() == device):
+        # something is off: find out what
+        _check("lens", lens, (rows,), i32, device)
+        _check("block_tables", block_tables, (rows, width), i32, device)
+        _check("free_pages", free_pages, (pool,), i32, device)
+        _check("n_free", n_free, (1,), i32, device)
+        _check("new_lens or keep", step, (rows,), i32, device)
     _page_size(page_size)
     return device, rows, width, pool
 
 
-def empty_batch(rows: int, max_tokens: int, device, stream=None) -> PageBatch:
-    """Unwritten buffers of a step's tables, for `build_tables(out=...)`."""
+def _batch(stream, like, rows: int, max_tokens: int) -> PageBatch:
     torch = _torch()
     cu, lens, n_free, status, pos = _empty(
-        stream, 2 * rows + 3 + max_tokens, torch.int32, device).split_with_sizes(
+        stream, like, 2 * rows + 3 + max_tokens, torch.int32).split_with_sizes(
             [rows + 1, rows, 1, 1, max_tokens])
-    return PageBatch(cu, _empty(stream, max_tokens, torch.int64, device), pos, lens, n_free, status)
+    return PageBatch(cu, _empty(stream, like, max_tokens, torch.int64), pos, lens, n_free, status)
+
+
+def empty_batch(rows: int, max_tokens: int, device) -> PageBatch:
+    """Unwritten buffers of a step's tables, for `build_tables(out=...)`."""
+    return _batch(None, _torch().empty(0, device=device), rows, max_tokens)
 
 
 def build_tables(lens, new_lens, block_tables, free_pages, n_free, *, page_size: int,
@@ -150,22 +171,21 @@ def build_tables(lens, new_lens, block_tables, free_pages, n_free, *, page_size:
     the caller reads when it suits it: its slots are -1 and its `cu_new` 0, so
     the step's `append` and `attend` do nothing."""
     device, rows, width, pool = _tables(lens, new_lens, block_tables, free_pages, n_free, page_size)
-    if max_tokens < 0:
-        raise ValueError(f"max_tokens {max_tokens} is negative")
+    if not 0 <= max_tokens < 2 ** 31:
+        raise ValueError(f"max_tokens {max_tokens} is outside [0, 2^31)")
     if out is None:
-        out = empty_batch(rows, max_tokens, lens.device, stream)
+        out = _batch(stream, lens, rows, max_tokens)
     else:
         torch = _torch()
         _check("out.slots", out.slots, (max_tokens,), torch.int64, device)
         for name, n in (("cu_new", rows + 1), ("positions", max_tokens), ("lens", rows),
                         ("n_free", 1), ("status", 1)):
             _check("out." + name, getattr(out, name), (n,), torch.int32, device)
-    a = KvqTables(lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(),
-                  free_pages.data_ptr(), n_free.data_ptr(), out.cu_new.data_ptr(),
-                  out.slots.data_ptr(), out.positions.data_ptr(), out.lens.data_ptr(),
-                  out.n_free.data_ptr(), out.status.data_ptr(), rows, width, pool, page_size,
-                  max_tokens)
-    _call(_native.lib().kvq_paged_tables, device, stream, ctypes.byref(a))
+    _call(_native.lib().kvq_paged_tables, device, stream, _TABLES.pack(
+        lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(), free_pages.data_ptr(),
+        n_free.data_ptr(), out.cu_new.data_ptr(), out.slots.data_ptr(), out.positions.data_ptr(),
+        out.lens.data_ptr(), out.n_free.data_ptr(), out.status.data_ptr(), rows, width, pool,
+        page_size, max_tokens))
     return out
 
 
@@ -179,16 +199,15 @@ def truncate(lens, keep, block_tables, free_pages, n_free, *, page_size: int, ou
     device, rows, width, pool = _tables(lens, keep, block_tables, free_pages, n_free, page_size)
     torch = _torch()
     if out is None:
-        lens_out, n_out = _empty(stream, rows + 1, torch.int32, lens.device).split_with_sizes([rows, 1])
+        lens_out, n_out = _empty(stream, lens, rows + 1, torch.int32).split_with_sizes([rows, 1])
     else:
         lens_out, n_out = out
         _check("out[0]", lens_out, (rows,), torch.int32, device)
         _check("out[1]", n_out, (1,), torch.int32, device)
-    a = KvqTables(lens=lens.data_ptr(), step=keep.data_ptr(), block_tables=block_tables.data_ptr(),
-                  free_pages=free_pages.data_ptr(), n_free=n_free.data_ptr(),
-                  lens_out=lens_out.data_ptr(), n_free_out=n_out.data_ptr(), rows=rows,
-                  width=width, pool=pool, page_size=page_size)
-    _call(_native.lib().kvq_paged_truncate, device, stream, ctypes.byref(a))
+    _call(_native.lib().kvq_paged_truncate, device, stream, _TABLES.pack(
+        lens.data_ptr(), keep.data_ptr(), block_tables.data_ptr(), free_pages.data_ptr(),
+        n_free.data_ptr(), 0, 0, 0, lens_out.data_ptr(), n_out.data_ptr(), 0, rows, width, pool,
+        page_size, 0))
     return lens_out, n_out
 
 
@@ -213,12 +232,19 @@ def _pools(k_wq, k_scales, k_biases, v_wq, v_scales, v_biases):
         raise ValueError("packed words must be int32/uint32 tensors")
     if lead[:3] != shape[:3]:
         raise ValueError(f"k_scales has shape {tuple(lead)}, expected {tuple(shape[:3])} first")
-    _check("k_wq", k_wq, shape, wdt, device)
-    _check("v_wq", v_wq, shape, wdt, device)
-    _check("k_scales", k_scales, lead, dtype, device)
-    _check("k_biases", k_biases, lead, dtype, device)
-    _check("v_scales", v_scales, lead, dtype, device)
-    _check("v_biases", v_biases, lead, dtype, device)
+    if not (v_wq.shape == shape and k_biases.shape == v_scales.shape == v_biases.shape == lead
+            and v_wq.dtype == wdt and k_biases.dtype == v_scales.dtype == v_biases.dtype == dtype
+            and k_wq.is_contiguous() and v_wq.is_contiguous() and k_scales.is_contiguous()
+            and k_biases.is_contiguous() and v_scales.is_contiguous() and v_biases.is_contiguous()
+            and v_wq.get_device() == k_scales.get_device() == k_biases.get_device()
+            == v_scales.get_device() == v_biases.get_device() == device):
+        # something is off: find out what
+        for name, ten, want, kind in (("k_wq", k_wq, shape, wdt), ("v_wq", v_wq, shape, wdt),
+                                      ("k_scales", k_scales, lead, dtype),
+                                      ("k_biases", k_biases, lead, dtype),
+                                      ("v_scales", v_scales, lead, dtype),
+                                      ("v_biases", v_biases, lead, dtype)):
+            _check(name, ten, want, kind, device)
     return (device, dtype, pages, heads, page, head_dim, head_dim // groups,
             (k_wq.data_ptr(), k_scales.data_ptr(), k_biases.data_ptr(), v_wq.data_ptr(),
              v_scales.data_ptr(), v_biases.data_ptr()))
@@ -256,9 +282,9 @@ def append(keys, values, k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, slo
     vp, vt, vh = _rows("values", values, (n, heads, head_dim), dtype, device)
     _check("slots", slots, (n,), _torch().int64, device)
     code = _dtype_code(dtype)
-    a = KvqPagedRows(*pool, kp, vp, slots.data_ptr(), kt, kh, vt, vh, n, heads, head_dim, group,
-                     pages, page, code, code)
-    _call(_native.lib().kvq_paged_append, device, stream, ctypes.byref(a))
+    _call(_native.lib().kvq_paged_append, device, stream, _ROWS.pack(
+        *pool, kp, vp, slots.data_ptr(), kt, kh, vt, vh, n, heads, head_dim, group, pages, page,
+        code, code))
 
 
 def gather(k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, slots, *, dtype=None, stream=None):
@@ -275,11 +301,11 @@ def gather(k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, slots, *, dtype=N
     dtype = held if dtype is None else dtype
     if dtype != held and dtype != torch.float32:
         raise ValueError(f"dtype {dtype}: the cache's {held} or float32")
-    out = _empty(stream, (2, n, heads, head_dim), dtype, k_wq.device)
+    out = _empty(stream, k_wq, (2, n, heads, head_dim), dtype)
     keys, values = out.unbind(0)
-    a = KvqPagedRows(*pool, keys.data_ptr(), values.data_ptr(), slots.data_ptr(), 0, 0, 0, 0, n,
-                     heads, head_dim, group, pages, page, _dtype_code(held), _dtype_code(dtype))
-    _call(_native.lib().kvq_paged_gather, device, stream, ctypes.byref(a))
+    _call(_native.lib().kvq_paged_gather, device, stream, _ROWS.pack(
+        *pool, keys.data_ptr(), values.data_ptr(), slots.data_ptr(), 0, 0, 0, 0, n, heads,
+        head_dim, group, pages, page, _dtype_code(held), _dtype_code(dtype)))
     return keys, values
 
 
@@ -317,33 +343,37 @@ def attend(q, k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, new_k, new_v, 
     rows, width = block_tables.shape
     if not 1 <= rows <= MAX_ROWS:
         raise ValueError(f"{rows} requests: 1 to {MAX_ROWS}")
-    _check("block_tables", block_tables, block_tables.shape, i32, device)
-    _check("ctx_lens", ctx_lens, (rows,), i32, device)
-    _check("cu_new", cu_new, (rows + 1,), i32, device)
+    if not (ctx_lens.shape == (rows,) and cu_new.shape == (rows + 1,)
+            and block_tables.dtype == ctx_lens.dtype == cu_new.dtype == i32
+            and block_tables.is_contiguous() and ctx_lens.is_contiguous() and cu_new.is_contiguous()
+            and block_tables.get_device() == ctx_lens.get_device() == cu_new.get_device() == device):
+        # something is off: find out what
+        _check("block_tables", block_tables, block_tables.shape, i32, device)
+        _check("ctx_lens", ctx_lens, (rows,), i32, device)
+        _check("cu_new", cu_new, (rows + 1,), i32, device)
     if max_ctx is None:
         max_ctx = width * page
     if not 0 <= max_ctx <= width * page:
         raise ValueError(f"max_ctx {max_ctx} is outside [0, {width * page}]: the tables hold {width} pages")
-    if max_new < 0:
-        raise ValueError(f"max_new {max_new} is negative")
+    if not 0 <= max_new < 2 ** 31:
+        raise ValueError(f"max_new {max_new} is outside [0, 2^31)")
     if out is None:
-        out = _empty(stream, (n, n_heads, head_dim), dtype, q.device)
+        out = _empty(stream, q, (n, n_heads, head_dim), dtype)
     else:
         _check("out", out, (n, n_heads, head_dim), dtype, device)
-    a = KvqPagedArgs(qp, kp, vp, *pool, block_tables.data_ptr(), ctx_lens.data_ptr(),
-                     cu_new.data_ptr(), qt, qh, kt, kh, vt, vh, rows, n, n_heads, heads, head_dim,
-                     group, pages, page, width, max_ctx, max_new, _dtype_code(dtype))
+    a = _ARGS.pack(qp, kp, vp, *pool, block_tables.data_ptr(), ctx_lens.data_ptr(),
+                   cu_new.data_ptr(), qt, qh, kt, kh, vt, vh, rows, n, n_heads, heads, head_dim,
+                   group, pages, page, width, max_ctx, max_new, _dtype_code(dtype))
     lib = _native.lib()
-    ref = ctypes.byref(a)
-    need = lib.kvq_paged_workspace_bytes(ref)
+    need = lib.kvq_paged_workspace_bytes(a)
     ws, have = None, 0
     if need:
         # a buffer of the call's own unless the caller keeps one: the allocator
         # orders its reuse after this call, and a captured step's is its graph's
         if workspace is None:
-            buf, have = _empty(stream, need, torch.uint8, q.device), need
+            buf, have = _empty(stream, q, need, torch.uint8), need
         else:
             buf, have = workspace.get(need, q.device, stream)
         ws = buf.data_ptr()
-    _call(lib.kvq_paged_attend, device, stream, ref, out.data_ptr(), ws, have)
+    _call(lib.kvq_paged_attend, device, stream, a, out.data_ptr(), ws, have)
     return out

@@ -167,3 +167,13 @@ def test_serving_classes_check_their_arguments():
     for bad in (dict(head_dim=96), dict(head_dim=64, group_size=128)):
         with pytest.raises(ValueError):
             serving.PagedKVCache(seqs, **(dict(n_kv_heads=2, head_dim=64) | bad))
+
+
+def test_packed_argument_blocks_are_the_structures():
+    """The blocks that are packed by hand have the C structures' layout."""
+    for form, struct_type in ((paged._TABLES, _native.KvqTables), (paged._ROWS, _native.KvqPagedRows),
+                              (paged._ARGS, _native.KvqPagedArgs)):
+        assert form.size == ctypes.sizeof(struct_type)
+        names = [n for n, _ in struct_type._fields_]
+        got = struct_type.from_buffer_copy(form.pack(*range(1, len(names) + 1)))
+        assert [getattr(got, n) for n in names] == list(range(1, len(names) + 1))
