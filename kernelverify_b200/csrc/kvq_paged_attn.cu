@@ -24,32 +24,64 @@ uint32_t grid_for(uint64_t tiles, uint64_t least, uint64_t most) {
     return (uint32_t)(n < 1 ? 1 : (n > most ? most : n));
 }
 
+// us on a B200 below: 8 cache heads of 128, groups of 64, a captured call.
+//
+// A request is the few kernel's while its columns (new tokens x shared heads) fit
+// two passes of 16. 32 requests of 8192 cached positions, R = 4, n new tokens each,
+// few / many: n = 1 71 / 252, n = 4 123 / 258, n = 6 195 / 260, n = 8 227 / 262;
+// one of 131072, n = 8: 123 / 137. A third pass would lose: n = 9 346 (five of
+// eight columns: 315) / 262. 31 requests of 8192 and
+// 2 tokens each beside a chunk of 512: 112 with the few kernel, 575 as units of the
+// many kernel with 8 of 256 rows in use.
+constexpr uint32_t FEW_COLS = 32;
+
+// Columns per pass. Up to four are held once per block of a tile (4 columns: 71
+// against 73 with 8, 32 x 8192). Two tiles of eight save a pass but leave room for
+// 8 warps instead of 12: 16 columns 123 against 136 (32 x 8192, n = 4), 73 against 76
+// (1 x 131072), 45 either way (32 x 8192 of 2 cache heads, R = 16), but 37 against 34
+// (32 x 1024) and 19 against 15 (1 x 32768 of one cache head, R = 16), where a warp
+// has few tiles. 24 columns are three passes of eight (195) or two of sixteen (216).
+uint32_t columns(uint64_t cols, uint64_t row_tiles, uint64_t sms) {
+    if (cols <= 4) return 4;
+    const uint64_t p8 = (cols + 7) / 8, p16 = (cols + 15) / 16;
+    return p8 == 2 * p16 && row_tiles * p8 > 20 * 12 * sms ? 16 : 8;
+}
+
 Choice choose(const Attend& a) {
     Choice c{};
     c.fits = true;
     const uint64_t cols = (uint64_t)a.max_new * a.r, sms = (uint64_t)sm_count();
     const uint64_t rows = a.rows < a.tokens ? a.rows : a.tokens;
+    const uint64_t row_tiles = rows * a.n_kv_heads * ((uint64_t)a.max_ctx / 32 + 1);
     c.few_most = 0xFFFFFFFFu;
-    c.cols = a.dtype == KVQ_F32 ? 8 : cols <= 4 ? 4 : cols <= 8 ? 8 : 16;
-    if (a.dtype == KVQ_F16 && a.r <= 128 && cols > 16) {
-        // one request: the many kernel alone, whatever it brings
-        c.cols = a.r <= 4 ? 4 : 8;
-        c.few_most = a.rows == 1 ? 0 : (a.r >= c.cols ? 1 : c.cols / a.r);
-        // units have at most 256 query rows
+    if (a.dtype == KVQ_F32) {
+        c.cols = 8;
+    } else if (a.r > 128 || cols <= FEW_COLS) {
+        c.cols = columns(cols, row_tiles, sms);
+    } else {
+        // one request: the many kernel alone (its bound is what it brings, but for a
+        // padded batch), so that no second pair of launches finds nothing to do
+        c.few_most = rows == 1 ? 0 : FEW_COLS / a.r;
+        // 8 columns cost a batch of single tokens 2 us of 107 and save one of pairs 14
+        c.cols = columns(a.r > 8 ? a.r : 8, row_tiles, sms);
+        // units have at most 256 query rows; no CTA for less than two tiles (64 tokens
+        // over 512: 21 us, with four 28, with one 21)
         const uint64_t tu = 2 * (128 / a.r), units = (uint64_t)a.n_kv_heads * (a.tokens / tu + rows);
         const uint64_t tiles = units * (((uint64_t)a.max_ctx + a.max_new) / MANY_KEYS + 2);
         c.fits = tiles < TOO_MANY;
-        c.many_grid = grid_for(tiles, 4, sms);
+        c.many_grid = grid_for(tiles, 2, sms);
         const size_t es = 2;
         c.vec = true;
         for (const void* p : {a.q, a.new_k, a.new_v}) c.vec = c.vec && reinterpret_cast<uintptr_t>(p) % 16 == 0;
         for (uint64_t st : {a.q_token, a.q_head, a.k_token, a.k_head, a.v_token, a.v_head}) c.vec = c.vec && st * es % 16 == 0;
     }
     if (c.few_most) {
-        // no CTA for less than a tile per warp
+        // passes of a request, of all of them at most one each more than their tokens fill
         const uint64_t few = c.few_most < a.max_new ? c.few_most : a.max_new, w = c.cols;
-        const uint64_t tiles = rows * a.n_kv_heads * ((few * a.r + w - 1) / w) * ((uint64_t)a.max_ctx / 32 + 1);
+        const uint64_t each = rows * ((few * a.r + w - 1) / w), all = (uint64_t)a.tokens * a.r / w + rows;
+        const uint64_t tiles = (each < all ? each : all) * a.n_kv_heads * ((uint64_t)a.max_ctx / 32 + 1);
         c.fits = c.fits && tiles < TOO_MANY;
+        // no CTA for less than a tile per warp (1 x 512: 11.7 us, with two per warp 13.3)
         c.few_grid = grid_for(tiles, a.dtype == KVQ_F16 && c.cols <= 8 ? 12 : 8, sms);
     }
     return c;

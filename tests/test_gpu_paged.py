@@ -322,6 +322,16 @@ def test_attend_keeps_later_tokens_out(new, at, what, value):
         assert bool((~torch.isfinite(got[at:new, 4:])).any(-1).all())
 
 
+@pytest.mark.parametrize("new, r", [([4, 3, 1], 4), ([8, 7, 2], 4), ([1, 1, 1], 16), ([2, 1, 2], 16), ([6, 5, 1], 4),
+                                    ([3, 6, 1], 5), ([32, 9, 30], 1), ([8, 90, 9], 4), ([1, 50, 2], 32), ([2, 33, 1], 48)])
+@pytest.mark.parametrize("loose", [False, True])
+def test_attend_columns_per_pass(new, r, loose):
+    """Few columns in one pass or several, tiles of eight or, where the bounds
+    allow long caches, sixteen; beside chunks and alone."""
+    s = Step([200, 75, 16], new, 2, r, 128, 64, 16, F16, extra_width=60000 if loose else 0)
+    s.check(s.call(paged, max_ctx=None))
+
+
 @pytest.mark.parametrize("new", [1, 70])
 def test_attend_cuts_to_its_bounds(new):
     """Lengths past max_ctx and negative ones are cut, not followed."""
