@@ -261,6 +261,17 @@ int kvq_paged_attend(const kvq_paged_args* a, void* out, void* workspace, size_t
     if (need && (workspace == nullptr || workspace_bytes < need))
         return api_fail(KVQ_ERR_INVALID, "workspace of %zu bytes is smaller than the %zu this call needs", workspace_bytes, need);
     if (need && !aligned(workspace, 256)) return api_fail(KVQ_ERR_INVALID, "workspace is not 256-byte aligned");
+    if (p.tokens) {
+        // rows are written while others are still read
+        const size_t es = p.dtype == KVQ_F16 ? 2 : 4, n = (size_t)p.tokens * p.n_heads * p.head_dim * es;
+        const auto span = [&](uint64_t token, uint64_t heads, uint64_t head) {
+            return ((p.tokens - 1) * token + (heads - 1) * head + p.head_dim) * es;
+        };
+        if (overlap(out, n, p.q, span(p.q_token, p.n_heads, p.q_head)) ||
+            overlap(out, n, p.new_k, span(p.k_token, p.n_kv_heads, p.k_head)) ||
+            overlap(out, n, p.new_v, span(p.v_token, p.n_kv_heads, p.v_head)))
+            return api_fail(KVQ_ERR_INVALID, "out overlaps q, new_k or new_v");
+    }
     if (int rc = api_device_ok()) return rc;
     if (p.tokens == 0 || p.max_new == 0) return KVQ_OK;
     return launched(launch_attend(p, workspace, static_cast<cudaStream_t>(stream)), "paged attention");

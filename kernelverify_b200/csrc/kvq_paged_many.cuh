@@ -138,8 +138,8 @@ __device__ __forceinline__ uint64_t desc128(uint32_t saddr, uint32_t leading) {
 // byte offset of 16-byte chunk c (eight dims) of row r in a panel
 __device__ __forceinline__ uint32_t swizzled(uint32_t r, uint32_t c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
-// Every wait ends: after WAIT_CYCLES, or once another wait gave up. (Tests with a
-// time to suspend for woke up late: a part of one tile took 60 us.)
+// Every wait ends: after WAIT_CYCLES, or once another wait gave up. The rows of a
+// CTA that gave up are NaN.
 template <bool SLACK = false>
 __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, volatile int* err) {
     if (mbar_try_wait(bar, parity)) return;

@@ -68,6 +68,15 @@ def test_attend_checks_its_output_and_workspace(lib):
     assert lib.kvq_paged_attend(None, 8192, None, 0, None) == _native.KVQ_ERR_INVALID
 
 
+def test_attend_refuses_its_inputs_as_output(lib):
+    a = _attend()
+    need = lib.kvq_paged_workspace_bytes(ctypes.byref(a))
+    for name in ("q", "new_k", "new_v"):
+        b = _attend(**{name: (1 << 30) + 256})
+        assert lib.kvq_paged_attend(ctypes.byref(b), 1 << 30, 1 << 20, need, None) == _native.KVQ_ERR_INVALID
+        assert b"overlaps" in lib.kvq_last_error()
+
+
 def _tables(**over):
     t = _native.KvqTables()
     for i, (name, _) in enumerate(_native.KvqTables._fields_[:11]):
@@ -139,7 +148,7 @@ def test_no_device_is_a_status(lib):
         assert entry(ctypes.byref(a), None) == _native.KVQ_ERR_UNSUPPORTED
     a = _attend()
     need = lib.kvq_paged_workspace_bytes(ctypes.byref(a))
-    assert lib.kvq_paged_attend(ctypes.byref(a), 8192, 1 << 20, need, None) == _native.KVQ_ERR_UNSUPPORTED
+    assert lib.kvq_paged_attend(ctypes.byref(a), 1 << 30, 1 << 20, need, None) == _native.KVQ_ERR_UNSUPPORTED
 
 
 def test_python_refuses_cpu_tensors():
