@@ -32,6 +32,8 @@
 // taken before the rounding.
 #pragma once
 
+#include <cuda.h>
+
 #include <atomic>
 
 #include "kvq_paged_work.cuh"
@@ -76,9 +78,9 @@ struct Cfg {
     static constexpr int K = 2 * TILE;
     static constexpr int V = K + STAGES * TILE;
     static constexpr int BAR = V + STAGES * TILE;
-    // q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2] (M tile, buffer), then k_full,
+    // q_full[2], s_full[2][2], p_full[2][2] (M tile, buffer), o_done[2], then k_full,
     // k_empty, v_full, v_empty [STAGES] each, and the MMA warps' last ones
-    static constexpr int NBAR = 14 + 4 * STAGES + 2;
+    static constexpr int NBAR = 12 + 4 * STAGES + 2;
     static constexpr int MISC = BAR + NBAR * 8;        // TMEM address, error flag
     static constexpr int BEFORE = MISC + 16;           // uint32 [rows + 1]
     static constexpr uint32_t S0 = 0, O0 = 256;        // TMEM columns: S_i's buffer b at 128 i + 64 b, O_i at 256 + 128 i
@@ -170,6 +172,13 @@ __device__ __forceinline__ uint4 values_of(uint32_t w, __half2 s, __half2 z) {
 // 16 bytes to shared memory, or 16 zeros
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+
+// 64 dims of a head's 128 consecutive tokens, swizzled, to a panel
+__device__ __forceinline__ void load_panel(uint32_t dst, const CUtensorMap& map, uint32_t dim, uint32_t head, uint32_t token, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(&map), "r"(dim), "r"(head), "r"(token), "r"(mma4::s_addr(bar))
+                 : "memory");
 }
 
 // sum_{i=0}^{n-1} floor((a i + b) / m), by steps of Euclid's algorithm
@@ -268,14 +277,15 @@ __device__ __forceinline__ Part first_part(const Attend& a, const uint32_t* befo
 
 template <int DH, int GROUP>
 __global__ void __launch_bounds__(THREADS, 1)
-many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ ws) {
+many_kernel(Attend a, uint32_t least_new, bool vec, bool maps, unsigned char* __restrict__ ws,
+            const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using C = Cfg<DH>;
     constexpr int G = DH / GROUP, W = DH / 8;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (mma4::s_addr(smem_raw) & 1023u)) & 1023u);
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::BAR);
-    uint64_t *q_full = bar, *s_full = bar + 2, *p_full = bar + 6, *pv_done = bar + 10;
-    uint64_t *k_full = bar + 14, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES;
+    uint64_t *q_full = bar, *s_full = bar + 2, *p_full = bar + 6, *o_done = bar + 10;
+    uint64_t *k_full = bar + 12, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES;
     uint64_t* drained = v_empty + STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::MISC);
     volatile int* err = reinterpret_cast<volatile int*>(smem + C::MISC + 4);
@@ -285,9 +295,9 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 4);
+            mbar_init(&o_done[i], 1);
         }
         for (int i = 0; i < 4; ++i) {
-            mbar_init(&pv_done[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
         }
@@ -338,10 +348,6 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
         constexpr int RPW = 32 / W;
         const uint32_t r0 = (warp & 3) * 32 + lane / W, c0 = lane % W;
         uint32_t done = 0;                                           // steps
-        // step g's combine is done. A parity tells only neighbouring phases apart, and
-        // arrivals at different barriers may pass one another, so every phase of either
-        // buffer's barrier is waited for in turn (two steps behind, when it is long over).
-        const auto combined = [&](uint32_t g) { wait(&pv_done[2 * mt + (g & 1)], (g >> 1) & 1, err); };
         do {
             if (mt == 1 && !p.second) continue;
             const uint32_t tok = p.tok0 + mt * tokm + rt;           // of the request
@@ -377,34 +383,52 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                 wait(&s_full[2 * mt + buf], (done >> 1) & 1, err);
                 __syncwarp();
                 tc_fence_after();
-                uint32_t s[KS];
-                ld32(s_buf, s);
-                ld32(s_buf + 32, s + 32);
-                tmem_wait_ld();
                 // visible keys of the step: the cached ones up to the length, of the step's
                 // own those up to the row's token
                 const uint32_t tile = p.lo - p.u0 + q / 2, key = (tile < p.s.past ? tile : tile - p.s.past) * KT + (q & 1) * KS;
                 const int lim = tile < p.s.past ? (int)p.s.rq.ctx - (int)key : (int)tok - (int)key + 1;
-                if (__any_sync(0xffffffffu, lim < KS)) {
+                const bool masked = __any_sync(0xffffffffu, lim < KS);
+                uint32_t s[KS];
+                float top;
+                float2 sum[2];
+                // The weights relative to the reference there is, and the maximum beside them
+                // (in front of them it was 500 of 2,300 cycles of a step). Where it turns out
+                // too far above the reference, which is rare, the step is done once more.
+                for (;;) {
+                    ld32(s_buf, s);
+                    ld32(s_buf + 32, s + 32);
+                    tmem_wait_ld();
+                    if (masked) {
 #pragma unroll
-                    for (int c = 0; c < KS; ++c)
-                        if (c >= lim) s[c] = 0xff800000u;
-                }
-                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        for (int c = 0; c < KS; ++c)
+                            if (c >= lim) s[c] = 0xff800000u;
+                    }
+                    float tops[2] = {-INFINITY, -INFINITY};
+                    sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+                    const float sub = ref == -INFINITY ? 0.0f : ref;
+                    const float2 mul2 = make_float2(scale2, scale2), sub2 = make_float2(-sub, -sub);
 #pragma unroll
-                for (int c = 0; c < KS; c += 2)
-                    tops[c / 2 % 4] = max_nan(tops[c / 2 % 4], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-                const float top = max_nan(max_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]) * scale2;
-                if (top != top) l = NAN;               // a NaN among the scores it sees: so is the row
-                const bool over = top - ref > RAISE;
-                if (__any_sync(0xffffffffu, over)) {
+                    for (int c = 0; c < KS; c += 2) {
+                        tops[c / 2 % 2] = max_nan(tops[c / 2 % 2], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+                        float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), mul2, sub2);
+                        x.x = ex2(x.x);
+                        x.y = ex2(x.y);
+                        sum[(c >> 1) & 1] = __fadd2_rn(sum[(c >> 1) & 1], x);
+                        const __half2 h = __floats2half2_rn(x.x, x.y);
+                        s[c >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                    top = max_nan(tops[0], tops[1], tops[1]) * scale2;
+                    const bool over = top - ref > RAISE;
+                    if (!__any_sync(0xffffffffu, over)) break;
                     const float to = over ? top - START : ref;
                     // a row that has seen nothing yet has nothing to rescale
                     const float f = ref == -INFINITY ? 0.0f : ex2(ref - to);
                     ref = to;
                     l *= f;
                     if (q > 0) {
-                        combined(done - 1);
+                        // the combine in front is done: the next scores are issued behind it
+                        if (q + 1 < steps) wait(&s_full[2 * mt + (buf ^ 1)], ((done + 1) >> 1) & 1, err);
+                        else wait(&o_done[mt], 0, err);
                         __syncwarp();
                         tc_fence_after();
 #pragma unroll
@@ -418,29 +442,19 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                         }
                     }
                 }
-                const float sub = ref == -INFINITY ? 0.0f : ref;
-                const float2 mul2 = make_float2(scale2, scale2), sub2 = make_float2(-sub, -sub);
-                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-                for (int c = 0; c < KS; c += 2) {
-                    float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), mul2, sub2);
-                    x.x = ex2(x.x);
-                    x.y = ex2(x.y);
-                    sum[(c >> 1) & 1] = __fadd2_rn(sum[(c >> 1) & 1], x);
-                    const __half2 h = __floats2half2_rn(x.x, x.y);
-                    s[c >> 1] = *reinterpret_cast<const uint32_t*>(&h);
-                }
+                if (!(top < INFINITY)) l = NAN;        // a NaN or an infinity among the scores it sees: the row is NaN
                 st32(s_buf, s);
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
                 tc_fence_before();
-                if (q >= 2) combined(done - 2);
+                // the part's two phases of o_done are waited for in turn: a parity tells only
+                // neighbouring ones apart
+                if (q + 1 == steps) wait(&o_done[mt], 0, err);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[2 * mt + buf]);
             }
             // ---- the part's result ------------------------------------------------
-            combined(done - 2);
-            combined(done - 1);
+            wait(&o_done[mt], 1, err);
             __syncwarp();
             tc_fence_after();
             const bool whole = p.u0 >= start && p.u1 <= end;
@@ -505,6 +519,16 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
+        };
+        // a whole tile of own entries by one thread's tensor copies, which the phase waits for
+        const auto fetch = [&](uint64_t* bar, const CUtensorMap& map, uint32_t to, uint32_t head, uint32_t token) {
+            if (warp == 8 && lane == 0) {
+                mma4::mbar_expect_tx(bar, C::TILE);
+#pragma unroll
+                for (int i = 0; i < C::PANELS; ++i) load_panel(to + i * C::PANEL, map, 64 * i, head, token, bar);
+            } else if (lane == 0) {
+                mbar_arrive(bar);
+            }
         };
         uint32_t done = 0;
         do {
@@ -586,43 +610,29 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                         *reinterpret_cast<uint4*>(tile_at + (c >> 3) * C::PANEL + swizzled(rr, c & 7)) = *reinterpret_cast<const uint4*>(h);
                     }
                 }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            };
-            // K and V copies are groups in turn; each is handed over when the one behind it
-            // is on its way
-            uint64_t* pending = nullptr;                        // the V in flight
-            const auto settle = [&]() {
-                if (pending == nullptr) return;
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                filled(pending);
-                pending = nullptr;
             };
             for (uint32_t tile = max(t0, p.s.past); tile < p.hi - p.u0; ++tile, ++done) {
                 const uint32_t st = done % STAGES, use = done / STAGES, key0 = (tile - p.s.past) * KT;
                 unsigned char* kd = smem + C::K + st * C::TILE;
                 unsigned char* vd = smem + C::V + st * C::TILE;
                 const bool all_see = key0 + KT - 1 <= p.tok0;   // every row sees every key
-                if (!all_see) settle();
                 if (use) wait<true>(&k_empty[st], (use - 1) & 1, err);
-                copy_rows(a.new_k, a.k_token, a.k_head, key0, kd);
-                if (all_see) {
-                    if (pending != nullptr) {
-                        asm volatile("cp.async.wait_group 1;" ::: "memory");
-                        filled(pending);
-                    }
+                __syncwarp();
+                if (maps && all_see) {
+                    fetch(&k_full[st], k_map, mma4::s_addr(kd), p.hk, p.s.rq.token0 + key0);
                     if (use) wait<true>(&v_empty[st], (use - 1) & 1, err);
-                    copy_rows(a.new_v, a.v_token, a.v_head, key0, vd);
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    filled(&k_full[st]);
-                    pending = &v_full[st];
+                    __syncwarp();
+                    fetch(&v_full[st], v_map, mma4::s_addr(vd), p.hk, p.s.rq.token0 + key0);
+                    __syncwarp();
                     continue;
                 }
+                copy_rows(a.new_k, a.k_token, a.k_head, key0, kd);
                 // A weight of zero does not keep an infinite or NaN value out of the rows that
                 // are masked from it. Such a value row is taken as zeros, and its key as NaN,
                 // which reaches the rows that see it and no other.
                 if (use) wait<true>(&v_empty[st], (use - 1) & 1, err);
                 copy_rows(a.new_v, a.v_token, a.v_head, key0, vd);
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 __syncwarp();
 #pragma unroll 4
                 for (int i = 0; i < STEPS; ++i) {
@@ -640,8 +650,14 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                 filled(&k_full[st]);
                 filled(&v_full[st]);
             }
-            settle();
         } while (p.next(a, before, least_new, end));
+        // no copy of this CTA's is on its way when it leaves, whatever the waits did
+        if (maps && warp == 8)
+            for (uint32_t t = done > STAGES ? done - STAGES : 0; t < done; ++t) {
+                const long long t0 = clock64();
+                while ((!mbar_try_wait(&k_full[t % STAGES], (t / STAGES) & 1) || !mbar_try_wait(&v_full[t % STAGES], (t / STAGES) & 1)) &&
+                       clock64() - t0 < WAIT_CYCLES) {}
+            }
     } else {
         // --------------------------- the MMAs -----------------------------------------
         if (warp < 14) {
@@ -689,7 +705,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
                             const uint64_t v = desc128(base + C::V + (vt % STAGES) * C::TILE + half * (KS * 128), C::PANEL);
 #pragma unroll
                             for (int k = 0; k < KS / 16; ++k) umma_ts(o_at, s_buf + 8 * k, v + k * (2048 >> 4), ID_O, q > 2 || k > 0);
-                            umma_commit(&pv_done[2 * mt + buf]);
+                            if (q >= n) umma_commit(&o_done[mt]);          // the part's last two
                             if (half) umma_commit(&v_empty[vt % STAGES]);
                         }
                         if (q < n) {
@@ -719,6 +735,26 @@ many_kernel(Attend a, uint32_t least_new, bool vec, unsigned char* __restrict__ 
     pdl_launch_dependents();
 }
 
+// x [tokens, heads, DH] with its strides as boxes of 64 dims x 1 head x 128 tokens
+template <int DH>
+bool map_of(const Attend& a, const void* x, uint64_t token, uint64_t head, CUtensorMap* map) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found);
+        return e == cudaSuccess && found == cudaDriverEntryPointSuccess ? reinterpret_cast<Encode>(f) : nullptr;
+    }();
+    if (encode == nullptr) return false;
+    const cuuint64_t dims[3] = {DH, a.n_kv_heads, a.tokens}, strides[2] = {2 * head, 2 * token};
+    const cuuint32_t box[3] = {64, 1, KT}, steps[3] = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(x), dims, strides, box, steps,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int DH, int GROUP>
 cudaError_t launch_many(const Attend& a, uint32_t least_new, bool vec, uint32_t grid, void* ws, cudaStream_t stream) {
     using C = Cfg<DH>;
@@ -727,7 +763,12 @@ cudaError_t launch_many(const Attend& a, uint32_t least_new, bool vec, uint32_t 
     cudaError_t e = allow_smem(kernel, 1024 + C::BEFORE + (MAX_ROWS + 1) * 4, done);
     if (e != cudaSuccess) return e;
     const size_t smem = 1024 + C::BEFORE + ((size_t)a.rows + 1) * 4;
-    kernel<<<grid, THREADS, smem, stream>>>(a, least_new, vec, static_cast<unsigned char*>(ws));
+    // whole tiles of own entries come by tensor copies, where their strides allow
+    // (multiples of 16 bytes, and not 0)
+    alignas(64) CUtensorMap k_map{}, v_map{};
+    const bool maps = vec && a.k_token && a.k_head && a.v_token && a.v_head && map_of<DH>(a, a.new_k, a.k_token, a.k_head, &k_map) &&
+                      map_of<DH>(a, a.new_v, a.v_token, a.v_head, &v_map);
+    kernel<<<grid, THREADS, smem, stream>>>(a, least_new, vec, maps, static_cast<unsigned char*>(ws), k_map, v_map);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     return launch_join<__half, DH, COLS>(a, grid, static_cast<const unsigned char*>(ws), stream);

@@ -270,6 +270,28 @@ def test_attend_reads_any_stride_and_leaves_padding(new, dtype):
     assert bool((out[new + 1:] == 7.0).all())
 
 
+@pytest.mark.parametrize("layout", ["plain", "packed", "heads", "one head for all", "odd"])
+@pytest.mark.parametrize("dh, hkv, r", [(128, 2, 4), (64, 3, 1), (128, 1, 2)])
+def test_attend_long_own_entries_of_any_layout(layout, dh, hkv, r):
+    """Whole tiles of the step's own keys and values, whatever their strides,
+    behind another request's; a NaN behind the last request's tokens."""
+    s = Step([30, 0, 200], [3, 700, 390], hkv, r, dh, 64, 16, F16, pad=200, packed=layout == "packed")
+    for name in ("nk", "nv"):
+        x = getattr(s, name)
+        x[1093:] = float("nan")
+        if layout == "heads":
+            x = x.transpose(0, 1).contiguous().transpose(0, 1)
+        elif layout == "one head for all":
+            x = x[:, :1].expand(-1, hkv, -1)
+        elif layout == "odd":
+            buf = torch.zeros(x.numel() + x.shape[0] + 1, dtype=F16, device="cuda")
+            view = buf.as_strided(x.shape, (hkv * dh + 1, dh, 1), 1)
+            view.copy_(x)
+            x = view
+        setattr(s, name, x)
+    s.check(s.call(paged))
+
+
 @pytest.mark.parametrize("new", [1, 70])
 @pytest.mark.parametrize("spread", [1e-3, 0.03, 6.0])
 def test_attend_small_and_peaky_values(new, spread):
