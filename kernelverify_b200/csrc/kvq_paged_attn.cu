@@ -29,10 +29,9 @@ uint32_t grid_for(uint64_t tiles, uint64_t least, uint64_t most) {
 // A request is the few kernel's while its columns (new tokens x shared heads) fit
 // two passes of 16. 32 requests of 8192 cached positions, R = 4, n new tokens each,
 // few / many: n = 1 71 / 252, n = 4 123 / 258, n = 6 195 / 260, n = 8 227 / 262;
-// one of 131072, n = 8: 123 / 137. A third pass would lose: n = 9 346 (five of
-// eight columns: 315) / 262. 31 requests of 8192 and
-// 2 tokens each beside a chunk of 512: 112 with the few kernel, 575 as units of the
-// many kernel with 8 of 256 rows in use.
+// one of 131072, n = 8: 123 / 137. A third pass would lose: n = 9 346 (five of eight
+// columns: 315) / 262. 31 requests of 8192 and 2 tokens each beside a chunk of 512:
+// 112 with the few kernel, 575 as units of the many kernel with 8 of 256 rows in use.
 constexpr uint32_t FEW_COLS = 32;
 
 // Columns per pass. Up to four are held once per block of a tile (4 columns: 71
@@ -67,7 +66,7 @@ Choice choose(const Attend& a) {
         // units have at most 256 query rows; no CTA for less than two tiles (64 tokens
         // over 512: 21 us, with four 28, with one 21)
         const uint64_t tu = 2 * (128 / a.r), units = (uint64_t)a.n_kv_heads * (a.tokens / tu + rows);
-        const uint64_t tiles = units * (((uint64_t)a.max_ctx + a.max_new) / MANY_KEYS + 2);
+        const uint64_t tiles = units * (((uint64_t)a.max_ctx + a.max_new) / MANY_KEYS + 2 + MANY_UNIT);
         c.fits = tiles < TOO_MANY;
         c.many_grid = grid_for(tiles, 2, sms);
         const size_t es = 2;

@@ -17,15 +17,24 @@
 //         the row's maximum passed it by 2^14, P back to tensor memory; at the
 //         end O / l to the output, or the unit's part to the workspace
 //   2     loads: cached rows a thread per key, the next tile's words on their way
-//         while this one's become fp16; own entries by 16-byte asynchronous
-//         copies; all stored with the 128-byte swizzle the MMAs read
+//         while this one's become fp16; tiles of own entries that every row sees by
+//         tensor copies, the others by 16-byte asynchronous copies; all with the
+//         128-byte swizzle the MMAs read
 //   3     a warp per M tile whose elected lane issues its MMAs (one warp for both
 //         spent 2,400 cycles on a step of 64 keys, waiting and issuing in turn)
 // Each M tile has two S buffers, so that the scores of a step are there before
-// the softmax is done with the one in front. (With one buffer of 128 keys the
-// softmax of an M tile waited for its own PV and S: 4,850 cycles per 128 keys,
-// 2,830 of them softmax.) K and V tiles have the same layout, rows of keys: K is
-// read as a K-major operand, V as an MN-major one.
+// the softmax is done with the one in front. K and V tiles have the same layout,
+// rows of keys: K is read as a K-major operand, V as an MN-major one.
+//
+// 4096 tokens over 8192 cached ones, 32 heads over 8 of 128: 717 us, 960 TFLOP/s; a
+// first chunk of 8192: 596 us, 922 TFLOP/s; 64 tokens of 64 requests over 8192:
+// 930 TFLOP/s. A step of 64 keys takes 2,200 cycles for both M tiles, of which the
+// tensor pipe is busy for at least 1,024 (1,536 if, as it seems, MMAs 64 columns
+// wide take as long as those of 128: without softmax and dequantizing it comes to
+// 1,470 TFLOP/s), the special-function unit for 1,024 and each scheduler's issue
+// slot for 1,100; what is left is their waiting for one another. Half of the
+// exponentials' share on the FMA pipe, more registers for the softmax and copies
+// further ahead changed nothing.
 //
 // Rounded to fp16: the dequantized K and V (as a cache held in fp16 would be)
 // and the weights P; everything else is fp32. P is at most 2^14 and its sum is
@@ -36,6 +45,7 @@
 
 #include <atomic>
 
+#include "kvq_paged_attn.h"
 #include "kvq_paged_work.cuh"
 #include "kvq_umma.cuh"
 
@@ -201,16 +211,20 @@ __device__ __forceinline__ uint64_t floor_sum(uint32_t n, uint32_t m, uint32_t a
 }
 
 // A request's units and their key tiles. Unit i brings tokens [i tu, (i + 1)
-// tu) and needs the cached tiles and the own tiles up to its last token.
+// tu) and needs the cached tiles and the own tiles up to its last token. It counts
+// MANY_UNIT tiles more, in front of its own, for what it costs besides them (queries,
+// the masked tile, its result), so that a share of many short units is no longer
+// than one of a few long ones (a first chunk of 4096: 198 us, counted by tiles alone
+// 270).
 struct Shape {
     Request rq;
     uint32_t tu, units, past;          // tokens per unit, units per cache head, cached tiles
     __device__ __forceinline__ uint32_t tiles(uint32_t i) const { return past + (min((i + 1) * tu, rq.n) + KT - 1) / KT; }
-    // key tiles of the units in front of unit i
+    // what the units in front of unit i count
     __device__ __forceinline__ uint32_t in_front(uint32_t i) const {
         const uint32_t full = i < units ? i : units - 1;
-        const uint32_t s = full * past + (uint32_t)floor_sum(full, KT, tu, tu + KT - 1);
-        return i < units ? s : s + tiles(full);
+        const uint32_t s = full * (past + MANY_UNIT) + (uint32_t)floor_sum(full, KT, tu, tu + KT - 1);
+        return i < units ? s : s + tiles(full) + MANY_UNIT;
     }
 };
 __device__ __forceinline__ Shape shape_of(const Attend& a, uint32_t b, uint32_t least_new) {
@@ -222,7 +236,8 @@ __device__ __forceinline__ Shape shape_of(const Attend& a, uint32_t b, uint32_t 
     return s;
 }
 
-// The part [lo, hi) (in tiles of the whole step) of a unit in a CTA's share.
+// The part [lo, hi) (counted over the whole step) of a unit's tiles [u0, u1) in a
+// CTA's share.
 struct Part {
     Shape s;
     uint32_t b, hk, unit, u0, u1, lo, hi;
@@ -235,19 +250,19 @@ struct Part {
         n_tok = min(s.tu, s.rq.n - tok0);
         second = n_tok > s.tu / 2;
     }
-    // the part behind this one; false at the end of the share
+    // the part behind this one; false if the share has none
     __device__ __forceinline__ bool next(const Attend& a, const uint32_t* before, uint32_t least_new, uint32_t end) {
-        if (hi >= end) return false;
-        lo = u0 = u1;
+        if (u1 + MANY_UNIT >= end) return false;
         if (++unit == s.units) {
             unit = 0;
             if (++hk == a.n_kv_heads) {
                 hk = 0;
                 do ++b;
-                while (before[b + 1] == u0);       // requests without a unit
+                while (before[b + 1] == u1);       // requests without a unit
                 s = shape_of(a, b, least_new);
             }
         }
+        lo = u0 = u1 + MANY_UNIT;
         settle(end);
         return true;
     }
@@ -269,8 +284,8 @@ __device__ __forceinline__ Part first_part(const Attend& a, const uint32_t* befo
         else hi = mid;
     }
     p.unit = lo;
-    p.u0 = before[p.b] + p.hk * per_head + p.s.in_front(lo);
-    p.lo = at;
+    p.u0 = before[p.b] + p.hk * per_head + p.s.in_front(lo) + MANY_UNIT;
+    p.lo = max(at, p.u0);
     p.settle(end);
     return p;
 }
@@ -323,6 +338,7 @@ many_kernel(Attend a, uint32_t least_new, bool vec, bool maps, unsigned char* __
     const uint32_t start = (uint32_t)start64, end = min(total, start + share);
 
     Part p = first_part(a, before, least_new, start, end);
+    if (p.lo >= end) return;                       // none of its tiles
     if (warp == 12) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
@@ -590,7 +606,9 @@ many_kernel(Attend a, uint32_t least_new, bool vec, bool maps, unsigned char* __
                 read(kind, r, a.v, vw, vs, vz);
             }
             // ---- own entries: W lanes copy a row, a warp RPW rows at a time ---------------
-            // (A thread per row left each load of a warp in 32 lines: 18,000 cycles a tile.)
+            // (A thread per row left each load of a warp in 32 lines: 18,000 cycles a tile. All
+            // tiles so: 5,000 cycles a tile for the copies alone, 886 us for a first chunk of 8192
+            // where the tensor copies take 739.)
             constexpr int RPW = 32 / W, STEPS = KT / (4 * RPW);
             const uint32_t c = lane % W, r0 = (warp & 3) * RPW + lane / W;
             const auto copy_rows = [&](const void* base, uint64_t token, uint64_t head, uint32_t key0, unsigned char* tile_at) {
