@@ -27,11 +27,11 @@ uint32_t grid_for(uint64_t tiles, uint64_t least, uint64_t most) {
 // us on a B200 below: 8 cache heads of 128, groups of 64, a captured call.
 //
 // A request is the few kernel's while its columns (new tokens x shared heads) fit
-// two passes of 16. 32 requests of 8192 cached positions, R = 4, n new tokens each,
-// few / many: n = 1 71 / 252, n = 4 123 / 258, n = 6 195 / 260, n = 8 227 / 262;
-// one of 131072, n = 8: 123 / 137. A third pass would lose: n = 9 346 (five of eight
-// columns: 315) / 262. 31 requests of 8192 and 2 tokens each beside a chunk of 512:
-// 112 with the few kernel, 575 as units of the many kernel with 8 of 256 rows in use.
+// two passes of 16, where the two are even. 32 requests of 8192 cached positions,
+// R = 4, n new tokens each, few / many: n = 1 71 / 219, n = 4 124 / 221, n = 6
+// 195 / 223, n = 8 225 / 225, n = 9 with a third pass 346 / 225; 32 of 1024, n = 8:
+// 53 / 56; one of 131072, n = 8: 123 / 118. 31 of 8192 with two tokens each beside a
+// chunk of 512: 105 / 286 with all of them units of the many kernel.
 constexpr uint32_t FEW_COLS = 32;
 
 // Columns per pass. Up to four are held once per block of a tile (4 columns: 71
@@ -61,10 +61,11 @@ Choice choose(const Attend& a) {
         // one request: the many kernel alone (its bound is what it brings, but for a
         // padded batch), so that no second pair of launches finds nothing to do
         c.few_most = rows == 1 ? 0 : FEW_COLS / a.r;
-        // 8 columns cost a batch of single tokens 2 us of 107 and save one of pairs 14
+        // (8 for R <= 8: against 4 they cost a batch of single tokens 2 us of 107 and save
+        // one of pairs 50 of 162, beside a chunk of 512)
         c.cols = columns(a.r > 8 ? a.r : 8, row_tiles, sms);
         // units have at most 256 query rows; no CTA for less than two tiles (64 tokens
-        // over 512: 21 us, with four 28, with one 21)
+        // over 512: 21 us, as with one; with four 22, with eight 27)
         const uint64_t tu = 2 * (128 / a.r), units = (uint64_t)a.n_kv_heads * (a.tokens / tu + rows);
         const uint64_t tiles = units * (((uint64_t)a.max_ctx + a.max_new) / MANY_KEYS + 2 + MANY_UNIT);
         c.fits = tiles < TOO_MANY;
