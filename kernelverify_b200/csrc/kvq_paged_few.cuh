@@ -37,14 +37,27 @@
 // other half's weights as zeros. The two halves are two online softmaxes, joined
 // at the end.
 //
-// Precision: products exact, sums fp32. The weights are carried as PP fp16
-// parts (2: 2^-22 relative, for fp16 steps; 3 for fp32 steps), held near the
-// top of fp16's range: p is relative to a reference that the running maximum
-// may pass by 2^14 before it moves (so accumulators are rarely rescaled), and
-// vs is divided by a power of two above the largest |vs| met so far. Queries
+// Precision: products exact, sums fp32. Of a weight p vs, fp16 steps give the MMAs
+// its fp16 rounding (2^-12 relative), and what that leaves times 7.5, the middle of
+// the codes, joins the bias term: a weight's error meets c - 7.5 where it would meet
+// c. (Root mean square error of an output against 64 bits, of its magnitude, 32 x
+// 8192: 2.2e-4, of which the output's own rounding is 2.1e-4; without the second
+// term 3.0e-4 and 64.5 us; as two fp16 parts 2.1e-4 and 70.7 us.) fp32 steps carry
+// three parts. Weights are held near the top of fp16's range: p is relative to a
+// reference that the running maximum may pass by 2^14 before it moves (so
+// accumulators are rarely rescaled), and vs is divided by a power of two above the
+// largest |vs| met so far. Queries
 // are scaled by a power of two per column (fp32 ones are three fp16 parts of
 // that, and their MMAs start from zero and are added in fp32, since a long
 // chain of additions in the tensor cores truncates).
+//
+// 32 requests of 8192 positions, 32 heads over 8 of 128: 66 us, 303 MB, 0.70 of the
+// measured copy bandwidth; one of 131072: 42 us, 151 MB, 0.55. Neither memory nor a
+// pipe is full: the schedulers issue in half of the cycles, from three warps each
+// (168 registers a thread), and wait for the results of MMAs and shuffles and for
+// the integer pipe, which is busy half of the time. What does not shrink with the
+// cache is about 11 us (1 x 512): two launches, the running sums, one chain of loads
+// (length, page, rows), the join.
 #pragma once
 
 #include <atomic>
@@ -78,7 +91,7 @@ struct Cfg {
     static constexpr int W = DH / 8;                // words per row
     static constexpr int SETS = DH / 32;            // runs of four words, one per lane of a quad
     static constexpr int MT = DH / 16;              // combine's 16-dim tiles
-    static constexpr int QP = HALF ? 1 : 3, PP = HALF ? 2 : 3;
+    static constexpr int QP = HALF ? 1 : 3, PP = HALF ? 1 : 3;
     static constexpr int COLS = PAIR ? 4 : 8 * NT;
     static constexpr int NB = PAIR ? 1 : SUBS;      // blocks whose weights a lane holds
     // One CTA per SM, its warps as many as registers and shared memory allow. (Two
@@ -487,7 +500,7 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
         own_entries();
 
         // ---- the cached tiles ------------------------------------------------------
-        float vlim = pow2(vexp), vinv = pow2(-vexp);
+        float vlim = pow2(vexp), vinv = pow2(-vexp), vmid = 7.5f * vlim;
         for (; wstart + k < seg_end; ++k) {
             const uint32_t s = k % C::NST;
             asm volatile("cp.async.wait_group %0;" ::"n"(C::NST - 1) : "memory");
@@ -625,6 +638,7 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
                         vexp = ve;
                         vlim = pow2(ve);
                         vinv = pow2(-ve);
+                        vmid = 7.5f * vlim;
 #pragma unroll
                         for (int m = 0; m < C::MT; ++m)
 #pragma unroll
@@ -652,9 +666,15 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
                                 uint32_t f[PP];
-                                parts_of<PP>(p[b][nt][2 * h] * sc, p[b][nt][2 * h + 1] * sc, f);
+                                const float w0 = p[b][nt][2 * h] * sc, w1 = p[b][nt][2 * h + 1] * sc;
+                                parts_of<PP>(w0, w1, f);
 #pragma unroll
                                 for (int c = 0; c < 2; ++c) ob[nt][c][i] = fmaf(p[b][nt][2 * h + c], vz[b][h][i], ob[nt][c][i]);
+                                if constexpr (PP == 1) {
+                                    const float2 r = unpack(f[0]);
+                                    ob[nt][0][i] = fmaf(w0 - r.x, vmid, ob[nt][0][i]);
+                                    ob[nt][1][i] = fmaf(w1 - r.y, vmid, ob[nt][1][i]);
+                                }
 #pragma unroll
                                 for (int x = 0; x < PP; ++x) bf[i][nt][x][h] = movmatrix(f[x]);
                             }
