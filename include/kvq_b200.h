@@ -445,7 +445,9 @@ int kvq_paged_gather(const kvq_paged_rows* a, void* stream);
  * max_ctx bounds ctx_lens and max_new the new tokens of a request (longer ones
  * are cut to it); the launch is sized by them, so a captured step serves every
  * batch within them. Pages are read up to ctx_lens only. A page id outside
- * the pool is never dereferenced: the rows that would read it come out NaN.
+ * the pool is never dereferenced: the rows that would read it come out NaN. An
+ * infinity or NaN among the step's own entries reaches the tokens that see it
+ * (whose rows are then not finite) and no other.
  * kvq_paged_workspace_bytes is 0 for invalid arguments and for none needed.
  */
 typedef struct kvq_paged_args {

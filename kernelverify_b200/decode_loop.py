@@ -386,7 +386,8 @@ class PagedDecode:
     4-bit cache (`serving.PagedSequences`, one `PagedKVCache` per layer).
 
     `prefill(prompts)` takes a list of token lists, one per row (an empty list
-    leaves its row empty), in one ragged step; `step()` decodes a token of
+    leaves its row as it is; tokens for a row that holds a request continue it,
+    in place of its latest token), in one ragged step; `step()` decodes a token of
     every live row, eagerly or, after `capture()`, as one graph replay that
     needs nothing from the host. `release(rows)` ends requests and returns
     their pages. `tok` [B] holds each row's latest token. With `shadow` (eager
@@ -470,6 +471,8 @@ class PagedDecode:
 
     def capture(self, warmup: int = 2) -> None:
         """Capture one step; the state is what it was before."""
+        if self.shadow:
+            raise ValueError("shadow steps read lengths on the host and cannot be captured")
         torch = _torch()
         s, device = self.seqs, self.model.device
         saved = [x.clone() for x in (self.tok, s.lens, s.n_free, s.block_tables)]

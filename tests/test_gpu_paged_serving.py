@@ -80,6 +80,14 @@ def test_requests_end_and_others_take_their_pages(model):
     assert held(d) == [0, 0, 0] and int(d.seqs.n_free.item()) == 9
 
 
+def test_shadow_steps_are_not_captured(model):
+    d = dl.PagedDecode(model, 1, 64, page_size=16, shadow=True)
+    d.prefill(prompts(model, [5]))
+    with pytest.raises(ValueError, match="shadow"):
+        d.capture()
+    assert d.graph is None and held(d) == [5]
+
+
 def test_a_step_that_does_not_fit_changes_nothing(model):
     d = dl.PagedDecode(model, 2, 64, pages=4, page_size=16)
     with pytest.raises(ValueError, match="fit"):
