@@ -12,8 +12,8 @@
 // rows at most), so every CTA makes them for itself in shared memory and none
 // waits for another; each thread then finds its tokens' row by bisection. One
 // launch, and it is bound by that launch: a decode step of 32 rows reads and
-// writes under 1 KB (2.9 us a captured call), 512 rows with 71,000 tokens 0.9 MB
-// (6.4 us: the sums over the rows, a bisection and a chain of three loads a token).
+// writes under 1 KB (2.8 us a captured call), 512 rows with 71,000 tokens 0.9 MB
+// (6.1 us: the sums over the rows, a bisection and a chain of three loads a token).
 #include "kvq_paged.h"
 
 namespace kvq {
