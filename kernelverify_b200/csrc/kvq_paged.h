@@ -18,7 +18,6 @@ int api_device_ok();
 
 namespace paged {
 
-constexpr int BITS = 4;
 // Rows of a batch: each CTA of the tables and attention kernels scans the
 // whole batch's lengths into shared memory (4 bytes a row, twice).
 constexpr uint32_t MAX_ROWS = 4096;

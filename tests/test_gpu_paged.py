@@ -431,6 +431,24 @@ def test_attend_captured_step_follows_lengths():
     del graphs
 
 
+def test_attend_captured_chunk_reads_its_tensors_anew():
+    """A captured chunk with whole tiles of own entries, replayed over other
+    queries, keys and values in the same memory."""
+    s = Step([100, 20], [400, 2], 2, 4, 128, 64, 16, F16)
+    s.call(paged)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = s.call(paged)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for _ in range(2):
+        for x in (s.q, s.nk, s.nv):
+            x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+        graph.replay()
+        s.check(out)
+    del graph
+
+
 def test_attend_refusals():
     s = Step([20], [2], 2, 2, 128, 64, 16, F16)
     ok = dict(block_tables=s.tables, ctx_lens=s.ctx_t, cu_new=s.cu, max_new=2)
