@@ -26,9 +26,9 @@
 // the softmax is done with the one in front. K and V tiles have the same layout,
 // rows of keys: K is read as a K-major operand, V as an MN-major one.
 //
-// 4096 tokens over 8192 cached ones, 32 heads over 8 of 128: 717 us, 960 TFLOP/s; a
-// first chunk of 8192: 596 us, 922 TFLOP/s; 64 tokens of 64 requests over 8192:
-// 930 TFLOP/s. A step of 64 keys takes 2,200 cycles for both M tiles, of which the
+// 4096 tokens over 8192 cached ones, 32 heads over 8 of 128: 700 us, 980 TFLOP/s; a
+// first chunk of 8192: 588 us, 935 TFLOP/s; 64 tokens of 64 requests over 8192:
+// 950 TFLOP/s. A step of 64 keys takes 2,200 cycles for both M tiles, of which the
 // tensor pipe is busy for at least 1,024 (1,536 if, as it seems, MMAs 64 columns
 // wide take as long as those of 128: without softmax and dequantizing it comes to
 // 1,470 TFLOP/s), the special-function unit for 1,024 and each scheduler's issue
@@ -214,7 +214,7 @@ __device__ __forceinline__ uint64_t floor_sum(uint32_t n, uint32_t m, uint32_t a
 // tu) and needs the cached tiles and the own tiles up to its last token. It counts
 // MANY_UNIT tiles more, in front of its own, for what it costs besides them (queries,
 // the masked tile, its result), so that a share of many short units is no longer
-// than one of a few long ones (a first chunk of 8192: 596 us, counted by tiles alone
+// than one of a few long ones (a first chunk of 8192: 588 us, counted by tiles alone
 // 739).
 struct Shape {
     Request rq;
@@ -229,7 +229,7 @@ struct Shape {
     // the unit in which position x of a cache head's list lies: the root of in_front's
     // mean (a parabola in i), put right by steps that double and then by bisection, so
     // that any first guess ends at the same unit. (By bisection alone, each step of it
-    // a sum by Euclid's algorithm, a first chunk of 4096 took 197 us, so 186.)
+    // a sum by Euclid's algorithm, a first chunk of 4096 took 197 us, so 186 to 194.)
     __device__ __forceinline__ uint32_t unit_at(uint32_t x) const {
         const float a = tu * (1.0f / (2 * KT)), b = past + MANY_UNIT + 0.5f + a, y = (float)x;
         const float root = 2.0f * y / (b + sqrtf(b * b + 4.0f * a * y));
