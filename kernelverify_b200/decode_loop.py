@@ -32,6 +32,7 @@ from __future__ import annotations
 
 import argparse
 import json
+import operator
 import statistics
 import sys
 import time
@@ -499,12 +500,24 @@ class PagedDecode:
         return self.status
 
     def release(self, rows) -> None:
-        """End the requests of `rows`: their pages go back, their rows are empty."""
+        """End the requests of `rows` (row numbers, from -batch on): their pages
+        go back, their rows are empty."""
         torch = _torch()
+        ended = []
+        for row in rows:
+            # checked here: a device's index kernel ends the process's context instead
+            if isinstance(row, bool) or not hasattr(row, "__index__"):
+                raise TypeError(f"{row!r} is not a row number")
+            row = operator.index(row)
+            if not -self.batch <= row < self.batch:
+                raise ValueError(f"row {row} of a batch of {self.batch}")
+            ended.append(row % self.batch)
+        went = torch.zeros(self.batch, dtype=torch.bool)
+        went[ended] = True
+        went = went.to(self.model.device)
         keep = torch.full((self.batch,), 2 ** 31 - 1, dtype=torch.int32, device=self.model.device)
-        keep[list(rows)] = 0
-        self.seqs.truncate(keep)
-        self.live[list(rows)] = 0
+        self.seqs.truncate(keep.masked_fill_(went, 0))
+        self.live.masked_fill_(went, 0)
 
 
 def paged_run(model: Decoder, lengths, steps: int, page_size: int = 64, seed: int = 0) -> dict:
