@@ -32,7 +32,6 @@ from __future__ import annotations
 
 import argparse
 import json
-import operator
 import statistics
 import sys
 import time
@@ -40,7 +39,8 @@ from dataclasses import dataclass
 
 from kernelverify_b200.pack import kv_attention as kva
 from kernelverify_b200.serving import (DecodeRouter, FullPrecisionKVCache, PagedKVCache,
-                                       PagedSequences, QuantizedKVCache, stock_paged_attention)
+                                       PagedSequences, QuantizedKVCache, row_number,
+                                       stock_paged_attention)
 
 GROUP_SIZE = 64
 
@@ -503,17 +503,8 @@ class PagedDecode:
         """End the requests of `rows` (row numbers, from -batch on): their pages
         go back, their rows are empty."""
         torch = _torch()
-        ended = []
-        for row in rows:
-            # checked here: a device's index kernel ends the process's context instead
-            if isinstance(row, bool) or not hasattr(row, "__index__"):
-                raise TypeError(f"{row!r} is not a row number")
-            row = operator.index(row)
-            if not -self.batch <= row < self.batch:
-                raise ValueError(f"row {row} of a batch of {self.batch}")
-            ended.append(row % self.batch)
         went = torch.zeros(self.batch, dtype=torch.bool)
-        went[ended] = True
+        went[[row_number(row, self.batch) for row in rows]] = True
         went = went.to(self.model.device)
         keep = torch.full((self.batch,), 2 ** 31 - 1, dtype=torch.int32, device=self.model.device)
         self.seqs.truncate(keep.masked_fill_(went, 0))

@@ -36,6 +36,7 @@ arm: an fp16 cache and the same torch attention.
 from __future__ import annotations
 
 import math
+import operator
 from dataclasses import dataclass, field
 
 from kernelverify_b200.pack import kv_attention as kva
@@ -144,6 +145,22 @@ class QuantizedKVCache:
         return deq(self.keys), deq(self.values)
 
 
+# Indexes of device tensors are checked on the host: one out of range is an
+# assertion of the device's index kernel, which ends the process's context.
+def whole_number(name: str, value) -> int:
+    if isinstance(value, bool) or not hasattr(value, "__index__"):
+        raise TypeError(f"{name} {value!r} is not a whole number")
+    return operator.index(value)
+
+
+def row_number(row, batch: int) -> int:
+    """`row` of a batch (from -batch on, as an index) as 0 .. batch - 1."""
+    row = whole_number("row", row)
+    if not -batch <= row < batch:
+        raise ValueError(f"row {row} of a batch of {batch}")
+    return row % batch
+
+
 class PagedSequences:
     """The requests of a continuous batch and the pages they hold, one for all
     layers: `lens` int32 [B], `block_tables` int32 [B, W], the stack
@@ -234,9 +251,13 @@ class PagedKVCache:
 
     def dequantized(self, row: int, length: int):
         """(K, V) [length, HKV, DH] in the cache dtype: request `row`'s first
-        positions, read back (what the stock composition attends over)."""
+        positions, read back (what the stock composition attends over); zeros
+        where its table has no page yet."""
         torch = _torch()
         s = self.sequences
+        row, length = row_number(row, s.batch), whole_number("length", length)
+        if not 0 <= length <= s.width * s.page_size:
+            raise ValueError(f"length {length}: a row holds 0 to {s.width * s.page_size} positions")
         pos = torch.arange(length, device=s.lens.device)
         slots = s.block_tables[row, pos // s.page_size].long() * s.page_size + pos % s.page_size
         return paged.gather(*self.keys, *self.values, slots)

@@ -62,3 +62,21 @@ def test_release_ends_requests(decode, model, rows, lens):
     d.release(rows)
     assert d.seqs.lens.tolist() == lens and d.live.tolist() == [int(n > 0) for n in lens]
     assert d.seqs.n_free.item() == d.seqs.pages - sum(-(-n // 16) for n in lens)
+
+
+@pytest.mark.parametrize("row, length", [(0, 65), (0, 2 ** 31), (3, 5), (-4, 5), (0, -1), (True, 5), (0, 5.0)])
+def test_read_back_checks_row_and_length(decode, model, row, length):
+    """A length past the row's table is not an index of the table."""
+    d = decode()
+    d.prefill(prompts(model, [5, 9, 20]))
+    with pytest.raises((ValueError, TypeError), match="row|length"):
+        d.caches[0].dequantized(row, length)
+
+
+def test_read_back_to_the_end_of_a_row(decode, model):
+    d = decode()
+    d.prefill(prompts(model, [64, 9, 20]))
+    k, v = d.caches[1].dequantized(0, 64)
+    assert k.shape == v.shape == (64, 2, 64) and bool((k.abs().amax((1, 2)) > 0).all())
+    assert torch.equal(d.caches[1].dequantized(-3, 10)[0], k[:10])
+    assert d.caches[0].dequantized(2, 0)[0].shape == (0, 2, 64)
