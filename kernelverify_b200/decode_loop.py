@@ -441,7 +441,11 @@ class PagedDecode:
         if total == 0:
             return
         device = self.model.device
-        tokens = torch.tensor([t for p in prompts for t in p], dtype=torch.long, device=device)
+        tokens = torch.tensor([t for p in prompts for t in p], dtype=torch.long)
+        least, most = (int(x) for x in tokens.aminmax())
+        if least < 0 or most >= self.model.shape.vocab:
+            raise ValueError(f"token {least if least < 0 else most} of a vocabulary of {self.model.shape.vocab}")
+        tokens = tokens.to(device)
         new_lens = torch.tensor(new, dtype=torch.int32, device=device)
         with torch.inference_mode():
             batch = self.seqs.begin(new_lens, total)

@@ -80,3 +80,16 @@ def test_read_back_to_the_end_of_a_row(decode, model):
     assert k.shape == v.shape == (64, 2, 64) and bool((k.abs().amax((1, 2)) > 0).all())
     assert torch.equal(d.caches[1].dequantized(-3, 10)[0], k[:10])
     assert d.caches[0].dequantized(2, 0)[0].shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("token", [1024, -1, 2 ** 40])
+def test_prefill_checks_its_tokens(decode, model, token):
+    """A token outside the vocabulary is not an index of the embedding."""
+    d = decode()
+    d.prefill(prompts(model, [5, 0, 20]))
+    before = state(d)
+    with pytest.raises(ValueError, match="token"):
+        d.prefill([[], [3, token, 4], [1]])
+    assert all(torch.equal(x, y) for x, y in zip(before, state(d)))
+    d.prefill([[], [0, 1023], torch.tensor([5, 6])])
+    assert d.seqs.lens.tolist() == [5, 2, 22]
