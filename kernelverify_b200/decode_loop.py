@@ -421,8 +421,8 @@ class PagedDecode:
             cache = self.caches[i]
             cache.append(k, v, batch)
             out = cache.attend(q, k, v, batch, max_new, workspace=self.workspace)
-            if self.shadow:
-                new = batch.cu_new.diff().tolist()
+            new = batch.cu_new.diff().tolist() if self.shadow else []
+            if sum(new):                     # a step that did not fit has no rows to compare
                 ref = stock_paged_attention(q, k, v, cache, self.seqs.lens.tolist(), new)[:sum(new)]
                 gap = (out[:sum(new)].float() - ref.float()).abs().max()
                 self.shadow_gap = max(self.shadow_gap, float(gap))

@@ -93,3 +93,16 @@ def test_prefill_checks_its_tokens(decode, model, token):
     assert all(torch.equal(x, y) for x, y in zip(before, state(d)))
     d.prefill([[], [0, 1023], torch.tensor([5, 6])])
     assert d.seqs.lens.tolist() == [5, 2, 22]
+
+
+def test_compared_steps_that_decode_nothing(decode, model):
+    """With every attention compared: a step that does not fit, and one without
+    a live row, return their status and change nothing."""
+    d = decode(batch=2, pages=4, shadow=True)
+    d.prefill(prompts(model, [32, 32]))
+    before = state(d)
+    assert d.step().item() == 1
+    assert all(torch.equal(x, y) for x, y in zip(before, state(d)))
+    d.release([0, 1])
+    assert d.step().item() == 0
+    assert d.seqs.lens.tolist() == [0, 0] and d.seqs.n_free.item() == 4
