@@ -642,6 +642,8 @@ def main(argv=None) -> int:
     ap.add_argument("--rounds", type=int, default=None)
     ap.add_argument("--steps", type=int, default=64, help="decode steps per round (--ab-graph)")
     args = ap.parse_args(argv)
+    if args.paged and not (args.prompt and min(args.prompt) >= 1):
+        ap.error("--paged needs one --prompt length or more, each at least 1")
     model = Decoder(TINY if args.tiny else QWEN3_4B)
     if args.smoke:
         report = smoke(model)

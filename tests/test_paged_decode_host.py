@@ -106,3 +106,11 @@ def test_compared_steps_that_decode_nothing(decode, model):
     d.release([0, 1])
     assert d.step().item() == 0
     assert d.seqs.lens.tolist() == [0, 0] and d.seqs.n_free.item() == 4
+
+
+@pytest.mark.parametrize("lengths", [[], ["0", "5"], ["-3"]])
+def test_the_command_checks_its_prompts(monkeypatch, capsys, lengths):
+    monkeypatch.setattr(dl, "Decoder", None)                 # refused before a model is made
+    with pytest.raises(SystemExit):
+        dl.main(["--paged", "--tiny", "--prompt", *lengths])
+    assert "--prompt" in capsys.readouterr().err
