@@ -382,8 +382,9 @@ typedef struct kvq_packed {
  * cu_new, slots, positions and status are not used. The rows' table entries
  * are left as they are.
  *
- * Inputs are read while outputs are written: an output that overlaps lens,
- * step or n_free is refused.
+ * Inputs are read while outputs are written: an array that the call writes
+ * (kvq_paged_tables block_tables too, kvq_paged_truncate free_pages) and that
+ * overlaps another one of the call is refused.
  */
 typedef struct kvq_tables {
     const int32_t* lens;      /* [rows]                                        */

@@ -80,20 +80,26 @@ int check_tables(const kvq_tables* a, bool build) {
                          a->cu_new, a->positions, a->status};
     for (const void* p : in4)
         if (p && !aligned(p, 4)) return api_fail(KVQ_ERR_INVALID, "a pointer is not 4-byte aligned");
-    const size_t rb = 4ull * a->rows;
-    // every CTA reads the lengths while the first one writes the new ones
-    const struct { const void* p; size_t n; } outs[] = {{a->lens_out, rb}, {a->n_free_out, 4}, {a->cu_new, build ? rb + 4 : 0},
-                                                        {a->status, build ? 4u : 0u}};
-    const struct { const void* p; size_t n; } ins[] = {{a->lens, rb}, {a->step, rb}, {a->n_free, 4}};
-    for (const auto& o : outs)
-        for (const auto& i : ins)
-            if (o.n && overlap(o.p, o.n, i.p, i.n))
-                return api_fail(KVQ_ERR_INVALID, "an output overlaps the lengths, the step or the free count it is computed from");
-    if (!build) return KVQ_OK;
-    if (!a->cu_new || !a->status || (a->max_tokens && (!a->slots || !a->positions)))
-        return api_fail(KVQ_ERR_INVALID, "a required pointer is NULL");
-    if (!aligned(a->slots, 8)) return api_fail(KVQ_ERR_INVALID, "slots must be 8-byte aligned");
-    if (a->max_tokens > 0x7FFFFFFFu) return api_fail(KVQ_ERR_INVALID, "max_tokens %u above 2^31 - 1", a->max_tokens);
+    if (build) {
+        if (!a->cu_new || !a->status || (a->max_tokens && (!a->slots || !a->positions)))
+            return api_fail(KVQ_ERR_INVALID, "a required pointer is NULL");
+        if (!aligned(a->slots, 8)) return api_fail(KVQ_ERR_INVALID, "slots must be 8-byte aligned");
+        if (a->max_tokens > 0x7FFFFFFFu) return api_fail(KVQ_ERR_INVALID, "max_tokens %u above 2^31 - 1", a->max_tokens);
+    }
+    // Every CTA reads the lengths, the tables and the stack, and again for each token,
+    // while others write: nothing that is written may lie over anything else.
+    const size_t rb = 4ull * a->rows, tokens = build ? a->max_tokens : 0;
+    const struct { const void* p; size_t n; bool written; } spans[] = {
+        {a->lens, rb, false}, {a->step, rb, false}, {a->n_free, 4, false},
+        {a->block_tables, rb * a->width, build}, {a->free_pages, 4ull * a->pool, !build},
+        {a->lens_out, rb, true}, {a->n_free_out, 4, true}, {a->cu_new, build ? rb + 4 : 0, true},
+        {a->status, build ? 4u : 0u, true}, {a->slots, 8 * tokens, true}, {a->positions, 4 * tokens, true}};
+    constexpr int N = sizeof spans / sizeof *spans;
+    for (int i = 0; i < N; ++i)
+        for (int j = 0; j < i; ++j)
+            if ((spans[i].written || spans[j].written) && spans[i].n && spans[j].n &&
+                overlap(spans[i].p, spans[i].n, spans[j].p, spans[j].n))
+                return api_fail(KVQ_ERR_INVALID, "an output overlaps an input or another output");
     return KVQ_OK;
 }
 
