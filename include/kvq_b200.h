@@ -440,8 +440,8 @@ int kvq_paged_gather(const kvq_paged_rows* a, void* stream);
  * before the step (dequantized from the pages) and the step's own keys and
  * values 0..i of the request at full precision -- for one new token, the step
  * of kvq_decode. out [tokens, n_heads, head_dim] dtype, contiguous. Rows of
- * `out` behind the last request's tokens are left as they were. An `out` that
- * overlaps q, new_k or new_v is refused.
+ * `out` behind the last request's tokens are left as they were. An `out` or a
+ * workspace that overlaps an input, or the other, is refused.
  *
  * max_ctx bounds ctx_lens and max_new the new tokens of a request (longer ones
  * are cut to it); the launch is sized by them, so a captured step serves every

@@ -268,15 +268,24 @@ int kvq_paged_attend(const kvq_paged_args* a, void* out, void* workspace, size_t
         return api_fail(KVQ_ERR_INVALID, "workspace of %zu bytes is smaller than the %zu this call needs", workspace_bytes, need);
     if (need && !aligned(workspace, 256)) return api_fail(KVQ_ERR_INVALID, "workspace is not 256-byte aligned");
     if (p.tokens) {
-        // rows are written while others are still read
+        // rows and parts are written while others are still read, the lengths and offsets
+        // that the reads follow among them
         const size_t es = p.dtype == KVQ_F16 ? 2 : 4, n = (size_t)p.tokens * p.n_heads * p.head_dim * es;
         const auto span = [&](uint64_t token, uint64_t heads, uint64_t head) {
             return ((p.tokens - 1) * token + (heads - 1) * head + p.head_dim) * es;
         };
-        if (overlap(out, n, p.q, span(p.q_token, p.n_heads, p.q_head)) ||
-            overlap(out, n, p.new_k, span(p.k_token, p.n_kv_heads, p.k_head)) ||
-            overlap(out, n, p.new_v, span(p.v_token, p.n_kv_heads, p.v_head)))
-            return api_fail(KVQ_ERR_INVALID, "out overlaps q, new_k or new_v");
+        const size_t held = ((size_t)p.pages * p.n_kv_heads << p.page_shift), words = held * p.head_dim / 2,
+                     scales = held * (p.head_dim / p.group) * es;
+        const struct { const void* p; size_t n; } ins[] = {
+            {p.q, span(p.q_token, p.n_heads, p.q_head)}, {p.new_k, span(p.k_token, p.n_kv_heads, p.k_head)},
+            {p.new_v, span(p.v_token, p.n_kv_heads, p.v_head)}, {p.k.words, words}, {p.k.scales, scales},
+            {p.k.biases, scales}, {p.v.words, words}, {p.v.scales, scales}, {p.v.biases, scales},
+            {p.block_tables, 4ull * p.rows * p.width}, {p.ctx_lens, 4ull * p.rows}, {p.cu_new, 4ull * p.rows + 4}};
+        for (const auto& i : ins) {
+            if (overlap(out, n, i.p, i.n)) return api_fail(KVQ_ERR_INVALID, "out overlaps an input");
+            if (need && overlap(workspace, need, i.p, i.n)) return api_fail(KVQ_ERR_INVALID, "the workspace overlaps an input");
+        }
+        if (need && overlap(workspace, need, out, n)) return api_fail(KVQ_ERR_INVALID, "the workspace overlaps out");
     }
     if (int rc = api_device_ok()) return rc;
     if (p.tokens == 0 || p.max_new == 0) return KVQ_OK;

@@ -325,7 +325,7 @@ def attend(q, k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, new_k, new_v, 
     `max_new` bounds a request's new tokens and `max_ctx` (default: W pages)
     its cached positions; the launch is sized by them and longer requests are
     cut to them. Rows of `out` past the last request's tokens are not written;
-    an `out` that overlaps q, new_k or new_v is refused.
+    an `out` that overlaps an input is refused.
     A page id outside the pool makes the rows that need it NaN."""
     torch = _torch()
     device, dtype, pages, heads, page, head_dim, group, pool = _pools(
