@@ -414,7 +414,9 @@ int kvq_paged_truncate(const kvq_tables* a, void* stream);
  * slots' values scale * code + bias into keys and values (contiguous,
  * out_dtype: the cache's dtype or KVQ_F32). A slot below 0 or past the pool is
  * not written, and reads as zeros. Two tokens of one append must not name the
- * same slot (the row would hold a mixture of both).
+ * same slot (the row would hold a mixture of both). An array that the call
+ * writes (append the pools, gather keys and values) and that overlaps another
+ * one of the call is refused.
  */
 typedef struct kvq_paged_rows {
     kvq_packed k, v;

@@ -167,6 +167,29 @@ int rows_of(const kvq_paged_rows* a, bool append, Rows* r) {
     return KVQ_OK;
 }
 
+// What the call writes may lie over nothing else of it: a row would hold a mixture of
+// two, or be read after it was written.
+int check_rows_apart(const kvq_paged_rows* a, bool append) {
+    const size_t es = a->dtype == KVQ_F16 ? 2 : 4, oes = a->out_dtype == KVQ_F16 ? 2 : 4;
+    const size_t held = (size_t)a->pages * a->n_kv_heads * a->page_size, words = held * a->head_dim / 2,
+                 scales = held * (a->head_dim / a->group_size) * es;
+    const auto rows = [&](uint64_t token, uint64_t head) -> size_t {
+        if (!append) return (size_t)a->tokens * a->n_kv_heads * a->head_dim * oes;
+        return ((a->tokens - 1) * token + (a->n_kv_heads - 1) * head + a->head_dim) * es;
+    };
+    const struct { const void* p; size_t n; bool written; } spans[] = {
+        {a->k.words, words, append}, {a->k.scales, scales, append}, {a->k.biases, scales, append},
+        {a->v.words, words, append}, {a->v.scales, scales, append}, {a->v.biases, scales, append},
+        {a->keys, rows(a->k_token_stride, a->k_head_stride), !append},
+        {a->values, rows(a->v_token_stride, a->v_head_stride), !append}, {a->slots, 8ull * a->tokens, false}};
+    constexpr int N = sizeof spans / sizeof *spans;
+    for (int i = 0; i < N; ++i)
+        for (int j = 0; j < i; ++j)
+            if ((spans[i].written || spans[j].written) && overlap(spans[i].p, spans[i].n, spans[j].p, spans[j].n))
+                return api_fail(KVQ_ERR_INVALID, "an array that is written overlaps another one of the call");
+    return KVQ_OK;
+}
+
 int attend_of(const kvq_paged_args* a, Attend* p) {
     if (!a) return api_fail(KVQ_ERR_INVALID, "args is NULL");
     if (int rc = check_cache(a->head_dim, a->group_size, a->dtype, a->pages, a->page_size, a->n_kv_heads)) return rc;
@@ -241,6 +264,7 @@ int kvq_paged_append(const kvq_paged_rows* a, void* stream) {
     if (int rc = rows_of(a, true, &r)) return rc;
     if (int rc = api_device_ok()) return rc;
     if (r.tokens == 0) return KVQ_OK;
+    if (int rc = check_rows_apart(a, true)) return rc;
     return launched(launch_append(r, static_cast<cudaStream_t>(stream)), "paged append");
 }
 
@@ -249,6 +273,7 @@ int kvq_paged_gather(const kvq_paged_rows* a, void* stream) {
     if (int rc = rows_of(a, false, &r)) return rc;
     if (int rc = api_device_ok()) return rc;
     if (r.tokens == 0) return KVQ_OK;
+    if (int rc = check_rows_apart(a, false)) return rc;
     return launched(launch_gather(r, static_cast<cudaStream_t>(stream)), "paged gather");
 }
 
