@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from kernelverify_b200.pack import kv_attention as kva
 from kernelverify_b200.pack import paged
 
 pytestmark = pytest.mark.gpu
@@ -36,3 +37,49 @@ def test_append_refuses_arrays_over_one_another():
     assert all(torch.equal(a, b) for a, b in zip(k, v))
     got = paged.gather(*k, *k, slots)                  # and one pool may be read twice
     assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("dh, group", [(64, 32), (128, 64), (128, 128)])
+def test_append_of_what_is_not_finite(dtype, dh, group):
+    """NaN and infinities, and in float32 groups whose range is infinite: the bits
+    of the other quantizer."""
+    top = torch.finfo(dtype).max
+    inf, nan = float("inf"), float("nan")
+    rows = torch.randn(16, 1, dh)
+    for i, values in enumerate(([nan], [inf], [-inf], [inf, -inf], [nan, inf], [nan, -inf], [nan] * dh, [inf] * dh,
+                                [-inf] * dh, [top, -top], [-top, top / 2], [top], [-top], [0.0, -0.0] * (dh // 2),
+                                [torch.finfo(dtype).tiny], [1e-7, -1e-7, nan])):
+        rows[i, 0, :len(values)] = torch.tensor(values)
+    x = rows.to(dtype).cuda()
+    k, v = pool(1, 1, 16, dh, group, dtype), pool(1, 1, 16, dh, group, dtype)
+    slots = torch.arange(16, device="cuda")
+    paged.append(x, x.neg(), *k, *v, slots)
+    for got, values in ((k, x), (v, x.neg())):
+        words, scales, biases = kva.quantize_cache(values.transpose(0, 1).contiguous(), bits=4, group_size=group)
+        assert torch.equal(got[0][0].view(torch.int32), words.view(torch.int32))
+        for a, b in ((got[1][0], scales), (got[2][0], biases)):
+            assert torch.equal(a.isnan(), b.isnan())
+            assert torch.equal(a.nan_to_num(0.0, inf, -inf), b.nan_to_num(0.0, inf, -inf))
+
+
+@pytest.mark.parametrize("rows, cut, room", [(3, 4, 5), (3, 4, 12), (3, 4, 0), (40, 7, 100)])
+def test_truncate_into_a_stack_without_room(rows, cut, room):
+    """What does not fit on the stack is dropped; nothing behind it is written."""
+    page, held = 16, cut + 2
+    tables = torch.arange(rows * held, dtype=torch.int32, device="cuda").view(rows, held)
+    lens = torch.full((rows,), held * page - 3, dtype=torch.int32, device="cuda")
+    keep = torch.full((rows,), 2 * page, dtype=torch.int32, device="cuda")
+    stack = 6
+    buf = torch.full((stack + room + 50,), -9, dtype=torch.int32, device="cuda")
+    free, n_free = buf[:stack + room], torch.tensor([stack], dtype=torch.int32, device="cuda")
+    out = torch.full((rows,), -1, dtype=torch.int32, device="cuda"), torch.full((1,), -1, dtype=torch.int32, device="cuda")
+    got = paged.truncate(lens, keep, tables, free, n_free, page_size=page, out=out)
+    assert got[0] is out[0] and got[1] is out[1]
+    back = tables[:, 2:].flatten().tolist()[:room]
+    assert out[0].tolist() == [2 * page] * rows and out[1].item() == stack + len(back)
+    assert buf.tolist() == [-9] * stack + back + [-9] * (buf.numel() - stack - len(back))
+    with pytest.raises(ValueError, match="out"):
+        paged.truncate(lens, keep, tables, free, n_free, page_size=page, out=(out[0][:-1], out[1]))
+    with pytest.raises(ValueError, match="out"):
+        paged.truncate(lens, keep, tables, free, n_free, page_size=page, out=(out[0].long(), out[1]))
