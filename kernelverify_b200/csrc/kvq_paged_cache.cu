@@ -179,8 +179,9 @@ __global__ void __launch_bounds__(THREADS) gather_kernel(Rows r) {
         const uint2 two = reinterpret_cast<const uint2*>(p.words)[(uint64_t)row * lanes + lane];
         const float s = to_f32(static_cast<const T*>(p.scales)[g]);
         const float b = to_f32(static_cast<const T*>(p.biases)[g]);
-        // codes i and i + 4 as fp16 1024 + c (even i) or 1024 + 16 c; s * c is one
-        // rounded multiply-add of that, as 1024 s and s / 16 are exact
+        // codes i and i + 4 as fp16 1024 + c (even i) or 1024 + 16 c; for fp16 scales s * c
+        // is one rounded multiply-add of that, as 1024 s and s / 16 are exact. (For fp32 ones
+        // they may be infinite or subnormal: the code first, exactly.)
         const float s16 = s * 0.0625f, m1024 = s * -1024.0f, m64 = s * -64.0f;
 #pragma unroll
         for (int j = 0; j < E / 8; ++j) {
@@ -189,8 +190,15 @@ __global__ void __launch_bounds__(THREADS) gather_kernel(Rows r) {
             for (int i = 0; i < 4; ++i) {
                 const uint32_t h = ((i & 2 ? w >> 8 : w) & (i & 1 ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;
                 const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&h));
-                const float2 m = make_float2(i & 1 ? s16 : s, i & 1 ? s16 : s), z = make_float2(i & 1 ? m64 : m1024, i & 1 ? m64 : m1024);
-                const float2 y = __fadd2_rn(__ffma2_rn(c, m, z), make_float2(b, b));
+                const auto both = [&](float odd, float even) { return i & 1 ? make_float2(odd, odd) : make_float2(even, even); };
+                float2 y;
+                if constexpr (sizeof(T) == 2) {
+                    y = __fadd2_rn(__ffma2_rn(c, both(s16, s), both(m64, m1024)), both(b, b));
+                } else {
+                    // (scalar: a packed product and sum come out as one fused operation)
+                    const float2 code = __ffma2_rn(c, both(0.0625f, 1.0f), both(-64.0f, -1024.0f));
+                    y = make_float2(__fadd_rn(__fmul_rn(code.x, s), b), __fadd_rn(__fmul_rn(code.y, s), b));
+                }
                 v[8 * j + i] = from_f32<TO>(y.x);
                 v[8 * j + i + 4] = from_f32<TO>(y.y);
             }

@@ -83,3 +83,23 @@ def test_truncate_into_a_stack_without_room(rows, cut, room):
         paged.truncate(lens, keep, tables, free, n_free, page_size=page, out=(out[0][:-1], out[1]))
     with pytest.raises(ValueError, match="out"):
         paged.truncate(lens, keep, tables, free, n_free, page_size=page, out=(out[0].long(), out[1]))
+
+
+@pytest.mark.parametrize("dh, group", [(64, 32), (128, 64)])
+@pytest.mark.parametrize("exponent", [-149, -130, -126, -122, -20, 0, 100, 114, 118, 123])
+def test_read_back_of_float32_scales_of_any_size(dh, group, exponent):
+    """scale * code + bias, a rounded product and a rounded sum, at both ends of the
+    scales' range: finite where the value is."""
+    g = torch.Generator().manual_seed(exponent + 200)
+    k = pool(2, 1, 16, dh, group, F32)
+    codes = torch.randint(0, 16, (32, dh), generator=g)
+    words = sum(codes[:, i::8].long() << (4 * i) for i in range(8))
+    words = torch.where(words >= 2 ** 31, words - 2 ** 32, words).int()
+    scales = torch.ldexp(torch.rand(32, dh // group, generator=g) + 1.0, torch.tensor(exponent))
+    scales *= torch.where(torch.rand(32, dh // group, generator=g) < 0.5, -1.0, 1.0)
+    biases = -scales * torch.randint(0, 16, (32, dh // group), generator=g)
+    for t, x in zip(k, (words, scales, biases)):
+        t.copy_(x.view(t.shape))
+    want = (codes.float() * scales.repeat_interleave(group, 1)) + biases.repeat_interleave(group, 1)
+    got, _ = paged.gather(*k, *k, torch.arange(32, device="cuda"))
+    assert torch.equal(got.cpu().view(32, dh), want)
