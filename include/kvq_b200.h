@@ -448,9 +448,14 @@ int kvq_paged_gather(const kvq_paged_rows* a, void* stream);
  * max_ctx bounds ctx_lens and max_new the new tokens of a request (longer ones
  * are cut to it); the launch is sized by them, so a captured step serves every
  * batch within them. Pages are read up to ctx_lens only. A page id outside
- * the pool is never dereferenced: the rows that would read it come out NaN. An
- * infinity or NaN among the step's own entries reaches the tokens that see it
- * (whose rows are then not finite) and no other.
+ * the pool is never dereferenced: the rows that would read it come out NaN.
+ *
+ * What is not finite among the step's own entries reaches the tokens that see
+ * it and no other. A NaN, or an infinite value, makes their rows not finite. An
+ * infinite key is a score of +inf (the row is then not finite) or of -inf (the
+ * entry has no weight, the row is as without it), as the query's sign has it.
+ * float32 steps serve queries, keys, values, scales and biases of magnitudes
+ * below 2^60; rows that larger finite ones enter may come out not finite.
  * kvq_paged_workspace_bytes is 0 for invalid arguments and for none needed.
  */
 typedef struct kvq_paged_args {

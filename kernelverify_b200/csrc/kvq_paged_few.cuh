@@ -221,7 +221,8 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
     constexpr bool HALF = C::HALF;
     constexpr float UNIT = HALF ? 16777216.0f : 1.0f;      // a code in an MMA is c / UNIT, or 16 c / UNIT
     // exponents of the power of two above |vs|: from below what the quantizer
-    // stores (its smallest step is 1e-7) to the type's largest
+    // stores (its smallest step is 1e-7) to fp16's largest; fp32 values are below 2^60
+    // (own entries come in at the lowest one: 16 v 2^30 times weights of up to 2^14)
     constexpr int VEXP0 = HALF ? -14 : -30, VEXP1 = HALF ? 16 : 90;
     // the join's CTAs may come as soon as there is room: none before these CTAs,
     // which hold a whole SM's registers each, have left

@@ -326,7 +326,10 @@ def attend(q, k_wq, k_scales, k_biases, v_wq, v_scales, v_biases, new_k, new_v, 
     its cached positions; the launch is sized by them and longer requests are
     cut to them. Rows of `out` past the last request's tokens are not written;
     an `out` that overlaps an input is refused.
-    A page id outside the pool makes the rows that need it NaN."""
+    A page id outside the pool makes the rows that need it NaN. An own entry that
+    is not finite reaches the tokens that see it alone: a key's infinity as a score
+    of +inf (a row that is not finite) or -inf (as without the entry). Float32
+    inputs are of magnitudes below 2^60."""
     torch = _torch()
     device, dtype, pages, heads, page, head_dim, group, pool = _pools(
         k_wq, k_scales, k_biases, v_wq, v_scales, v_biases)
