@@ -191,23 +191,27 @@ __device__ __forceinline__ void load_panel(uint32_t dst, const CUtensorMap& map,
                  : "memory");
 }
 
-// sum_{i=0}^{n-1} floor((a i + b) / m), by steps of Euclid's algorithm
-__device__ __forceinline__ uint64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
-    uint64_t s = 0;
-    while (n > 0) {
-        const uint32_t qa = a / m, qb = b / m;
-        s += (uint64_t)n * (n - 1) / 2 * qa + (uint64_t)n * qb;
-        a -= qa * m;
-        b -= qb * m;
-        const uint64_t y = (uint64_t)a * n + b;
-        if (y < m) break;
-        n = (uint32_t)y / m;                // y < 2^31: a < m <= 128, and at most 2^23 units
-        b = (uint32_t)y - n * m;
-        const uint32_t t = a;
-        a = m;
-        m = t;
+// sum_{i=1}^{n} ceil(i t / m) modulo 2^32, for n t < 2^32: lattice points under a line,
+// counted by columns, then by rows, and so on, the slope being turned over each time as
+// in Euclid's algorithm. With t < m (whole slopes are triangles, n (n + 1) / 2 points),
+//   sum_{i=1}^{n} ceil(i t / m)  = n J - sum_{j=1}^{J-1} floor(j m / t),   J = ceil(n t / m):
+//     row j < J has the i with i t > j m, which are n - floor(j m / t) many;
+//   sum_{j=1}^{n} floor(j t / m) = (n + 1) K - sum_{k=1}^{K} ceil(k m / t),   K = floor(n t / m):
+//     row k <= K has the j with j t >= k m, which are n + 1 - ceil(k m / t) many.
+__device__ __forceinline__ uint32_t ceil_sum(uint32_t n, uint32_t t, uint32_t m) {
+    uint32_t points = 0, sign = 1;
+    for (bool up = true; n > 0; up = !up) {
+        const uint32_t slope = t / m, rest = t - slope * m;
+        points += sign * slope * (n & 1 ? (n + 1) / 2 * n : n / 2 * (n + 1));
+        if (rest == 0) break;
+        const uint32_t height = (n * rest + (up ? m - 1 : 0)) / m;
+        points += sign * height * (up ? n : n + 1);
+        n = up ? height - 1 : height;
+        t = m;
+        m = rest;
+        sign = 0u - sign;
     }
-    return s;
+    return points;
 }
 
 // A request's units and their key tiles. Unit i brings tokens [i tu, (i + 1)
@@ -223,7 +227,7 @@ struct Shape {
     // what the units in front of unit i count
     __device__ __forceinline__ uint32_t in_front(uint32_t i) const {
         const uint32_t full = i < units ? i : units - 1;
-        const uint32_t s = full * (past + MANY_UNIT) + (uint32_t)floor_sum(full, KT, tu, tu + KT - 1);
+        const uint32_t s = full * (past + MANY_UNIT) + ceil_sum(full, tu, KT);
         return i < units ? s : s + tiles(full) + MANY_UNIT;
     }
     // the unit in which position x of a cache head's list lies: the root of in_front's
