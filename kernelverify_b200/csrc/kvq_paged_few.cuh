@@ -37,12 +37,15 @@
 // other half's weights as zeros. The two halves are two online softmaxes, joined
 // at the end.
 //
-// Precision: products exact, sums fp32. Of a weight p vs, fp16 steps give the MMAs
-// its fp16 rounding (2^-12 relative), and what that leaves times 7.5, the middle of
-// the codes, joins the bias term: a weight's error meets c - 7.5 where it would meet
-// c. (Root mean square error of an output against 64 bits, of its magnitude, 32 x
-// 8192: 2.2e-4, of which the output's own rounding is 2.1e-4; without the second
-// term 3.0e-4 and 64.5 us; as two fp16 parts 2.1e-4 and 70.7 us.) fp32 steps carry
+// Precision: products exact, sums fp32. Weights p vs of requests with up to SHORT
+// cached positions go to the MMAs as two fp16 parts (2^-22 relative), those of longer
+// ones as their fp16 rounding (2^-11 at most), and what that leaves times 7.5, the middle
+// of the codes, joins the bias term: a weight's error meets c - 7.5 where it would meet
+// c. (Root mean square error of an output against 64 bits, over that of its own
+// rounding, 2.1e-4 of its magnitude; one part: 1.43 at 4 cached positions, 1.24 at 32, 1.07
+// at 128, 1.04 at 256, 1.01 at 1024, 1.004 at 8192: fewer positions average less, as do
+// more of them where the softmax rests on few; two parts: 1.000. They cost 12.5 us for
+// 12.4 at 32 x 128, 37.4 for 36.2 at 256 x 256, and 70.7 for 66 at 32 x 8192.) fp32 steps carry
 // three parts. Weights are held near the top of fp16's range: p is relative to a
 // reference that the running maximum may pass by 2^14 before it moves (so
 // accumulators are rarely rescaled), and vs is divided by a power of two above the
@@ -75,6 +78,7 @@ using mma4::mma_f16;
 constexpr int BLK = 16, SUBS = 2;          // positions per block, blocks per tile
 constexpr int TP = BLK * SUBS;
 constexpr float RAISE = 14.0f, START = 5.0f;   // log2 room above the reference
+constexpr uint32_t SHORT = 256;            // cached positions up to which fp16 weights have two parts (see above)
 
 // A part of a unit that is not a warp's alone; cols = 0: none.
 struct Info {
@@ -91,7 +95,7 @@ struct Cfg {
     static constexpr int W = DH / 8;                // words per row
     static constexpr int SETS = DH / 32;            // runs of four words, one per lane of a quad
     static constexpr int MT = DH / 16;              // combine's 16-dim tiles
-    static constexpr int QP = HALF ? 1 : 3, PP = HALF ? 1 : 3;
+    static constexpr int QP = HALF ? 1 : 3;         // fp16 parts of a query
     static constexpr int COLS = PAIR ? 4 : 8 * NT;
     static constexpr int NB = PAIR ? 1 : SUBS;      // blocks whose weights a lane holds
     // One CTA per SM, its warps as many as registers and shared memory allow. (Two
@@ -217,7 +221,7 @@ __global__ void __launch_bounds__(Cfg<T, DH, GROUP, NT, PAIR>::THREADS, 1)
 few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
     using C = Cfg<T, DH, GROUP, NT, PAIR>;
     constexpr int NB = C::NB;
-    constexpr int G = C::G, COLS = C::COLS, QP = C::QP, PP = C::PP, CW = C::CW, THREADS = C::THREADS;
+    constexpr int G = C::G, COLS = C::COLS, QP = C::QP, CW = C::CW, THREADS = C::THREADS;
     constexpr bool HALF = C::HALF;
     constexpr float UNIT = HALF ? 16777216.0f : 1.0f;      // a code in an MMA is c / UNIT, or 16 c / UNIT
     // exponents of the power of two above |vs|: from below what the quantizer
@@ -502,223 +506,230 @@ few_kernel(Attend a, uint32_t most_new, unsigned char* __restrict__ ws) {
 
         // ---- the cached tiles ------------------------------------------------------
         float vlim = pow2(vexp), vinv = pow2(-vexp), vmid = 7.5f * vlim;
-        for (; wstart + k < seg_end; ++k) {
-            const uint32_t s = k % C::NST;
-            asm volatile("cp.async.wait_group %0;" ::"n"(C::NST - 1) : "memory");
-            __syncwarp();
-            const unsigned char* stage = ring + s * C::STAGE;
-            const uint32_t pos0 = (wstart + k - u0) * TP;
-            const uint32_t valid = rq.ctx > pos0 ? rq.ctx - pos0 : 0;
-            if (valid > 0) {
-                float p[NB][NT][4];                      // rows g (0, 1) and g + 8, columns 2t, 2t + 1
-                float vs[NB][2][G], vz[NB][2][G];
-                // scores: blocks and groups are independent chains of MMAs, taken in turn
-                float sacc[SUBS][NT][G][4];
-#pragma unroll
-                for (int b = 0; b < SUBS; ++b)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int i = 0; i < G; ++i)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) sacc[b][nt][i][c] = 0.0f;
-                constexpr int PER = C::SETS / G;           // runs of words per group
-#pragma unroll
-                for (int e = 0; e < PER; ++e)
+        // `weight_parts`: fp16 parts of a weight
+        const auto cached_tiles = [&](auto weight_parts) {
+            constexpr int PP = decltype(weight_parts)::value;
+            for (; wstart + k < seg_end; ++k) {
+                const uint32_t s = k % C::NST;
+                asm volatile("cp.async.wait_group %0;" ::"n"(C::NST - 1) : "memory");
+                __syncwarp();
+                const unsigned char* stage = ring + s * C::STAGE;
+                const uint32_t pos0 = (wstart + k - u0) * TP;
+                const uint32_t valid = rq.ctx > pos0 ? rq.ctx - pos0 : 0;
+                if (valid > 0) {
+                    float p[NB][NT][4];                      // rows g (0, 1) and g + 8, columns 2t, 2t + 1
+                    float vs[NB][2][G], vz[NB][2][G];
+                    // scores: blocks and groups are independent chains of MMAs, taken in turn
+                    float sacc[SUBS][NT][G][4];
 #pragma unroll
                     for (int b = 0; b < SUBS; ++b)
 #pragma unroll
-                        for (int gi = 0; gi < G; ++gi) {
-                            const int u = gi * PER + e;
-                            static_assert(group_of(C::SETS - 1) == G - 1, "runs of a group are consecutive");
-                            const uint32_t* kw = reinterpret_cast<const uint32_t*>(stage + b * C::BLOCK);
-                            const uint32_t wa = kw[g * C::W + word_of(u)], wb = kw[(g + 8) * C::W + word_of(u)];
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const uint32_t f[4] = {nib<HALF>(wa, 2 * i), nib<HALF>(wb, 2 * i), nib<HALF>(wa, 2 * i + 1),
-                                                       nib<HALF>(wb, 2 * i + 1)};
-#pragma unroll
-                                for (int x = 0; x < QP; ++x)
-#pragma unroll
-                                    for (int nt = 0; nt < NT; ++nt)
-                                        mma<HALF>(sacc[b][nt][gi], f, qf[x][nt][u][2 * i], qf[x][nt][u][2 * i + 1]);
-                            }
-                        }
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const unsigned char* st = stage + (PAIR ? t >> 1 : b) * C::BLOCK;
-                    if (PAIR) {
-#pragma unroll
-                        for (int i = 0; i < G; ++i)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) sacc[0][0][i][c] = t < 2 ? sacc[0][0][i][c] : sacc[1][0][i][c];
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int at_pos = (g + 8 * h) * G;
-                        float ks[G], kz[G];
-                        scales_of(reinterpret_cast<const T*>(st + C::KS) + at_pos, ks);
-                        scales_of(reinterpret_cast<const T*>(st + C::KZ) + at_pos, kz);
-                        scales_of(reinterpret_cast<const T*>(st + C::VS) + at_pos, vs[b][h]);
-                        scales_of(reinterpret_cast<const T*>(st + C::VZ) + at_pos, vz[b][h]);
-                        if (!HALF) {                          // the codes' 8
-#pragma unroll
-                            for (int i = 0; i < G; ++i) {
-                                kz[i] = fmaf(8.0f, ks[i], kz[i]);
-                                vz[b][h][i] = fmaf(8.0f, vs[b][h][i], vz[b][h][i]);
-                            }
-                        }
-#pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int c = 0; c < 2; ++c) {
-                                float x = sacc[b][nt][0][2 * h + c] * ks[0], z = -ref[nt][c];
+                            for (int i = 0; i < G; ++i)
 #pragma unroll
-                                for (int i = 0; i < G; ++i) {
-                                    if (i) x = fmaf(sacc[b][nt][i][2 * h + c], ks[i], x);
-                                    z = fmaf(kz[i], qs[nt][c][i], z);
+                                for (int c = 0; c < 4; ++c) sacc[b][nt][i][c] = 0.0f;
+                    constexpr int PER = C::SETS / G;           // runs of words per group
+#pragma unroll
+                    for (int e = 0; e < PER; ++e)
+#pragma unroll
+                        for (int b = 0; b < SUBS; ++b)
+#pragma unroll
+                            for (int gi = 0; gi < G; ++gi) {
+                                const int u = gi * PER + e;
+                                static_assert(group_of(C::SETS - 1) == G - 1, "runs of a group are consecutive");
+                                const uint32_t* kw = reinterpret_cast<const uint32_t*>(stage + b * C::BLOCK);
+                                const uint32_t wa = kw[g * C::W + word_of(u)], wb = kw[(g + 8) * C::W + word_of(u)];
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    const uint32_t f[4] = {nib<HALF>(wa, 2 * i), nib<HALF>(wb, 2 * i), nib<HALF>(wa, 2 * i + 1),
+                                                           nib<HALF>(wb, 2 * i + 1)};
+#pragma unroll
+                                    for (int x = 0; x < QP; ++x)
+#pragma unroll
+                                        for (int nt = 0; nt < NT; ++nt)
+                                            mma<HALF>(sacc[b][nt][gi], f, qf[x][nt][u][2 * i], qf[x][nt][u][2 * i + 1]);
                                 }
-                                p[b][nt][2 * h + c] = fmaf(x, cs[nt][c], z);
                             }
-                    }
-                }
-                if (valid < TP) {
-                    // rows past the length may hold anything
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
+                    for (int b = 0; b < NB; ++b) {
+                        const unsigned char* st = stage + (PAIR ? t >> 1 : b) * C::BLOCK;
+                        if (PAIR) {
+#pragma unroll
+                            for (int i = 0; i < G; ++i)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) sacc[0][0][i][c] = t < 2 ? sacc[0][0][i][c] : sacc[1][0][i][c];
+                        }
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            if ((uint32_t)((PAIR ? t >> 1 : b) * BLK + 8 * h + g) < valid) continue;
+                            const int at_pos = (g + 8 * h) * G;
+                            float ks[G], kz[G];
+                            scales_of(reinterpret_cast<const T*>(st + C::KS) + at_pos, ks);
+                            scales_of(reinterpret_cast<const T*>(st + C::KZ) + at_pos, kz);
+                            scales_of(reinterpret_cast<const T*>(st + C::VS) + at_pos, vs[b][h]);
+                            scales_of(reinterpret_cast<const T*>(st + C::VZ) + at_pos, vz[b][h]);
+                            if (!HALF) {                          // the codes' 8
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) p[b][nt][2 * h] = p[b][nt][2 * h + 1] = -INFINITY;
+                                for (int i = 0; i < G; ++i) {
+                                    kz[i] = fmaf(8.0f, ks[i], kz[i]);
+                                    vz[b][h][i] = fmaf(8.0f, vs[b][h][i], vz[b][h][i]);
+                                }
+                            }
 #pragma unroll
-                            for (int i = 0; i < G; ++i) vs[b][h][i] = vz[b][h][i] = 0.0f;
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) {
+                                    float x = sacc[b][nt][0][2 * h + c] * ks[0], z = -ref[nt][c];
+#pragma unroll
+                                    for (int i = 0; i < G; ++i) {
+                                        if (i) x = fmaf(sacc[b][nt][i][2 * h + c], ks[i], x);
+                                        z = fmaf(kz[i], qs[nt][c][i], z);
+                                    }
+                                    p[b][nt][2 * h + c] = fmaf(x, cs[nt][c], z);
+                                }
                         }
-                }
-                if (bad & (1u << s)) {
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) p[b][nt][c] = NAN;
-                }
-                float top[NT][2], vtop = 0.0f;
-                bool over = false;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        top[nt][c] = fmaxf(p[0][nt][c], p[0][nt][2 + c]);
-                        if (!PAIR) top[nt][c] = fmaxf(top[nt][c], fmaxf(p[NB - 1][nt][c], p[NB - 1][nt][2 + c]));
-                        over |= top[nt][c] > room[nt][c];
                     }
-                if (__any_sync(0xffffffffu, over)) {
+                    if (valid < TP) {
+                        // rows past the length may hold anything
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                if ((uint32_t)((PAIR ? t >> 1 : b) * BLK + 8 * h + g) < valid) continue;
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) p[b][nt][2 * h] = p[b][nt][2 * h + 1] = -INFINITY;
+#pragma unroll
+                                for (int i = 0; i < G; ++i) vs[b][h][i] = vz[b][h][i] = 0.0f;
+                            }
+                    }
+                    if (bad & (1u << s)) {
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) p[b][nt][c] = NAN;
+                    }
+                    float top[NT][2], vtop = 0.0f;
+                    bool over = false;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                            for (int o = 4; o < 32; o <<= 1) top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(0xffffffffu, top[nt][c], o));
-                            const float by = raise(nt, c, top[nt][c]);
-#pragma unroll
-                            for (int b = 0; b < NB; ++b) {
-                                p[b][nt][c] -= by;
-                                p[b][nt][2 + c] -= by;
-                            }
+                            top[nt][c] = fmaxf(p[0][nt][c], p[0][nt][2 + c]);
+                            if (!PAIR) top[nt][c] = fmaxf(top[nt][c], fmaxf(p[NB - 1][nt][c], p[NB - 1][nt][2 + c]));
+                            over |= top[nt][c] > room[nt][c];
                         }
-                }
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int i = 0; i < G; ++i) vtop = fmaxf(vtop, fmaxf(fabsf(vs[b][0][i]), fabsf(vs[b][1][i])));
-                if (__any_sync(0xffffffffu, vtop >= vlim)) {
-                    const int ve = min((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)) >> 23) - 126, VEXP1);
-                    if (ve > vexp) {               // |vs| < 2^ve
-                        const float f = pow2(vexp - ve);
-                        vexp = ve;
-                        vlim = pow2(ve);
-                        vinv = pow2(-ve);
-                        vmid = 7.5f * vlim;
-#pragma unroll
-                        for (int m = 0; m < C::MT; ++m)
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                for (int c = 0; c < 4; ++c) acc[m][nt][c] *= f;
-                    }
-                }
-                uint32_t bf[G][NT][PP][2];
-#pragma unroll
-                for (int b = 0; b < SUBS; ++b) {
-                    if (!PAIR || b == 0) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            p[b][nt][c] = ex2(p[b][nt][c]);
-                            l[nt][c & 1] += p[b][nt][c];
-                        }
-#pragma unroll
-                    for (int i = 0; i < G; ++i)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float sc = vs[b][h][i] * vinv;
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                uint32_t f[PP];
-                                const float w0 = p[b][nt][2 * h] * sc, w1 = p[b][nt][2 * h + 1] * sc;
-                                parts_of<PP>(w0, w1, f);
-#pragma unroll
-                                for (int c = 0; c < 2; ++c) ob[nt][c][i] = fmaf(p[b][nt][2 * h + c], vz[b][h][i], ob[nt][c][i]);
-                                if constexpr (PP == 1) {
-                                    const float2 r = unpack(f[0]);
-                                    ob[nt][0][i] = fmaf(w0 - r.x, vmid, ob[nt][0][i]);
-                                    ob[nt][1][i] = fmaf(w1 - r.y, vmid, ob[nt][1][i]);
-                                }
-#pragma unroll
-                                for (int x = 0; x < PP; ++x) bf[i][nt][x][h] = movmatrix(f[x]);
-                            }
-                        }
-                    }
-                    uint32_t bm[G][NT][PP][2];              // the weights of this block
-#pragma unroll
-                    for (int i = 0; i < G; ++i)
+                    if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int x = 0; x < PP; ++x)
+                            for (int c = 0; c < 2; ++c) {
 #pragma unroll
-                                for (int h = 0; h < 2; ++h) bm[i][nt][x][h] = !PAIR || (g >> 2) == b ? bf[i][nt][x][h] : 0u;
-                    const uint32_t va = v_at + s * C::STAGE + b * C::BLOCK;
+                                for (int o = 4; o < 32; o <<= 1) top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(0xffffffffu, top[nt][c], o));
+                                const float by = raise(nt, c, top[nt][c]);
 #pragma unroll
-                    for (int c2 = 0; c2 < DH / 64; ++c2) {
-                        uint32_t w[4];              // 32 dims at positions 0..7 and 8..15, the next 32
-                        ldsm_trans(va + 32 * c2, w);
-                        uint32_t f[4][4];
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) {
-                            const int c = m >> 1, j = m & 1;
-                            f[m][0] = nib<HALF>(w[2 * c], 2 * j);
-                            f[m][1] = nib<HALF>(w[2 * c], 2 * j + 1);
-                            f[m][2] = nib<HALF>(w[2 * c + 1], 2 * j);
-                            f[m][3] = nib<HALF>(w[2 * c + 1], 2 * j + 1);
-                        }
-#pragma unroll
-                        for (int x = 0; x < PP; ++x)
-#pragma unroll
-                            for (int m = 0; m < 4; ++m) {
-                                const int i = (2 * c2 + (m >> 1)) * 32 / GROUP;
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt)
-                                    mma<HALF>(acc[4 * c2 + m][nt], f[m], bm[i][nt][x][0], bm[i][nt][x][1]);
+                                for (int b = 0; b < NB; ++b) {
+                                    p[b][nt][c] -= by;
+                                    p[b][nt][2 + c] -= by;
+                                }
                             }
                     }
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int i = 0; i < G; ++i) vtop = fmaxf(vtop, fmaxf(fabsf(vs[b][0][i]), fabsf(vs[b][1][i])));
+                    if (__any_sync(0xffffffffu, vtop >= vlim)) {
+                        const int ve = min((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)) >> 23) - 126, VEXP1);
+                        if (ve > vexp) {               // |vs| < 2^ve
+                            const float f = pow2(vexp - ve);
+                            vexp = ve;
+                            vlim = pow2(ve);
+                            vinv = pow2(-ve);
+                            vmid = 7.5f * vlim;
+#pragma unroll
+                            for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                    for (int c = 0; c < 4; ++c) acc[m][nt][c] *= f;
+                        }
+                    }
+                    uint32_t bf[G][NT][PP][2];
+#pragma unroll
+                    for (int b = 0; b < SUBS; ++b) {
+                        if (!PAIR || b == 0) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                p[b][nt][c] = ex2(p[b][nt][c]);
+                                l[nt][c & 1] += p[b][nt][c];
+                            }
+#pragma unroll
+                        for (int i = 0; i < G; ++i)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float sc = vs[b][h][i] * vinv;
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    uint32_t f[PP];
+                                    const float w0 = p[b][nt][2 * h] * sc, w1 = p[b][nt][2 * h + 1] * sc;
+                                    parts_of<PP>(w0, w1, f);
+#pragma unroll
+                                    for (int c = 0; c < 2; ++c) ob[nt][c][i] = fmaf(p[b][nt][2 * h + c], vz[b][h][i], ob[nt][c][i]);
+                                    if constexpr (PP == 1) {
+                                        const float2 r = unpack(f[0]);
+                                        ob[nt][0][i] = fmaf(w0 - r.x, vmid, ob[nt][0][i]);
+                                        ob[nt][1][i] = fmaf(w1 - r.y, vmid, ob[nt][1][i]);
+                                    }
+#pragma unroll
+                                    for (int x = 0; x < PP; ++x) bf[i][nt][x][h] = movmatrix(f[x]);
+                                }
+                            }
+                        }
+                        uint32_t bm[G][NT][PP][2];              // the weights of this block
+#pragma unroll
+                        for (int i = 0; i < G; ++i)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int x = 0; x < PP; ++x)
+#pragma unroll
+                                    for (int h = 0; h < 2; ++h) bm[i][nt][x][h] = !PAIR || (g >> 2) == b ? bf[i][nt][x][h] : 0u;
+                        const uint32_t va = v_at + s * C::STAGE + b * C::BLOCK;
+#pragma unroll
+                        for (int c2 = 0; c2 < DH / 64; ++c2) {
+                            uint32_t w[4];              // 32 dims at positions 0..7 and 8..15, the next 32
+                            ldsm_trans(va + 32 * c2, w);
+                            uint32_t f[4][4];
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) {
+                                const int c = m >> 1, j = m & 1;
+                                f[m][0] = nib<HALF>(w[2 * c], 2 * j);
+                                f[m][1] = nib<HALF>(w[2 * c], 2 * j + 1);
+                                f[m][2] = nib<HALF>(w[2 * c + 1], 2 * j);
+                                f[m][3] = nib<HALF>(w[2 * c + 1], 2 * j + 1);
+                            }
+#pragma unroll
+                            for (int x = 0; x < PP; ++x)
+#pragma unroll
+                                for (int m = 0; m < 4; ++m) {
+                                    const int i = (2 * c2 + (m >> 1)) * 32 / GROUP;
+#pragma unroll
+                                    for (int nt = 0; nt < NT; ++nt)
+                                        mma<HALF>(acc[4 * c2 + m][nt], f[m], bm[i][nt][x][0], bm[i][nt][x][1]);
+                                }
+                        }
+                    }
                 }
+                __syncwarp();
+                fill(k + C::NST);
             }
-            __syncwarp();
-            fill(k + C::NST);
-        }
+        };
+        if constexpr (!HALF) cached_tiles(std::integral_constant<int, 3>{});
+        else if (rq.ctx <= SHORT) cached_tiles(std::integral_constant<int, 2>{});
+        else cached_tiles(std::integral_constant<int, 1>{});
 
         // ---- the part's result -------------------------------------------------------
         const float back = pow2(vexp) * UNIT;

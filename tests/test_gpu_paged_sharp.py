@@ -139,6 +139,21 @@ def test_short_contexts(ctx, new):
     sharp.check(s, s.call(paged))
 
 
+@pytest.mark.parametrize("ctx", [1, 2, 4, 8, 32, 100, 256])
+@pytest.mark.parametrize("new, r, dh", [(1, 4, 128), (1, 8, 64), (4, 4, 128)])
+def test_short_contexts_are_rounded_once(ctx, new, r, dh):
+    """Requests with few tokens and few cached positions: the error is the output's
+    own rounding (root mean squares within a tenth: other roundings of half its size
+    would add an eighth), weights rounded to float16 would add up to two fifths."""
+    own = err = 0.0
+    for seed in range(8):
+        s = Step([ctx] * 4, [new] * 4, 2, r, dh, 64, 16, F16, seed=seed, packed=False)
+        want = sharp.reference(s)[0]
+        err += float((s.call(paged).double() - want).square().sum())
+        own += float((want.half().double() - want).square().sum())
+    assert err <= 1.1 ** 2 * own
+
+
 def test_a_captured_step_over_other_lengths():
     s = Step([700, 300, 90], [3, 1, 40], 2, 4, 128, 64, 16, F16)
     s.call(paged)
