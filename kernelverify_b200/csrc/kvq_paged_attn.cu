@@ -28,18 +28,19 @@ uint32_t grid_for(uint64_t tiles, uint64_t least, uint64_t most) {
 //
 // A request is the few kernel's while its columns (new tokens x shared heads) fit
 // two passes of 16, where the two are even. 32 requests of 8192 cached positions,
-// R = 4, n new tokens each, few / many: n = 1 71 / 219, n = 4 124 / 221, n = 6
-// 195 / 223, n = 8 225 / 225, n = 9 with a third pass 346 / 225; 32 of 1024, n = 8:
-// 53 / 56; one of 131072, n = 8: 123 / 118. 31 of 8192 with two tokens each beside a
-// chunk of 512: 105 / 286 with all of them units of the many kernel.
+// R = 4, n new tokens each, few / many: n = 1 66 / 219, n = 4 116 / 221, n = 6
+// 188 / 222, n = 8 216 / 224, n = 9 with a third pass 301 / 224; 32 of 1024, n = 8:
+// 56 / 58, n = 9 63 / 58; one of 131072, n = 8: 119 / 117, n = 9 152 / 118. 31 of 8192
+// with two tokens each beside a chunk of 512 over 8192: 173 / 353 with all of them units
+// of the many kernel.
 constexpr uint32_t FEW_COLS = 32;
 
-// Columns per pass. Up to four are held once per block of a tile (4 columns: 71
-// against 73 with 8, 32 x 8192). Two tiles of eight save a pass but leave room for
-// 8 warps instead of 12: 16 columns 123 against 136 (32 x 8192, n = 4), 73 against 76
-// (1 x 131072), 45 either way (32 x 8192 of 2 cache heads, R = 16), but 37 against 34
-// (32 x 1024) and 19 against 15 (1 x 32768 of one cache head, R = 16), where a warp
-// has few tiles. 24 columns are three passes of eight (195) or two of sixteen (216).
+// Columns per pass. Up to four are held once per block of a tile (4 columns: 66
+// against 69 with 8, 32 x 8192). Two tiles of eight save a pass but leave room for
+// 8 warps instead of 12: 16 columns 116 against 126 (32 x 8192, n = 4), 66 against 68
+// (1 x 131072, R = 8, n = 2), 43 either way (32 x 8192 of 2 cache heads, R = 16), but 41
+// against 38 (32 x 1024) and 20 against 15 (1 x 32768 of one cache head, R = 16), where a
+// warp has few tiles. 24 columns are three passes of eight (188) or two of sixteen (208).
 uint32_t columns(uint64_t cols, uint64_t row_tiles, uint64_t sms) {
     if (cols <= 4) return 4;
     const uint64_t p8 = (cols + 7) / 8, p16 = (cols + 15) / 16;
@@ -61,8 +62,8 @@ Choice choose(const Attend& a) {
         // one request: the many kernel alone (its bound is what it brings, but for a
         // padded batch), so that no second pair of launches finds nothing to do
         c.few_most = rows == 1 ? 0 : FEW_COLS / a.r;
-        // (8 for R <= 8: against 4 they cost a batch of single tokens 2 us of 107 and save
-        // one of pairs 50 of 162, beside a chunk of 512)
+        // (8 for R <= 8: against 4 they cost 31 single tokens of 8192 2 us of 169 and save as
+        // many pairs 46 of 218, beside a chunk of 512 over 8192)
         c.cols = columns(a.r > 8 ? a.r : 8, row_tiles, sms);
         // units have at most 256 query rows; no CTA for less than two tiles (64 tokens
         // over 512: 21 us, as with one; with four 22, with eight 27)

@@ -26,19 +26,25 @@
 // the softmax is done with the one in front. K and V tiles have the same layout,
 // rows of keys: K is read as a K-major operand, V as an MN-major one.
 //
-// 4096 tokens over 8192 cached ones, 32 heads over 8 of 128: 700 us, 980 TFLOP/s; a
-// first chunk of 8192: 588 us, 935 TFLOP/s; 64 tokens of 64 requests over 8192:
-// 950 TFLOP/s. A step of 64 keys takes 2,200 cycles for both M tiles, of which the
-// tensor pipe is busy for at least 1,024 (1,536 if, as it seems, MMAs 64 columns
-// wide take as long as those of 128: without softmax and dequantizing it comes to
-// 1,470 TFLOP/s), the special-function unit for 1,024 and each scheduler's issue
-// slot for 1,100; what is left is their waiting for one another. Half of the
-// exponentials' share on the FMA pipe, more registers for the softmax and copies
-// further ahead changed nothing.
+// 4096 tokens over 8192 cached ones, 32 heads over 8 of 128: 700 us, 980 TFLOP/s (756
+// in a long run, under the power limit); a first chunk of 8192: 582 us, 945 TFLOP/s
+// (630 to 640); 64 tokens of 64 requests over 8192: 580 us, 950 TFLOP/s (655). A step of
+// 64 keys takes 2,200 cycles for both M tiles, of which the tensor pipe is busy for at
+// least 1,024 (1,536 if, as it seems, MMAs 64 columns wide take as long as those of
+// 128: without softmax and dequantizing it comes to 1,470 TFLOP/s), the special-function
+// unit for 1,024 and each scheduler's issue slot for 1,100; what is left is their waiting
+// for one another, which bounds the kernel. Half of the exponentials' share on the FMA
+// pipe, more registers for the softmax and copies further ahead changed nothing. Steps of
+// 128 keys with one score buffer per query tile fill the tensor memory just as well; they
+// were slower (872 us against 842 for the 4096 tokens) while the maximum still was a pass
+// of its own, and have not been tried since. At 128 registers a thread groups of 128
+// spill 104 bytes, groups of 64 four.
 //
 // Rounded to fp16: the dequantized K and V (as a cache held in fp16 would be)
 // and the weights P; everything else is fp32. P is at most 2^14 and its sum is
-// taken before the rounding.
+// taken before the rounding. (Root mean square error of an output over that of its own
+// rounding, chunks of 64: 1.18 with an empty cache, 1.52 over 16 positions, 1.27 over 256,
+// 1.10 over 1024, 1.02 over 8192.)
 #pragma once
 
 #include <cuda.h>
