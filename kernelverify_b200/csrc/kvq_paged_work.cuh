@@ -4,13 +4,13 @@
 // each a run of key tiles. Only the device knows the lengths, so every CTA
 // makes the running sum of the requests' tiles in shared memory and takes an
 // equal, contiguous share of the whole list: no CTA has more than one share
-// whatever the lengths, and none waits for another. (The few-token kernel's tiles are
-// the cached ones; a unit's own entries come with its first tile and are not counted.) A unit that lies in one
-// share is finished there. Of the others, a CTA leaves at most two partial
-// results -- of the unit that began before its share (slot 0), and of the one
-// that goes on after it (slot 1) -- and the merge kernel joins a unit's parts,
-// which are those of consecutive CTAs, in their order (results do not depend on
-// timing).
+// whatever the lengths, and none waits for another. (The few-token kernel's
+// tiles are the cached ones; a unit's own entries come with its first tile and
+// are not counted.) A unit that lies in one share is finished there. Of the
+// others, a CTA leaves at most two partial results -- of the unit that began
+// before its share (slot 0), and of the one that goes on after it (slot 1) --
+// and the merge kernel joins a unit's parts, which are those of consecutive
+// CTAs, in their order (results do not depend on timing).
 #pragma once
 
 #include <atomic>

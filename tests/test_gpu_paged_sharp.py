@@ -75,6 +75,14 @@ def test_own_entries_of_a_chunk_count_once(new):
         sharp.check(s, s.call(paged))
 
 
+@pytest.mark.parametrize("r", [64, 65, 100, 128, 129, 200])
+@pytest.mark.parametrize("ctx, new", [([300, 5], [1, 1]), ([130, 0, 40], [7, 3, 1]), ([257], [150])])
+def test_many_query_heads(ctx, new, r):
+    """One token, or half of one, to a tile of queries."""
+    s = Step(ctx, new, 1, r, 64, 64, 16, F16)
+    sharp.check(s, s.call(paged))
+
+
 @pytest.mark.parametrize("rows", [600, 4096])
 @pytest.mark.parametrize("new, dtype", [((1, 1), F16), ((0, 3), F16), ((0, 12), F16), ((1, 2), F32)])
 def test_attend_many_requests(rows, new, dtype):
