@@ -353,7 +353,9 @@ int kvq_abi_version(void);
  * page_size, head_dim/group_size], contiguous and 16-byte aligned; page_size
  * is 16, 32, 64 or 128. Slot s is position s % page_size of page s /
  * page_size. Request b's position p is in page block_tables[b * width + p /
- * page_size]. A batch has 1 to 4096 requests (rows).
+ * page_size]. A batch has 1 to 4096 requests (rows). What a call reads on the
+ * device (lengths, offsets, tables, slots) must not change while it runs: its
+ * kernels read it more than once.
  */
 typedef struct kvq_packed {
     const uint32_t* words;
